@@ -7,7 +7,7 @@ compiled with NVRTC and launched through the C ABI in ``include/ae_b200.h``.
 import sys as _sys
 
 from . import attn_engine, core
-from .attn_engine import AttentionEngine, LinearAttentionEngine, OnlineFunc
+from .attn_engine import AttentionEngine, LinearAttentionEngine, OnlineFunc, PagedCache8, PagePlan, plan_pages
 from .core import (CustomIO, SymbolicArray, SymbolicTensor, SymbolScalar, Var, create_block_mask, meta_tensor)
 
 
@@ -21,4 +21,5 @@ def install_reference_aliases():
 
 
 __all__ = ["AttentionEngine", "OnlineFunc", "LinearAttentionEngine", "CustomIO", "SymbolicArray", "SymbolicTensor",
-           "SymbolScalar", "Var", "create_block_mask", "meta_tensor", "install_reference_aliases"]
+           "SymbolScalar", "Var", "create_block_mask", "meta_tensor", "install_reference_aliases", "PagedCache8", "PagePlan",
+           "plan_pages"]

@@ -67,6 +67,7 @@ class H100:
 
 
 _DYN_PROBE = 1024  # sequence length on which a dynamic-shape engine classifies its mask
+MAX_PACKED = 4096  # sequences of a packed call (AE_MAX_SEQ of attn_fwd.cuh)
 MAX_LIST_KV_TILES = 2048  # kv tiles a block list may cover (AE_MAX_KT of attn_fwd.cuh): 262,144 keys
 
 _TORCH_DTYPES = {torch.float16: rt.DTYPE_F16, torch.bfloat16: rt.DTYPE_BF16}
@@ -105,7 +106,7 @@ class _AttnKernels:
     """Compiled kernels of one engine instance."""
 
     def __init__(self, low: LoweredAttention, D: int, DV: int, dtype_tag: int, mask_mode: int, stages: int,
-                 tuned: Optional[dict] = None):
+                 tuned: Optional[dict] = None, packed: bool = False):
         self.low = low
         self.D, self.DV, self.dtype_tag, self.mask_mode, self.stages = D, DV, dtype_tag, mask_mode, stages
         self.tuned = tuned or {}  # tile choices of the backward kernels (attentionengine_b200/tune.py)
@@ -118,8 +119,15 @@ class _AttnKernels:
         # forward over CTA pairs (tcgen05 cta_group::2): for the shapes it is written for, when the tuned entry or
         # AE_B200_FWD_PAIR asks for it
         pair = int(os.environ.get("AE_B200_FWD_PAIR", self.tuned.get("fwd_pair", FWD_PAIR)))
-        self.fwd_pair = bool(pair) and mask_mode in (0, 1, 3) and DV == 128 and D in (64, 128)
-        if self.fwd_pair:
+        self.fwd_pair = bool(pair) and mask_mode in (0, 1, 3) and DV == 128 and D in (64, 128) and not packed
+        if packed:
+            smem += 16 + 4 * MAX_PACKED  # where the CTA is, and the q-tile pairs of every sequence
+            cfg = rt.KernelConfig(kind=rt.KIND_ATTN_PACKED, dtype=dtype_tag, head_dim=D, head_dim_v=DV, threads=384, smem_bytes=smem,
+                                  stages=stages, mask_mode=mask_mode)
+            cfg.reserved[1] = len(low.final_names)
+            self.fwd_src = rt.kernel_source("attn_fwd.cuh", prelude=low.prelude_fwd, defines={"AE_PACKED": 1})
+            self.fwd = rt.compile_module(self.fwd_src, "ae_attn_fwd", cfg)
+        elif self.fwd_pair:
             pstages = int(os.environ.get("AE_B200_FWD_PAIR_STAGES", self.tuned.get("fwd_pair_stages", 5)))
             smem = 128 * D * 2 + pstages * (64 * D * 2 + 128 * 64 * 2) + 512 + 2048 + 1024
             cfg = rt.KernelConfig(kind=rt.KIND_ATTN_FWD_PAIR, dtype=dtype_tag, head_dim=D, head_dim_v=DV, threads=320,
@@ -182,7 +190,10 @@ class AttentionEngine:
     def __init__(self, qkv_meta, custom_fwd_inputs, score_mod, mask_mod, online_func, mask_value="-inf",
                  device=None, backend="tl", tune=False, tune_file="", tune_bwd=False, tune_file_bwd="",
                  infer_mask=True, infer_mask_block_M=128, infer_mask_block_N=128, extern_block_mask=False,
-                 kv_shared=False, tuned_config=None):
+                 kv_shared=False, tuned_config=None, cache_dtype=None, packed=False):
+        """Two keywords beyond the reference.  ``cache_dtype=torch.float8_e4m3fn`` (decode metas, q_len != kv_len): the engine reads a
+        ``PagedCache8`` through ``decode_cache8``.  ``packed=True``: the engine takes sequences of different lengths behind each other
+        through ``prefill_packed``.  Such an engine has that call alone."""
         if backend not in ("tl", "b200"):
             raise NotImplementedError(f"backend={backend!r}: only the B200 back end exists here "
                                       "(the reference's 'cute' sm_90a path is not part of it)")
@@ -209,6 +220,21 @@ class AttentionEngine:
         # shape-class dispatch, as attn_engine.py:218-332
         self._mla = None
         self._decode = None
+        self._decode8 = None
+        self.packed = bool(packed)
+        if packed and (kv_shared or extern_block_mask or cache_dtype is not None):
+            raise NotImplementedError("packed sequences go with neither kv_shared, extern_block_mask nor cache_dtype")
+        if cache_dtype is not None:
+            from .cache8 import E4M3, CacheDecode8
+            if cache_dtype != E4M3:
+                raise NotImplementedError(f"cache_dtype {cache_dtype}: torch.float8_e4m3fn only")
+            if kv_shared or not all(isinstance(x, int) for x in (Hq, Hkv, Sq)) or Sq == Skv:
+                raise NotImplementedError("cache_dtype belongs to decode engines (q_len != kv_len) of MHA and GQA")
+            self._decode8 = CacheDecode8(score_mod, mask_mod, online_func, self.custom_fwd_inputs, Hq, Hkv, Sq, D, DV, self.dtype,
+                                         mask_value)
+            self.tl_code = self._decode8.src
+            self.mask_mode = 0
+            return
         if kv_shared:
             from .mla_decode import MlaDecode
             self._mla = MlaDecode(score_mod, online_func, self.custom_fwd_inputs, Hq, D, DV, self.dtype)
@@ -216,7 +242,7 @@ class AttentionEngine:
             self.mask_mode = 0
             return
         ints = all(isinstance(x, int) for x in (Hq, Hkv, Sq))
-        if ints and Sq != Skv and (isinstance(Skv, str) or not dynamic):
+        if not packed and ints and Sq != Skv and (isinstance(Skv, str) or not dynamic):
             # decode shape classes (reference: attn_engine.py:252-286): split-KV kernel + OnlineFunc.combine.  The KV
             # length (and the batch) may be named dims: a serving loop calls one engine with a growing cache.
             if isinstance(Skv, int) and Sq > Skv:
@@ -246,6 +272,11 @@ class AttentionEngine:
         self._mask_counts = None
         if extern_block_mask:
             mask_mode = 2
+        elif packed and mask_mod is not None:
+            # positions count from the start of each sequence and lengths are the call's: causal bounds, or element by element
+            probe = block_mask_counts(mask_mod, 2, 2, _DYN_PROBE, _DYN_PROBE, "cpu", 128, 128)
+            causal_cnt = block_mask_counts(lambda b, h, q, kv: q >= kv, 1, 1, _DYN_PROBE, _DYN_PROBE, "cpu", 128, 128)
+            mask_mode = 1 if probe.shape[:2] == (1, 1) and torch.equal(probe, causal_cnt) else 3
         elif mask_mod is not None:
             if infer_mask and not dynamic:
                 cnt = block_mask_counts(mask_mod, B, Hq, Sq, Skv, "cpu", 128, 128)
@@ -285,7 +316,9 @@ class AttentionEngine:
                               bf16=self.dtype == torch.bfloat16, mask_mode=mask_mode, stages=stages,
                               mask_value=mask_value)
         self.lowered = low
-        self.kernels = _AttnKernels(low, D, DV, _TORCH_DTYPES[self.dtype], mask_mode, stages, tuned_config)
+        if packed and any(d > 1 for sp in low.custom for d in sp.dim_slots):
+            raise NotImplementedError("custom inputs over positions are not read beside packed sequences: batch and heads only")
+        self.kernels = _AttnKernels(low, D, DV, _TORCH_DTYPES[self.dtype], mask_mode, stages, tuned_config, packed)
         if tuned_config.get("mode") in ("fused", "split"):
             self.bwd_mode = tuned_config["mode"]
         self.tl_code = self.kernels.fwd_src  # name kept from the reference (attn_engine.py:365): generated source
@@ -311,14 +344,14 @@ class AttentionEngine:
 
     @property
     def _status(self):
-        part = self._mla or self._decode
+        part = self._mla or self._decode or self._decode8
         if part is not None:
             return part.status
         return self._plan.status if self._plan is not None else None
 
     @_status.setter
     def _status(self, t):
-        if self._mla is None and self._decode is None:
+        if self._mla is None and self._decode is None and self._decode8 is None:
             self._native_plan().status = t
 
     def _get_status(self, device):
@@ -459,11 +492,64 @@ class AttentionEngine:
             raise NotImplementedError("decode_varlen belongs to decode engines (q_len != kv_len)")
         return self._decode.decode_varlen(q, k, v, cache_seqlens, *custom, block_table=block_table, metadata=metadata)
 
+    def decode_cache8(self, q, cache, block_table, seq_lens, *custom):
+        """Engines built with ``cache_dtype``: ``q`` [B, q_len, Hq, D] against the first ``seq_lens[b]`` keys of each row's pages,
+        ``block_table`` [B, max_pages] and ``seq_lens`` [B] int32 on the GPU, where alone they are read.  Lengths outside the table and
+        pages outside the cache are reported by ``check_status``.  A row without keys gets zeros."""
+        if self._decode8 is None:
+            raise NotImplementedError("decode_cache8 belongs to engines built with cache_dtype=torch.float8_e4m3fn")
+        return self._decode8(q, cache, block_table, seq_lens, *custom)
+
+    def prefill_packed(self, q, k, v, cu_seqlens, *custom):
+        """Engines built with ``packed``: ``q`` [T, Hq, D], ``k`` [T, Hkv, D], ``v`` [T, Hkv, DV] hold sequences behind each other,
+        sequence i at positions ``cu_seqlens[i]`` ... ``cu_seqlens[i + 1] - 1`` (int32 on the GPU, from 0 to T; up to 4096 sequences).  Each
+        attends to itself: masks and score_mod see positions in the sequence, ``b`` is its number.  Forward only."""
+        if not self.packed:
+            raise NotImplementedError("prefill_packed belongs to engines built with packed=True")
+        if self.DV_total != self.DV and v.dim() == 3:
+            if v.shape[-1] != self.DV_total:
+                raise ValueError(f"v has head dim {v.shape[-1]}, engine was built for {self.DV_total}")
+            return torch.cat([self._packed(q, k, v[..., i:i + self.DV], cu_seqlens, custom)
+                              for i in range(0, self.DV_total, self.DV)], dim=-1)
+        return self._packed(q, k, v, cu_seqlens, custom)
+
+    def _packed(self, q, k, v, cu_seqlens, custom):
+        o = rt.host().attn_packed(self._plan or self._native_plan(), q, k, v, cu_seqlens, custom)
+        if o is None:
+            self._refuse_packed(q, k, v, cu_seqlens, custom)
+        return o
+
+    def _refuse_packed(self, q, k, v, cu_seqlens, custom):
+        for name, t in (("q", q), ("k", k), ("v", v)):
+            if not t.is_cuda:
+                raise rt.AeError(f"{name} must be a CUDA tensor: this back end has no CPU path")
+            if t.dtype != self.dtype:
+                raise TypeError(f"{name} has dtype {t.dtype}, engine was built for {self.dtype}")
+            if t.dim() != 3 or t.stride(2) != 1:
+                raise ValueError(f"{name} must be [T, H, D] with a contiguous last dimension")
+            if t.device != q.device:
+                raise ValueError(f"{name} is on {t.device}, q on {q.device}")
+            if t.requires_grad and torch.is_grad_enabled():
+                raise NotImplementedError(f"{name} requires a gradient: packed sequences are forward only")
+        if (q.shape[2], k.shape[2], v.shape[2]) != (self.D, self.D, self.DV) or k.shape[:2] != v.shape[:2] or k.shape[0] != q.shape[0] or \
+                k.shape[1] == 0 or q.shape[1] % k.shape[1] or q.shape[1] == 0:
+            raise ValueError("q / k / v must be [T, Hq, D], [T, Hkv, D], [T, Hkv, DV] with the engine's head dims and Hq a multiple of Hkv")
+        if not cu_seqlens.is_cuda:
+            raise rt.AeError("cu_seqlens must be a CUDA tensor: this back end has no CPU path")
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or not 2 <= cu_seqlens.shape[0] <= MAX_PACKED + 1 or \
+                cu_seqlens.stride(0) != 1 or cu_seqlens.device != q.device:
+            raise ValueError(f"cu_seqlens must be contiguous int32 [sequences + 1] beside q, with 1 to {MAX_PACKED} sequences")
+        if len(custom) != len(self.lowered.custom):
+            raise TypeError(f"expected {len(self.lowered.custom)} custom input(s) {[s.name for s in self.lowered.custom]}, got {len(custom)}")
+        raise ValueError("tensors do not fit this engine")
+
     def _launch_bwd(self, q, k, v, o, d_o, finals, custom, lists=None):
         from .attn_bwd import launch_bwd
         return launch_bwd(self, q, k, v, o, d_o, finals, custom, lists)
 
     def __call__(self, *args, **kargs):
+        if self._decode8 is not None or self.packed:
+            raise NotImplementedError("this engine was built for " + ("prefill_packed" if self.packed else "decode_cache8"))
         if self._mla is not None:
             if len(args) == 2:
                 # mod(q [B, 1, H, 576], kcache [B * S / 64, 64, 1, 576]) -> (out, lse): the call of the reference's

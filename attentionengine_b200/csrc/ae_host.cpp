@@ -342,6 +342,179 @@ py::object attn(const std::shared_ptr<AttnPlan>& plan, py::handle eng, const Ten
   return py::cast(o);
 }
 
+// ---------------------------------------------------------------------------------------------------- packed prompts
+// What the calls below take of custom inputs: values of a batch row (or packed sequence) and head, as many as there are.
+bool row_customs(const std::vector<Custom>& specs, const std::vector<Tensor>& ts, int64_t B, int64_t H) {
+  if (specs.size() != ts.size()) return false;
+  for (size_t i = 0; i < specs.size(); ++i)
+    for (size_t d = 0; d < specs[i].dim_slots.size() && d < (size_t)ts[i].dim(); ++d) {
+      const int slot = specs[i].dim_slots[d];
+      if (slot > 1 || (slot >= 0 && ts[i].size(d) != 1 && ts[i].size(d) < (slot ? H : B))) return false;
+    }
+  return true;
+}
+
+bool good_ints(const Tensor& t, int64_t dim, const Tensor& like) {
+  return t.is_cuda() && t.scalar_type() == at::kInt && t.dim() == dim && t.device() == like.device() &&
+         (dim == 0 || t.size(dim - 1) < 2 || t.stride(dim - 1) == 1);
+}
+
+// o [T, Hq, DV] of sequences behind each other; None when the tensors do not fit.
+py::object attn_packed(const std::shared_ptr<AttnPlan>& plan, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu,
+                       py::handle custom) {
+  const AttnPlan& P = *plan;
+  for (const Tensor* t : {&q, &k, &v})
+    if (!t->is_cuda() || t->scalar_type() != P.dtype || t->dim() != 3 || t->stride(2) != 1 || t->device() != q.device())
+      return py::none();
+  const int64_t T = q.size(0), Hq = q.size(1), Hkv = k.size(1);
+  if (T > 0x7fffffff || q.size(2) != P.D || k.size(2) != P.D || v.size(2) != P.DV || Hkv < 1 || Hq < 1 || Hq % Hkv || k.size(0) != T ||
+      v.size(0) != T || v.size(1) != Hkv || !good_ints(cu, 1, q) || cu.size(0) < 2 || cu.size(0) > 4097)
+    return py::none();
+  std::vector<Tensor> C = tensors_of(custom);
+  if (!row_customs(P.custom, C, cu.size(0) - 1, Hq) || wants_grad({&q, &k, &v}) || needs_function({&q, &k, &v})) return py::none();
+  py::gil_scoped_release nogil;
+  c10::cuda::CUDAGuard guard(q.device());
+  at::AutoGradMode no_grad(false);
+  Tensor o;
+  AeAttnPackedParams p;
+  memset(&p, 0, sizeof p);
+  if (custom_args(P.custom, C, P.dtype, T, T, true, p.custom, p.custom_stride)) {
+    o = at::empty({T, Hq, P.DV}, q.options());
+    if (T > 0) {
+      Tensor finals;
+      if (P.n_final) finals = at::empty({P.n_final, Hq, T}, q.options().dtype(at::kFloat));
+      for (int i = 0; i < P.n_final; ++i) p.final_rowscales[i] = (float*)finals.data_ptr() + i * Hq * T;
+      p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr(); p.o = o.data_ptr();
+      p.cu_seqlens = (const int32_t*)cu.data_ptr();
+      for (int i = 0; i < 2; ++i) {
+        p.q_stride[i] = q.stride(i); p.k_stride[i] = k.stride(i); p.v_stride[i] = v.stride(i); p.o_stride[i] = o.stride(i);
+      }
+      p.n_seq = (int)cu.size(0) - 1; p.T = (int)T; p.Hq = (int)Hq; p.Hkv = (int)Hkv;
+      p.status = word(plan->status_for(q));
+      check(ae_launch_attn_packed(plan->fwd, &p, stream_of(q)), "ae_launch_attn_packed");
+    }
+  }
+  py::gil_scoped_acquire gil;
+  return o.defined() ? py::cast(o) : py::none();
+}
+
+// ---------------------------------------------------------------------------------------------------- paged 8-bit cache
+// (block_table, cu_seqlens, positions, slots, seq_lens, free_head, segments, status), or None.
+py::object plan_pages(uint64_t kernel, const Tensor& old_lens, const Tensor& new_lens, const Tensor& table, const Tensor& free_pages,
+                      const Tensor& free_head, int64_t page_size, int64_t n_tokens) {
+  const int64_t B = old_lens.dim() == 1 ? old_lens.size(0) : 0;
+  if (!good_ints(old_lens, 1, old_lens) || !good_ints(new_lens, 1, old_lens) || !good_ints(table, 2, old_lens) ||
+      !good_ints(free_pages, 1, old_lens) || !good_ints(free_head, 1, old_lens) || B < 1 || B > 4096 || new_lens.size(0) != B ||
+      table.size(0) != B || table.size(1) < 1 || free_head.size(0) != 1 || page_size < 1 || page_size > (1 << 30) ||
+      (page_size & (page_size - 1)) || n_tokens < 0 || n_tokens > 0x7fffffff || free_pages.size(0) > 0x7fffffff)
+    return py::none();
+  const int64_t n_seg = std::min(n_tokens, n_tokens / page_size + 2 * B);
+  py::gil_scoped_release nogil;
+  c10::cuda::CUDAGuard guard(old_lens.device());
+  at::AutoGradMode no_grad(false);
+  const auto ints = old_lens.options();
+  Tensor cu = at::empty({B + 1}, ints), positions = at::empty({n_tokens}, ints), slots = at::empty({n_tokens}, ints.dtype(at::kLong)),
+         lens = at::empty({B}, ints), out = at::empty({2}, ints), segments = at::empty({n_seg, 4}, ints);
+  AePlanPagesParams p;
+  memset(&p, 0, sizeof p);
+  p.old_lens = (const int32_t*)old_lens.data_ptr(); p.new_lens = (const int32_t*)new_lens.data_ptr();
+  p.block_table = (int32_t*)table.data_ptr();
+  p.free_pages = (const int32_t*)free_pages.data_ptr(); p.free_head = (const int32_t*)free_head.data_ptr();
+  p.cu_seqlens = (int32_t*)cu.data_ptr(); p.positions = (int32_t*)positions.data_ptr(); p.slots = (int64_t*)slots.data_ptr();
+  p.seq_lens = (int32_t*)lens.data_ptr(); p.head_out = (int32_t*)out.data_ptr(); p.segments = (int32_t*)segments.data_ptr();
+  p.status = reinterpret_cast<uint32_t*>(p.head_out + 1);
+  p.table_stride = table.stride(0);
+  p.B = (int)B; p.max_pages = (int)table.size(1); p.n_free = (int)free_pages.size(0); p.page_size = (int)page_size;
+  p.n_tokens = (int)n_tokens; p.n_segments = (int)n_seg;
+  check(ae_launch_plan_pages(handle(kernel), &p, stream_of(old_lens)), "ae_launch_plan_pages");
+  Tensor head = out.narrow(0, 0, 1), status = out.narrow(0, 1, 1);
+  py::gil_scoped_acquire gil;
+  return py::make_tuple(table, cu, positions, slots, lens, head, segments, status);
+}
+
+// The tensors of a cache, as PagedCache8 has checked them: codes [pages, page, H, D], scales [pages, H].
+struct Cache8 {
+  Tensor k, v, ks, vs;
+};
+
+void strides_of(const Cache8& c, int64_t (&kst)[3], int64_t (&vst)[3], int64_t& ks, int64_t& vs) {
+  strides3(c.k, kst);
+  strides3(c.v, vst);
+  ks = c.ks.stride(0);
+  vs = c.vs.stride(0);
+}
+
+bool cache8_write(uint64_t kernel, const std::shared_ptr<Cache8>& cache, const Tensor& k, const Tensor& v, const Tensor& segments) {
+  const Cache8& c = *cache;
+  for (const Tensor* t : {&k, &v})
+    if (!t->is_cuda() || (t->scalar_type() != at::kHalf && t->scalar_type() != at::kBFloat16) || t->dim() != 3 || t->stride(2) != 1 ||
+        t->device() != c.k.device() || t->size(1) != c.k.size(2))
+      return false;
+  if (k.scalar_type() != v.scalar_type() || k.size(0) != v.size(0) || k.size(0) > 0x7fffffff || k.size(2) != c.k.size(3) ||
+      v.size(2) != c.v.size(3) || !good_ints(segments, 2, c.k) || segments.size(1) != 4 || (segments.size(0) > 1 && segments.stride(0) != 4) ||
+      segments.size(0) > 0x7fffffff || wants_grad({&k, &v}) || needs_function({&k, &v}))
+    return false;
+  py::gil_scoped_release nogil;
+  c10::cuda::CUDAGuard guard(k.device());
+  AeCache8WriteParams p;
+  memset(&p, 0, sizeof p);
+  p.k = k.data_ptr(); p.v = v.data_ptr();
+  p.k_codes = (uint8_t*)c.k.data_ptr(); p.v_codes = (uint8_t*)c.v.data_ptr();
+  p.k_scale = (float*)c.ks.data_ptr(); p.v_scale = (float*)c.vs.data_ptr();
+  p.segments = (const int32_t*)segments.data_ptr();
+  for (int i = 0; i < 2; ++i) p.k_stride[i] = k.stride(i), p.v_stride[i] = v.stride(i);
+  strides_of(c, p.k_codes_stride, p.v_codes_stride, p.k_scale_stride, p.v_scale_stride);
+  p.n_tokens = (int)k.size(0); p.n_segments = (int)segments.size(0); p.num_pages = (int)c.k.size(0); p.H = (int)c.k.size(2);
+  p.dtype = k.scalar_type() == at::kBFloat16 ? AE_DTYPE_BF16 : AE_DTYPE_F16;
+  check(ae_launch_cache8_write(handle(kernel), &p, stream_of(k)), "ae_launch_cache8_write");
+  return true;
+}
+
+struct Decode8Plan : Plan {
+  void* kernel = nullptr;
+  int Hq = 0, Hkv = 0, Sq = 0, D = 0, DV = 0;
+  std::vector<Custom> custom;
+};
+
+py::object decode8(const std::shared_ptr<Decode8Plan>& plan, const std::shared_ptr<Cache8>& cache, const Tensor& q,
+                   const Tensor& table, const Tensor& lens, py::handle custom) {
+  const Decode8Plan& P = *plan;
+  const Cache8& c = *cache;
+  if (!good4(q, P.dtype) || q.size(1) != P.Sq || q.size(2) != P.Hq || q.size(3) != P.D || q.device() != c.k.device() ||
+      c.k.size(2) != P.Hkv || c.k.size(3) != P.D || c.v.size(3) != P.DV)
+    return py::none();
+  const int64_t B = q.size(0);
+  if (!good_ints(table, 2, q) || table.size(0) != B || table.size(1) < 1 || table.size(1) > 0x7fffffff || !good_ints(lens, 1, q) ||
+      lens.size(0) != B || B > 65535)
+    return py::none();
+  std::vector<Tensor> C = tensors_of(custom);
+  if (!row_customs(P.custom, C, B, P.Hq) || wants_grad({&q}) || needs_function({&q})) return py::none();
+  py::gil_scoped_release nogil;
+  c10::cuda::CUDAGuard guard(q.device());
+  at::AutoGradMode no_grad(false);
+  Tensor o;
+  AeCache8DecodeParams p;
+  memset(&p, 0, sizeof p);
+  if (custom_args(P.custom, C, P.dtype, P.Sq, 0, true, p.custom, p.custom_stride)) {
+    o = at::empty({B, P.Sq, P.Hq, P.DV}, q.options());
+    if (B > 0) {
+      p.q = q.data_ptr(); p.o = o.data_ptr();
+      p.k_codes = (const uint8_t*)c.k.data_ptr(); p.v_codes = (const uint8_t*)c.v.data_ptr();
+      p.k_scale = (const float*)c.ks.data_ptr(); p.v_scale = (const float*)c.vs.data_ptr();
+      p.block_table = (const int32_t*)table.data_ptr(); p.seq_lens = (const int32_t*)lens.data_ptr();
+      strides3(q, p.q_stride);
+      strides_of(c, p.k_codes_stride, p.v_codes_stride, p.k_scale_stride, p.v_scale_stride);
+      p.table_stride = table.stride(0);
+      p.B = (int)B; p.Hq = P.Hq; p.Hkv = P.Hkv; p.Sq = P.Sq; p.max_pages = (int)table.size(1); p.num_pages = (int)c.k.size(0);
+      p.page_size = (int)c.k.size(1);
+      p.status = word(plan->status_for(q));
+      check(ae_launch_cache8_decode(P.kernel, &p, stream_of(q)), "ae_launch_cache8_decode");
+    }
+  }
+  py::gil_scoped_acquire gil;
+  return o.defined() ? py::cast(o) : py::none();
+}
+
 // ---------------------------------------------------------------------------------------------------- split-KV decode
 struct DecodePlan : Plan {
   void *kernel = nullptr, *combine = nullptr;
@@ -998,6 +1171,22 @@ PYBIND11_MODULE(_ae_host, m) {
           AE_HANDLE(ScanPlan, fwd_cut64) AE_HANDLE(ScanPlan, fwd_cut128) AE_HANDLE(ScanPlan, fwd_mods_cut)
       .def_readwrite("segments", &ScanPlan::segments) AE_STATUS(ScanPlan);
   m.def("attn", torch::wrap_pybind_function(&attn));
+  py::class_<Cache8, std::shared_ptr<Cache8>>(m, "Cache8").def(py::init([](Tensor k, Tensor v, Tensor ks, Tensor vs) {
+    return std::make_shared<Cache8>(Cache8{std::move(k), std::move(v), std::move(ks), std::move(vs)});
+  }));
+  py::class_<Decode8Plan, std::shared_ptr<Decode8Plan>>(m, "Decode8Plan")
+      .def(py::init([](uint64_t kernel, bool bf16, int Hq, int Hkv, int Sq, int D, int DV, py::list custom) {
+        auto p = std::make_shared<Decode8Plan>();
+        p->kernel = handle(kernel);
+        p->dtype = bf16 ? at::kBFloat16 : at::kHalf;
+        p->Hq = Hq; p->Hkv = Hkv; p->Sq = Sq; p->D = D; p->DV = DV;
+        p->custom = customs_from(custom);
+        return p;
+      })) AE_STATUS(Decode8Plan);
+  m.def("attn_packed", torch::wrap_pybind_function(&attn_packed));
+  m.def("plan_pages", torch::wrap_pybind_function(&plan_pages));
+  m.def("cache8_write", torch::wrap_pybind_function(&cache8_write));
+  m.def("decode8", torch::wrap_pybind_function(&decode8));
   m.def("decode", torch::wrap_pybind_function(&decode));
   m.def("mla", torch::wrap_pybind_function(&mla));
   m.def("mla_paged", torch::wrap_pybind_function(&mla_paged));

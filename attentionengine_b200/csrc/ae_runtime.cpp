@@ -5,6 +5,7 @@
 #include <dlfcn.h>
 #include <nvrtc.h>
 
+#include <algorithm>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -527,6 +528,172 @@ int ae_launch_attn_fwd(void* module, const AeAttnParams* p, void* stream) {
     return AE_ERR_INVALID;
   }
   return launch(m, (unsigned)ctas, 1, 1, &args, stream);
+}
+
+int ae_launch_attn_packed(void* module, const AeAttnPackedParams* p, void* stream) {
+  if (!module || !p || !p->q || !p->k || !p->v || !p->o || !p->cu_seqlens) return AE_ERR_INVALID;
+  Module* m = (Module*)module;
+  int rc = check_attn_common(m, AE_KIND_ATTN_PACKED, p->n_seq, p->Hq, p->Hkv, p->T, p->T);
+  if (rc) return rc;
+  if (p->n_seq > 4096) {
+    set_error("at most 4096 packed sequences");
+    return AE_ERR_INVALID;
+  }
+  for (int i = 0; i < m->cfg.reserved[1] && i < AE_MAX_FINAL; ++i)
+    if (!p->final_rowscales[i]) return AE_ERR_INVALID;
+  rc = ensure_loaded(m);
+  if (rc) return rc;
+  AeAttnFwdArgs args;
+  memset(&args, 0, sizeof args);
+  const int D = m->cfg.head_dim, DV = m->cfg.head_dim_v;
+  const int64_t qs[3] = {0, p->q_stride[0], p->q_stride[1]}, ks[3] = {0, p->k_stride[0], p->k_stride[1]},
+                vs[3] = {0, p->v_stride[0], p->v_stride[1]};
+  rc = make_bshd_map(&args.tm_q, p->q, m->cfg.dtype, 1, p->T, p->Hq, D, qs, 128);
+  if (rc) return rc;
+  rc = make_bshd_map(&args.tm_k, p->k, m->cfg.dtype, 1, p->T, p->Hkv, D, ks, 128);
+  if (rc) return rc;
+  rc = make_bshd_map(&args.tm_v, p->v, m->cfg.dtype, 1, p->T, p->Hkv, DV, vs, 128);
+  if (rc) return rc;
+  args.o = p->o;
+  args.o_ss = p->o_stride[0];
+  args.o_sh = p->o_stride[1];
+  if ((reinterpret_cast<uintptr_t>(p->o) & 15) || (args.o_ss % 8) || (args.o_sh % 8)) {
+    set_error("output must be 16-byte aligned with strides that are multiples of 8 elements");
+    return AE_ERR_INVALID;
+  }
+  for (int i = 0; i < AE_MAX_FINAL; ++i) args.final_rs[i] = p->final_rowscales[i];
+  for (int i = 0; i < AE_MAX_CUSTOM; ++i) {
+    args.custom[i] = p->custom[i];
+    for (int k = 0; k < 4; ++k) args.custom_st[i][k] = p->custom_stride[i][k];
+  }
+  args.B = p->n_seq;
+  args.Hq = p->Hq;
+  args.Hkv = p->Hkv;
+  args.Sq = args.Skv = p->T;
+  args.cu_seqlens = p->cu_seqlens;
+  args.status = p->status;
+  // no more pairs than this whatever the lengths: a sequence of n positions has at most n / 256 + 1
+  const int64_t pairs = (int64_t)p->T / 256 + std::min(p->n_seq, p->T), ctas = pairs * p->Hq;
+  if (ctas > 0x7fffffff) {
+    set_error("packed attention: too many q tiles for one launch");
+    return AE_ERR_INVALID;
+  }
+  return launch(m, (unsigned)ctas, 1, 1, &args, stream);
+}
+
+static int page_log2_of(int page_size) {
+  for (int i = 0; i < 31; ++i)
+    if (page_size == 1 << i) return i;
+  return -1;
+}
+
+int ae_launch_plan_pages(void* module, const AePlanPagesParams* p, void* stream) {
+  if (!module || !p || !p->old_lens || !p->new_lens || !p->block_table || !p->free_head || !p->cu_seqlens || !p->seq_lens ||
+      !p->head_out || !p->status || (p->n_free > 0 && !p->free_pages))
+    return AE_ERR_INVALID;
+  Module* m = (Module*)module;
+  if (m->cfg.kind != AE_KIND_PLAN_PAGES) {
+    set_error("module kind does not match the entry point");
+    return AE_ERR_UNSUPPORTED;
+  }
+  if (p->n_tokens > 0 && (!p->positions || !p->slots || !p->segments)) return AE_ERR_INVALID;
+  const int log2 = page_log2_of(p->page_size);
+  const int64_t room = std::min<int64_t>(p->n_tokens, (int64_t)p->n_tokens / std::max(p->page_size, 1) + 2 * (int64_t)p->B);
+  if (log2 < 0 || p->B < 1 || p->B > 4096 || p->max_pages < 1 || p->n_free < 0 || p->n_tokens < 0 || p->n_segments < room ||
+      p->free_head == p->head_out || (reinterpret_cast<uintptr_t>(p->segments) & 15)) {
+    set_error("plan_pages: 1 to 4096 rows, a page size that is a power of two, room for min(n_tokens, n_tokens / page_size + 2 B) segments");
+    return AE_ERR_INVALID;
+  }
+  int rc = ensure_loaded(m);
+  if (rc) return rc;
+  AePlanPagesArgs a;
+  memset(&a, 0, sizeof a);
+  a.old_lens = p->old_lens; a.new_lens = p->new_lens; a.table = p->block_table; a.free_pages = p->free_pages;
+  a.free_head = p->free_head; a.cu = p->cu_seqlens; a.positions = p->positions; a.slots = (i64*)p->slots; a.lens = p->seq_lens;
+  a.head_out = p->head_out; a.segments = (AePageSegment*)p->segments; a.status = p->status; a.table_stride = p->table_stride;
+  a.B = p->B; a.max_pages = p->max_pages; a.n_free = p->n_free; a.page_log2 = log2; a.n_tokens = p->n_tokens;
+  a.n_seg = p->n_segments;
+  // two tokens a thread: the sums over the rows that every CTA makes cost more than its tokens
+  const int64_t ctas = std::min<int64_t>(148, std::max<int64_t>(1, ((int64_t)p->n_tokens + 511) / 512));
+  return launch(m, (unsigned)ctas, 1, 1, &a, stream);
+}
+
+int ae_launch_cache8_write(void* module, const AeCache8WriteParams* p, void* stream) {
+  if (!module || !p || !p->k_codes || !p->v_codes || !p->k_scale || !p->v_scale) return AE_ERR_INVALID;
+  Module* m = (Module*)module;
+  if (m->cfg.kind != AE_KIND_CACHE8_WRITE) {
+    set_error("module kind does not match the entry point");
+    return AE_ERR_UNSUPPORTED;
+  }
+  if (p->n_tokens < 0 || p->n_segments < 0 || p->num_pages < 0 || p->H < 1 || p->H > 65535) return AE_ERR_INVALID;
+  if (p->n_tokens == 0 || p->n_segments == 0) return AE_OK;
+  if (!p->k || !p->v || !p->segments) return AE_ERR_INVALID;
+  AeCache8WriteArgs a;
+  memset(&a, 0, sizeof a);
+  a.x[0] = p->k; a.x[1] = p->v;
+  a.codes[0] = p->k_codes; a.codes[1] = p->v_codes;
+  a.scales[0] = p->k_scale; a.scales[1] = p->v_scale;
+  a.segments = (const AePageSegment*)p->segments;
+  const int64_t* xs[2] = {p->k_stride, p->v_stride};
+  const int64_t* cs[2] = {p->k_codes_stride, p->v_codes_stride};
+  bool aligned = (reinterpret_cast<uintptr_t>(p->segments) & 15) == 0;
+  for (int i = 0; i < 2; ++i) {
+    a.x_st[i] = xs[i][0]; a.x_sh[i] = xs[i][1];
+    a.c_sp[i] = cs[i][0]; a.c_st[i] = cs[i][1]; a.c_sh[i] = cs[i][2];
+    aligned = aligned && !((reinterpret_cast<uintptr_t>(a.x[i]) | reinterpret_cast<uintptr_t>(a.codes[i])) & 15) &&
+              !((a.x_st[i] | a.x_sh[i]) & 7) && !((a.c_sp[i] | a.c_st[i] | a.c_sh[i]) & 15);
+  }
+  if (!aligned) {
+    set_error("cache write: keys, values, codes and their strides must be multiples of 16 bytes");
+    return AE_ERR_INVALID;
+  }
+  a.s_sp[0] = p->k_scale_stride; a.s_sp[1] = p->v_scale_stride;
+  a.n_tokens = p->n_tokens; a.num_pages = p->num_pages; a.bf16 = p->dtype == AE_DTYPE_BF16;
+  int rc = ensure_loaded(m);
+  if (rc) return rc;
+  return launch(m, (unsigned)p->n_segments, (unsigned)p->H, 2, &a, stream);
+}
+
+int ae_launch_cache8_decode(void* module, const AeCache8DecodeParams* p, void* stream) {
+  if (!module || !p || !p->q || !p->o || !p->k_codes || !p->v_codes || !p->k_scale || !p->v_scale || !p->block_table || !p->seq_lens)
+    return AE_ERR_INVALID;
+  Module* m = (Module*)module;
+  int rc = check_attn_common(m, AE_KIND_CACHE8_DECODE, p->B, p->Hq, p->Hkv, p->Sq, std::max(p->max_pages, 1));
+  if (rc) return rc;
+  const int gq = p->Hq / p->Hkv;
+  if (gq > 1 && p->Sq != 1) {
+    set_error("decode with grouped query heads takes one query position");
+    return AE_ERR_UNSUPPORTED;
+  }
+  AeCache8DecodeArgs a;
+  memset(&a, 0, sizeof a);
+  a.q = p->q; a.o = p->o; a.k = p->k_codes; a.v = p->v_codes; a.ks = p->k_scale; a.vs = p->v_scale;
+  a.table = p->block_table; a.lens = p->seq_lens;
+  a.q_sb = p->q_stride[0]; a.q_ss = p->q_stride[1]; a.q_sh = p->q_stride[2];
+  a.k_sp = p->k_codes_stride[0]; a.k_st = p->k_codes_stride[1]; a.k_sh = p->k_codes_stride[2];
+  a.v_sp = p->v_codes_stride[0]; a.v_st = p->v_codes_stride[1]; a.v_sh = p->v_codes_stride[2];
+  a.ks_sp = p->k_scale_stride; a.vs_sp = p->v_scale_stride; a.table_stride = p->table_stride;
+  if (((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.o) | reinterpret_cast<uintptr_t>(a.k) |
+        reinterpret_cast<uintptr_t>(a.v)) & 15) ||
+      ((a.q_sb | a.q_ss | a.q_sh) & 7) || ((a.k_sp | a.k_st | a.k_sh | a.v_sp | a.v_st | a.v_sh) & 15)) {
+    set_error("8-bit decode: queries, codes, the output and their strides must be multiples of 16 bytes");
+    return AE_ERR_INVALID;
+  }
+  for (int i = 0; i < AE_MAX_CUSTOM; ++i) {
+    a.custom[i] = p->custom[i];
+    for (int k = 0; k < 4; ++k) a.custom_st[i][k] = p->custom_stride[i][k];
+  }
+  a.B = p->B; a.Hq = p->Hq; a.Hkv = p->Hkv; a.gq = gq; a.rows = gq > 1 ? gq : p->Sq;
+  a.max_pages = p->max_pages; a.num_pages = p->num_pages; a.status = p->status;
+  a.page_log2 = page_log2_of(p->page_size);
+  if (a.page_log2 < 4 || a.page_log2 > 7) {
+    set_error("8-bit decode: pages of 16, 32, 64 or 128 keys");
+    return AE_ERR_INVALID;
+  }
+  rc = ensure_loaded(m);
+  if (rc) return rc;
+  const int rt = m->cfg.reserved[0];  // query rows of a tile
+  return launch(m, (unsigned)((a.rows + rt - 1) / rt), (unsigned)p->Hkv, (unsigned)p->B, &a, stream);
 }
 
 static int fill_bwd_args(Module* m, const AeAttnBwdParams* p, AeAttnBwdArgs* a, int q_rows, int kv_rows) {

@@ -68,6 +68,10 @@ struct AeAttnFwdArgs {
   int n_intervals;
   int* row_info;
   int in_cluster;  // the n_split (2 ... 8) CTAs of a unit are a cluster and merge their partials in it
+  // Packed sequences (the same kernel built with AE_PACKED): q, k, v, o are [T, H, D] as one batch row of Sq = Skv = T positions and
+  // sequence b of B is positions cu_seqlens[b] ... cu_seqlens[b + 1].  One CTA per (q-tile pair, q-head), the pairs of all sequences
+  // found from cu_seqlens.
+  const int* cu_seqlens;  // [B + 1]
 };
 
 // ---- attention backward ------------------------------------------------------------
@@ -243,6 +247,62 @@ struct AeRowScaleArgs {
   const void* g2;
   const float* d;
   float* gs2;
+};
+
+// ---- pages of a step (kernel ae_plan_pages) --------------------------------------------------
+struct alignas(16) AePageSegment {  // a run of new tokens inside one page
+  int page;
+  int slot;    // first slot in the page
+  int token;   // first packed token
+  int tokens;  // 0: nothing
+};
+struct AePlanPagesArgs {
+  const int* old_lens;    // [B] tokens of each row that are in its pages
+  const int* new_lens;    // [B] tokens that come
+  int* table;             // [B, max_pages], row stride table_stride: the new pages are entered
+  const int* free_pages;  // [n_free]
+  const int* free_head;   // [1] how many of free_pages are taken
+  int* cu;                // [B + 1]
+  int* positions;         // [n_tokens]
+  i64* slots;             // [n_tokens]
+  int* lens;              // [B] old + new
+  int* head_out;          // [1]
+  AePageSegment* segments;  // [n_seg]
+  u32* status;            // [1] written
+  i64 table_stride;
+  int B, max_pages, n_free, page_log2, n_tokens, n_seg;
+};
+
+// ---- write into a paged 8-bit cache (kernel ae_cache8_write) ------------------------------------
+struct AeCache8WriteArgs {
+  const void* x[2];       // new keys, values [n_tokens, H, D / DV], 16 bits
+  u8* codes[2];           // [num_pages, page, H, D / DV] e4m3
+  float* scales[2];       // [num_pages, H]
+  const AePageSegment* segments;  // [n_seg]
+  i64 x_st[2], x_sh[2];               // element strides of x: token, head
+  i64 c_sp[2], c_st[2], c_sh[2];      // of codes: page, token, head
+  i64 s_sp[2];                        // of scales: page
+  int n_tokens, num_pages, bf16;
+};
+
+// ---- decode over a paged 8-bit cache (kernel ae_cache8_decode) -----------------------------------
+struct AeCache8DecodeArgs {
+  const void* q;   // [B, Sq, Hq, D] 16 bits
+  void* o;         // [B, Sq, Hq, DV] contiguous
+  const u8* k;     // [num_pages, page, Hkv, D] e4m3
+  const u8* v;
+  const float* ks; // [num_pages, Hkv]
+  const float* vs;
+  const int* table;  // [B, max_pages]
+  const int* lens;   // [B]
+  i64 q_sb, q_ss, q_sh;
+  i64 k_sp, k_st, k_sh, v_sp, v_st, v_sh;
+  i64 ks_sp, vs_sp, table_stride;
+  const void* custom[AE_MAX_CUSTOM];
+  i64 custom_st[AE_MAX_CUSTOM][4];
+  int B, Hq, Hkv, gq, rows;  // gq query heads per kv head; rows of a unit: gq, or with gq == 1 the positions
+  int max_pages, num_pages, page_log2;  // page_log2 4 ... 7
+  u32* status;
 };
 
 // ---- UMMA / TMA probe kernels (bring-up checks, kernel ae_probe) -------------------

@@ -1,0 +1,170 @@
+// Pages of one step of a serving loop, from the rows' lengths: which free pages the rows take, the slot and position of every new
+// token, and the segments (runs of new tokens inside one page) that the write into the cache works on.
+//
+// With P slots a page, have = ceil(old / P) and want = ceil((old + new) / P), row b takes want - have pages, the i-th of them
+// free_pages[head + sum of the earlier rows' needs + i].  Everything else is arithmetic on three running sums over the rows (new
+// tokens, needed pages, segments), so every CTA makes the sums for itself (at most 4096 rows: 16 a thread, two block scans) and then
+// takes its share of the tokens, pages and segments; each finds its row by bisection in shared memory.  One launch, no CTA waits for another,
+// and what a CTA writes into the table no CTA reads: entries below `have` are read, new ones are looked up in free_pages.
+// Latency-bound.
+// Bits of the status word: 1 free pages ran out, 2 a row outgrew the table, 4 more new tokens than n_tokens (the later ones are left out),
+// 8 a negative length (taken as 0).  A token without a page has slot -1 and its segment no tokens.
+// Expects AE_PLAN_ROWS (most rows).
+
+#define AE_PLAN_THREADS 256
+
+struct AePlanSmem {
+  int cu[AE_PLAN_ROWS + 1];     // first new token of each row
+  int take[AE_PLAN_ROWS + 1];   // first needed page
+  int seg[AE_PLAN_ROWS + 1];    // first segment
+  i64 warp_sum[AE_PLAN_THREADS / 32];
+};
+
+// Exclusive sum over the block; `total` is the whole.
+AE_DEVICE i64 ae_block_scan(i64 x, i64* warp_sum, i64& total) {
+  const u32 lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  i64 s = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const i64 y = __shfl_up_sync(0xffffffffu, s, o);
+    if ((int)lane >= o) s += y;
+  }
+  __syncthreads();  // the sums of an earlier scan have been read
+  if (lane == 31) warp_sum[warp] = s;
+  __syncthreads();
+  i64 before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < AE_PLAN_THREADS / 32; ++w) {
+    if (w < (int)warp) before += warp_sum[w];
+    total += warp_sum[w];
+  }
+  return before + s - x;
+}
+
+// The row whose share of a running sum holds item i: the last r with first[r] <= i (rows without a share are passed over).
+AE_DEVICE int ae_row_of(const int* first, int B, int i) {
+  int lo = 0, hi = B;  // first[lo] <= i < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= i)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+extern "C" __global__ void __launch_bounds__(AE_PLAN_THREADS) ae_plan_pages(const __grid_constant__ AePlanPagesArgs a) {
+  extern __shared__ u8 smem_raw[];
+  AePlanSmem& sm = *(AePlanSmem*)smem_raw;
+  const int P = 1 << a.page_log2;
+  const int per = (a.B + AE_PLAN_THREADS - 1) / AE_PLAN_THREADS;  // rows of a thread
+  const int r0 = min((int)threadIdx.x * per, a.B), r1 = min(r0 + per, a.B);
+  u32 bad = 0;
+  auto old_len = [&](int r) { return max(a.old_lens[r], 0); };
+
+  i64 sum = 0, total;
+  for (int r = r0; r < r1; ++r) {
+    const int n = a.new_lens[r];
+    if (n < 0 || a.old_lens[r] < 0) bad |= 8u;
+    sum += max(n, 0);
+  }
+  i64 at = ae_block_scan(sum, sm.warp_sum, total);
+  if (total > a.n_tokens) bad |= 4u;
+  for (int r = r0; r < r1; ++r) {
+    sm.cu[r] = (int)min(at, (i64)a.n_tokens);
+    at += max(a.new_lens[r], 0);
+  }
+  if (threadIdx.x == 0) sm.cu[a.B] = (int)min(total, (i64)a.n_tokens);
+  __syncthreads();
+
+  // pages from `have` to `want`, segments: pages of the table that get a token
+  auto pages = [&](int r, int& have, int& want, int& n_seg, bool& outgrown) {
+    const i64 o = old_len(r), n = sm.cu[r + 1] - sm.cu[r];
+    const i64 h = (o + P - 1) >> a.page_log2, w = (o + n + P - 1) >> a.page_log2;
+    have = (int)min(h, (i64)a.max_pages);
+    want = (int)min(w, (i64)a.max_pages);
+    outgrown = w > a.max_pages;
+    n_seg = n > 0 ? (int)(w - (o >> a.page_log2)) : 0;
+  };
+  i64 need = 0, segs = 0, all_need, all_segs;
+  for (int r = r0; r < r1; ++r) {
+    int have, want, n_seg;
+    bool outgrown;
+    pages(r, have, want, n_seg, outgrown);
+    need += want - have;
+    segs += n_seg;
+    if (outgrown) bad |= 2u;
+  }
+  need = ae_block_scan(need, sm.warp_sum, all_need);
+  segs = ae_block_scan(segs, sm.warp_sum, all_segs);
+  for (int r = r0; r < r1; ++r) {
+    int have, want, n_seg;
+    bool outgrown;
+    pages(r, have, want, n_seg, outgrown);
+    sm.take[r] = (int)need;
+    sm.seg[r] = (int)segs;
+    need += want - have;
+    segs += n_seg;
+  }
+  if (threadIdx.x == 0) {
+    sm.take[a.B] = (int)all_need;
+    sm.seg[a.B] = (int)all_segs;
+  }
+  const i64 head = max(*a.free_head, 0);
+  if (head + all_need > a.n_free) bad |= 1u;
+  bad = (u32)__syncthreads_or(bad & 1u) | (u32)(__syncthreads_or(bad & 2u) ? 2 : 0) | (u32)(__syncthreads_or(bad & 4u) ? 4 : 0) |
+        (u32)(__syncthreads_or(bad & 8u) ? 8 : 0);
+
+  // page i of row r, which may be one that this step takes
+  auto page_of = [&](int r, i64 i) -> int {
+    if (i >= a.max_pages) return -1;
+    const int have = (int)min((i64)((old_len(r) + (i64)P - 1) >> a.page_log2), (i64)a.max_pages);
+    if (i < have) return a.table[(i64)r * a.table_stride + i];
+    const i64 f = head + sm.take[r] + (i - have);
+    return f < a.n_free ? a.free_pages[f] : -1;
+  };
+  const int tid = (int)(blockIdx.x * AE_PLAN_THREADS + threadIdx.x), step = (int)(gridDim.x * AE_PLAN_THREADS);
+  for (int t = tid; t < a.n_tokens; t += step) {
+    if (t >= sm.cu[a.B]) {
+      a.positions[t] = -1;
+      a.slots[t] = -1;
+      continue;
+    }
+    const int r = ae_row_of(sm.cu, a.B, t);
+    const i64 pos = (i64)old_len(r) + (t - sm.cu[r]);
+    const int page = page_of(r, pos >> a.page_log2);
+    a.positions[t] = (int)pos;
+    a.slots[t] = page < 0 ? -1 : ((i64)page << a.page_log2) + (pos & (P - 1));
+  }
+  for (int s = tid; s < a.n_seg; s += step) {
+    AePageSegment e = {0, 0, 0, 0};
+    if (s < all_segs) {
+      const int r = ae_row_of(sm.seg, a.B, s), j = s - sm.seg[r];
+      const i64 o = old_len(r);
+      const int into = (int)(o & (P - 1));
+      const int page = page_of(r, (o >> a.page_log2) + j);
+      if (page >= 0) {
+        e.page = page;
+        e.slot = j == 0 ? into : 0;
+        e.token = sm.cu[r] + (j == 0 ? 0 : j * P - into);
+        e.tokens = min(sm.cu[r + 1], e.token + P - e.slot) - e.token;
+      }
+    }
+    a.segments[s] = e;
+  }
+  for (i64 i = tid; i < all_need; i += step) {
+    const int r = ae_row_of(sm.take, a.B, (int)i);
+    const int have = (int)min((i64)((old_len(r) + (i64)P - 1) >> a.page_log2), (i64)a.max_pages);
+    a.table[(i64)r * a.table_stride + have + (i - sm.take[r])] = head + i < a.n_free ? a.free_pages[head + i] : -1;
+  }
+  for (int r = tid; r <= a.B; r += step) {
+    a.cu[r] = sm.cu[r];
+    if (r < a.B) a.lens[r] = old_len(r) + (sm.cu[r + 1] - sm.cu[r]);
+  }
+  if (tid == 0) {
+    *a.head_out = (int)min(head + all_need, (i64)a.n_free);
+    *a.status = bad;
+  }
+}

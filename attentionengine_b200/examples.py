@@ -6,7 +6,7 @@ import math
 
 import torch
 
-from .attn_engine import AttentionEngine, LinearAttentionEngine, OnlineFunc
+from .attn_engine import AttentionEngine, LinearAttentionEngine, OnlineFunc, PagedCache8, plan_pages
 from .core import CustomIO, SymbolScalar, Var, meta_tensor
 
 
@@ -87,13 +87,13 @@ class OnlineSoftmaxSplit(OnlineSoftmax):
         return (lse - lse_sum).exp()
 
 
-def decode_engine(B, Hq, Hkv, Sq, Skv, D, dtype, scale=None, online=None):
+def decode_engine(B, Hq, Hkv, Sq, Skv, D, dtype, scale=None, online=None, **kw):
     """q_len != kv_len: the split-KV decode path (reference scripts gqa_inference.py / mha_inference.py)."""
     scale = 1.0 / math.sqrt(D) if scale is None else scale
     metas_ = (meta_tensor(B, Hq, Sq, D, dtype=dtype), meta_tensor(B, Hkv, Skv, D, dtype=dtype),
               meta_tensor(B, Hkv, Skv, D, dtype=dtype))
     return AttentionEngine(metas_, CustomIO({}), score_mod=lambda s, c, b, h, q, kv: s * scale, mask_mod=None,
-                           online_func=online if online is not None else OnlineSoftmaxSplit())
+                           online_func=online if online is not None else OnlineSoftmaxSplit(), **kw)
 
 
 def softmax_engine(B, Hq, Hkv, S, D, DV, dtype, causal, scale=None, **kw):
@@ -221,3 +221,50 @@ def retention_engine(B, H, S, D, DV, dtype):
 
     return AttentionEngine(metas(B, H, H, S, D, DV, dtype), CustomIO({"mask": (1, "heads", "seq_len", "seq_len_kv")}),
                            score_mod=score_mod, mask_mod=causal_mask, online_func=OnlineRetention(), mask_value="0")
+
+
+class PagedLayers:
+    """The attention of a server's layers over paged 8-bit caches: ``prompts`` admits a batch of requests of different lengths, ``tokens``
+    takes one more token for each.  The layers share the pages' numbers, so one plan serves a step; nothing is read back."""
+
+    def __init__(self, n_layers, Hq, Hkv, D, dtype, rows, num_pages, page_size, max_len, device="cuda"):
+        self.page_size, self.rows = page_size, rows
+        self.caches = [PagedCache8(num_pages, page_size, Hkv, D, device=device) for _ in range(n_layers)]
+        self.prompt = softmax_engine("B", Hq, Hkv, "S", D, D, dtype, True, packed=True)
+        self.token = decode_engine("B", Hq, Hkv, 1, "S", D, dtype, cache_dtype=torch.float8_e4m3fn)
+        ints = dict(dtype=torch.int32, device=device)
+        self.free, self.head = torch.arange(num_pages, **ints), torch.zeros(1, **ints)
+        self.table, self.lens = torch.zeros(rows, -(-max_len // page_size), **ints), torch.zeros(rows, **ints)
+        self.one = torch.ones(rows, **ints)
+        self.status = torch.zeros(1, **ints)
+
+    def _plan(self, new_lens, n_tokens):
+        plan = plan_pages(self.lens, new_lens, self.table, self.free, self.head, self.page_size, n_tokens)
+        self.lens, self.head = plan.seq_lens, plan.free_head
+        self.status |= plan.status
+        return plan
+
+    def prompts(self, layers, new_lens):
+        """``layers``: (q, k, v) of every layer, [T, heads, D] with the requests' tokens behind each other; returns the layers' outputs."""
+        plan = self._plan(new_lens, layers[0][0].shape[0])
+        out = []
+        for cache, (q, k, v) in zip(self.caches, layers):
+            cache.write(k, v, plan.segments)
+            out.append(self.prompt.prefill_packed(q, k, v, plan.cu_seqlens))
+        return out
+
+    def tokens(self, layers):
+        """``layers``: (q, k, v) of every layer, [rows, heads, D]."""
+        plan = self._plan(self.one, self.rows)
+        out = []
+        for cache, (q, k, v) in zip(self.caches, layers):
+            cache.write(k, v, plan.segments)
+            out.append(self.token.decode_cache8(q.unsqueeze(1), cache, plan.block_table, plan.seq_lens).squeeze(1))
+        return out
+
+    def check(self):
+        """Raise if a step did not fit the pages or a kernel reported something (waits for the GPU)."""
+        if int(self.status.item()):
+            raise ValueError(f"plan_pages reported 0x{int(self.status.item()):x}")
+        self.prompt.check_status()
+        self.token.check_status()

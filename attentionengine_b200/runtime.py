@@ -27,6 +27,7 @@ KIND_ROWSCALE = 11
 KIND_ATTN_BWD_FUSED, KIND_ATTN_BWD_CAST = 12, 13
 KIND_ATTN_FWD_PAIR = 14
 KIND_LINEAR_SEGMENTS = 15
+KIND_ATTN_PACKED, KIND_PLAN_PAGES, KIND_CACHE8_WRITE, KIND_CACHE8_DECODE = 16, 17, 18, 19
 DTYPE_F16, DTYPE_BF16 = 0, 1
 
 
@@ -133,13 +134,44 @@ class LinearBwdParams(C.Structure):
                 ("gasc", C.c_void_p)]
 
 
+class AttnPackedParams(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p), ("cu_seqlens", C.c_void_p),
+                ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2), ("o_stride", C.c_int64 * 2),
+                ("final_rowscales", C.c_void_p * AE_MAX_FINAL), ("custom", C.c_void_p * AE_MAX_CUSTOM),
+                ("custom_stride", (C.c_int64 * 4) * AE_MAX_CUSTOM),
+                ("n_seq", C.c_int32), ("T", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("status", C.c_void_p)]
+
+
+class PlanPagesParams(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("old_lens", "new_lens", "block_table", "free_pages", "free_head", "cu_seqlens", "positions",
+                                          "slots", "seq_lens", "head_out", "segments", "status")] + \
+               [("table_stride", C.c_int64)] + \
+               [(n, C.c_int32) for n in ("B", "max_pages", "n_free", "page_size", "n_tokens", "n_segments")]
+
+
+class Cache8WriteParams(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_codes", "v_codes", "k_scale", "v_scale", "segments")] + \
+               [("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2), ("k_codes_stride", _S3), ("v_codes_stride", _S3),
+                ("k_scale_stride", C.c_int64), ("v_scale_stride", C.c_int64)] + \
+               [(n, C.c_int32) for n in ("n_tokens", "n_segments", "num_pages", "H", "dtype")]
+
+
+class Cache8DecodeParams(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "o", "k_codes", "v_codes", "k_scale", "v_scale", "block_table", "seq_lens")] + \
+               [("q_stride", _S3), ("k_codes_stride", _S3), ("v_codes_stride", _S3), ("k_scale_stride", C.c_int64),
+                ("v_scale_stride", C.c_int64), ("table_stride", C.c_int64), ("custom", C.c_void_p * AE_MAX_CUSTOM),
+                ("custom_stride", (C.c_int64 * 4) * AE_MAX_CUSTOM)] + \
+               [(n, C.c_int32) for n in ("B", "Hq", "Hkv", "Sq", "max_pages", "num_pages", "page_size")] + [("status", C.c_void_p)]
+
+
 _lib = None
 _lib_lock = threading.Lock()
 
 EXPORTS = ["ae_compile", "ae_module_from_cubin", "ae_module_cubin", "ae_query", "ae_release", "ae_strerror",
            "ae_last_error", "ae_launch_attn_fwd", "ae_launch_attn_bwd_prep", "ae_launch_attn_bwd_dq",
            "ae_launch_attn_bwd_dkv", "ae_launch_attn_bwd_fused", "ae_launch_attn_bwd_dq_cast", "ae_launch_probe", "ae_launch_attn_bwd_static_scratch", "ae_launch_mla_decode", "ae_launch_mla_combine", "ae_launch_mla_decode_paged", "ae_launch_attn_decode", "ae_launch_decode_combine", "ae_launch_rowscale", "ae_launch_linear_fwd", "ae_launch_linear_states", "ae_launch_linear_bwd",
-           "ae_launch_linear_segments"]
+           "ae_launch_linear_segments", "ae_launch_attn_packed", "ae_launch_plan_pages", "ae_launch_cache8_write",
+           "ae_launch_cache8_decode"]
 
 
 def lib() -> C.CDLL:
@@ -176,6 +208,10 @@ def lib() -> C.CDLL:
             L.ae_launch_linear_segments.argtypes = [C.c_void_p, C.POINTER(LinearSegParams), C.c_void_p]
             L.ae_launch_linear_states.argtypes = [C.c_void_p, C.POINTER(LinearBwdParams), C.c_void_p]
             L.ae_launch_linear_bwd.argtypes = [C.c_void_p, C.POINTER(LinearBwdParams), C.c_void_p]
+            L.ae_launch_attn_packed.argtypes = [C.c_void_p, C.POINTER(AttnPackedParams), C.c_void_p]
+            L.ae_launch_plan_pages.argtypes = [C.c_void_p, C.POINTER(PlanPagesParams), C.c_void_p]
+            L.ae_launch_cache8_write.argtypes = [C.c_void_p, C.POINTER(Cache8WriteParams), C.c_void_p]
+            L.ae_launch_cache8_decode.argtypes = [C.c_void_p, C.POINTER(Cache8DecodeParams), C.c_void_p]
             L.ae_launch_probe.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
                                           C.c_void_p, C.c_void_p]
             _lib = L

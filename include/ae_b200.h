@@ -60,6 +60,10 @@ enum {
   AE_KIND_ATTN_BWD_CAST = 13,
   AE_KIND_LINEAR_SEGMENTS = 15,
   AE_KIND_ATTN_FWD_PAIR = 14, /* kernel "ae_attn_fwd_pair": launched through ae_launch_attn_fwd */
+  AE_KIND_ATTN_PACKED = 16,   /* kernel "ae_attn_fwd" built for packed sequences */
+  AE_KIND_PLAN_PAGES = 17,
+  AE_KIND_CACHE8_WRITE = 18,
+  AE_KIND_CACHE8_DECODE = 19,
 };
 
 #define AE_MAX_CUSTOM_INPUTS 4
@@ -133,6 +137,89 @@ typedef struct AeAttnParams {
  * "ae_attn_fwd_pair": a cluster of two CTAs per two q tiles on tcgen05 cta_group::2; mask_mode 0, 1 or 3, head_dim_v 128,
  * head_dim 64 or 128, AE_ERR_INVALID otherwise).  Same parameter block and results for both. */
 int ae_launch_attn_fwd(void* module, const AeAttnParams* p, void* stream);
+
+/* ---- packed prompts -------------------------------------------------------------
+ * Sequences of different lengths behind each other: sequence b is positions cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of
+ * every tensor, and attends to itself alone.  cu_seqlens starts at 0 and ends at T; other values set status 0x2000 and are
+ * cut to the tensors.  The lengths are read on the device.  Module kind AE_KIND_ATTN_PACKED. */
+typedef struct AeAttnPackedParams {
+  const void* q;             /* [T, Hq, D]   */
+  const void* k;             /* [T, Hkv, D]  */
+  const void* v;             /* [T, Hkv, DV] */
+  void* o;                   /* [T, Hq, DV]  */
+  const int32_t* cu_seqlens; /* [n_seq + 1] device */
+  int64_t q_stride[2], k_stride[2], v_stride[2], o_stride[2]; /* (position, head) */
+  float* final_rowscales[AE_MAX_FINAL_ROWSCALES];             /* each [Hq, T] fp32 */
+  const void* custom[AE_MAX_CUSTOM_INPUTS];
+  int64_t custom_stride[AE_MAX_CUSTOM_INPUTS][4]; /* over (sequence, h, q, kv); the last two 0 */
+  int32_t n_seq, T, Hq, Hkv;                      /* n_seq: at most 4096 */
+  uint32_t* status;
+} AeAttnPackedParams;
+int ae_launch_attn_packed(void* module, const AeAttnPackedParams* p, void* stream);
+
+/* ---- paged cache of 8-bit floating point ------------------------------------------------
+ * Pages of a step.  Row b of B holds old_lens[b] tokens and gets new_lens[b] more, packed behind each other in n_tokens
+ * positions.  The pages it needs are the next ones of free_pages behind *free_head, in the order of the rows; they are entered
+ * into block_table.  Written: cu_seqlens, positions and slots (page * page_size + offset) of the new tokens, the
+ * rows' new lengths, the new head, and for every page that gets tokens a segment {page, first slot, first token, tokens} (unused
+ * ones all 0; n_segments = min(n_tokens, n_tokens / page_size + 2 B) holds them all).  *status receives 0 or bits: 1 the free pages
+ * ran out, 2 a row outgrew block_table, 4 more than n_tokens new tokens, 8 a negative length; tokens without a page have slot -1 and no segment. */
+typedef struct AePlanPagesParams {
+  const int32_t* old_lens;   /* [B] */
+  const int32_t* new_lens;   /* [B] */
+  int32_t* block_table;      /* [B, max_pages] */
+  const int32_t* free_pages; /* [n_free] */
+  const int32_t* free_head;  /* [1] */
+  int32_t* cu_seqlens;       /* [B + 1] */
+  int32_t* positions;        /* [n_tokens], or null if n_tokens is 0; slots and segments likewise */
+  int64_t* slots;            /* [n_tokens] */
+  int32_t* seq_lens;         /* [B] */
+  int32_t* head_out;         /* [1], not free_head itself */
+  int32_t* segments;         /* [n_segments][4], 16-byte aligned */
+  uint32_t* status;          /* [1] */
+  int64_t table_stride;
+  int32_t B, max_pages, n_free, page_size, n_tokens, n_segments; /* B: at most 4096; page_size: a power of two */
+} AePlanPagesParams;
+int ae_launch_plan_pages(void* module, const AePlanPagesParams* p, void* stream);
+
+/* New keys and values into e4m3 pages, a power-of-two scale for each page and head; a page that goes on keeps its codes, at a
+ * coarser scale where the new tokens need one.  Segments outside the pool or the tokens are passed over.  No two segments of a call
+ * name the same page. */
+typedef struct AeCache8WriteParams {
+  const void* k;           /* [n_tokens, H, D] 16-bit, rows 16-byte aligned  */
+  const void* v;           /* [n_tokens, H, DV] */
+  uint8_t* k_codes;        /* [num_pages, page, H, D] */
+  uint8_t* v_codes;        /* [num_pages, page, H, DV] */
+  float* k_scale;          /* [num_pages, H] */
+  float* v_scale;
+  const int32_t* segments; /* [n_segments][4] */
+  int64_t k_stride[2], v_stride[2];             /* (token, head) */
+  int64_t k_codes_stride[3], v_codes_stride[3]; /* (page, slot, head) */
+  int64_t k_scale_stride, v_scale_stride;       /* (page) */
+  int32_t n_tokens, n_segments, num_pages, H, dtype;
+} AeCache8WriteParams;
+int ae_launch_cache8_write(void* module, const AeCache8WriteParams* p, void* stream);
+
+/* Softmax attention of Sq query positions a row (one with grouped heads) over the row's first seq_lens[b] cached keys.  A length
+ * outside the table is cut to it (status 0x800), a page outside the pool counts as zeros (status 0x1000).  A row without keys gets zeros. */
+typedef struct AeCache8DecodeParams {
+  const void* q;             /* [B, Sq, Hq, D] */
+  void* o;                   /* [B, Sq, Hq, DV] contiguous */
+  const uint8_t* k_codes;    /* [num_pages, page, Hkv, D] */
+  const uint8_t* v_codes;    /* [num_pages, page, Hkv, DV] */
+  const float* k_scale;      /* [num_pages, Hkv], positive */
+  const float* v_scale;
+  const int32_t* block_table; /* [B, max_pages] */
+  const int32_t* seq_lens;    /* [B] */
+  int64_t q_stride[3];        /* (batch, position, head) */
+  int64_t k_codes_stride[3], v_codes_stride[3];
+  int64_t k_scale_stride, v_scale_stride, table_stride;
+  const void* custom[AE_MAX_CUSTOM_INPUTS];
+  int64_t custom_stride[AE_MAX_CUSTOM_INPUTS][4];
+  int32_t B, Hq, Hkv, Sq, max_pages, num_pages, page_size; /* page_size: 16, 32, 64 or 128 */
+  uint32_t* status;
+} AeCache8DecodeParams;
+int ae_launch_cache8_decode(void* module, const AeCache8DecodeParams* p, void* stream);
 
 /* ---- attention backward -----------------------------------------------------------
  * Stands in for `_attention.backward` (attn_tl.py:582-601): `mod_prep(o, dO)` (K2,
