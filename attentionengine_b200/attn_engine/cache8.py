@@ -216,8 +216,6 @@ def is_softmax(online_func) -> bool:
 class CacheDecode8:
     """The 8-bit side of a decode engine: traced ``score_mod`` and ``mask_mod``, softmax rows."""
 
-    WARPS, TILE = 8, 32
-
     def __init__(self, score_mod, mask_mod, online_func, custom_fwd_inputs, Hq, Hkv, Sq, D, DV, dtype, mask_value="-inf"):
         if Hq % Hkv:
             raise ValueError("query heads must be a multiple of kv heads")
@@ -237,20 +235,28 @@ class CacheDecode8:
         if any(d > 1 for sp in self.low.custom for d in sp.dim_slots):
             raise NotImplementedError("custom inputs over positions are not read beside an 8-bit cache: batch and heads only")
         self.rt = 8 if self.rows <= 8 else 16
-        self.kernel = self._build()
-        self.plan = rt.host().Decode8Plan(self.kernel.handle.value, bf16, Hq, Hkv, Sq, D, DV, [(sp.slot, bool(sp.is_16bit), [int(d) for d in sp.dim_slots])
-                                                                     for sp in self.low.custom])
+        self.kernel, self.merge = self._build()
+        customs = [(sp.slot, bool(sp.is_16bit), [int(d) for d in sp.dim_slots]) for sp in self.low.custom]
+        self.plan = rt.host().Decode8Plan(self.kernel.handle.value, self.merge.handle.value, bf16, Hq, Hkv, Sq, D, DV, customs)
 
     def _build(self):
-        T, W = self.TILE, self.WARPS
-        smem = W * T * (self.D + self.DV) + W * self.rt * (self.DV + 2) * 4
+        # 32 keys a tile at 128 dims, 64 at 64: 8 KB; eight warps with three tiles under way each (two where the partials of 16 query rows need
+        # the room) fill an SM's shared memory.  Measured with 64 ragged rows of up to 16384 keys, 128 dims: 6 warps of four tiles 182 us,
+        # 8 of three 158, 12 of two 165, 4 of three 64-key tiles 185 (cp.async; 120 since the copies are a warp's of their own).
+        # A team takes two tiles at least; a unit of up to four tiles a warp is a CTA's (`single`).
+        tile, warps, slots, least, single = 4096 // max(self.D, self.DV), 8, 3 if self.rt == 8 else 2, 2, 4
+        smem = warps * slots * (tile * (self.D + self.DV) + tile // 8 * 4 + 16) + warps * (self.rt * (self.DV + 2) * 4 + 64) + 208 + 1024
         cfg = rt.KernelConfig(kind=rt.KIND_CACHE8_DECODE, dtype=rt.DTYPE_BF16 if self.dtype == torch.bfloat16 else rt.DTYPE_F16,
-                              head_dim=self.D, head_dim_v=self.DV, threads=32 * W, smem_bytes=smem,
+                              head_dim=self.D, head_dim_v=self.DV, threads=32 * warps + 32, smem_bytes=smem, stages=slots,
                               mask_mode=self.low.defines["AE_MASK_MODE"])
-        cfg.reserved[0] = self.rt
-        self.src = rt.kernel_source("cache8_decode.cuh", prelude=self.low.prelude_fwd,
-                                    defines={"AE_RT": self.rt, "AE_T": T, "AE_WARPS": W})
-        return rt.compile_module(self.src, "ae_cache8_decode", cfg)
+        cfg.reserved[0], cfg.reserved[2], cfg.reserved[3], cfg.reserved[4] = self.rt, tile, least, single
+        self.src = rt.kernel_source("cache8_decode.cuh", prelude=self.low.prelude_fwd, defines={
+            "AE_RT": self.rt, "AE_T": tile, "AE_T_LOG2": tile.bit_length() - 1, "AE_WARPS": warps, "AE_C8_SLOTS": slots, "AE_MIN_TILES": least})
+        merge_cfg = rt.KernelConfig(kind=rt.KIND_CACHE8_MERGE, dtype=cfg.dtype, head_dim=self.D, head_dim_v=self.DV, threads=128)
+        merge_cfg.reserved[0] = warps
+        self.merge_src = rt.kernel_source("cache8_merge.cuh", defines={
+            "AE_BF16": int(self.dtype == torch.bfloat16), "AE_DV": self.DV, "AE_RT": self.rt, "AE_WARPS": warps})
+        return rt.compile_module(self.src, "ae_cache8_decode", cfg), rt.compile_module(self.merge_src, "ae_cache8_merge", merge_cfg)
 
     @property
     def status(self):

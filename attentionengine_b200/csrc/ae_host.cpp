@@ -472,6 +472,8 @@ bool cache8_write(uint64_t kernel, const std::shared_ptr<Cache8>& cache, const T
 
 struct Decode8Plan : Plan {
   void* kernel = nullptr;
+  void* merge = nullptr;
+  int64_t workspace = 0;
   int Hq = 0, Hkv = 0, Sq = 0, D = 0, DV = 0;
   std::vector<Custom> custom;
 };
@@ -485,7 +487,7 @@ py::object decode8(const std::shared_ptr<Decode8Plan>& plan, const std::shared_p
     return py::none();
   const int64_t B = q.size(0);
   if (!good_ints(table, 2, q) || table.size(0) != B || table.size(1) < 1 || table.size(1) > 0x7fffffff || !good_ints(lens, 1, q) ||
-      lens.size(0) != B || B > 65535)
+      lens.size(0) != B || B > 16384)
     return py::none();
   std::vector<Tensor> C = tensors_of(custom);
   if (!row_customs(P.custom, C, B, P.Hq) || wants_grad({&q}) || needs_function({&q})) return py::none();
@@ -508,7 +510,11 @@ py::object decode8(const std::shared_ptr<Decode8Plan>& plan, const std::shared_p
       p.B = (int)B; p.Hq = P.Hq; p.Hkv = P.Hkv; p.Sq = P.Sq; p.max_pages = (int)table.size(1); p.num_pages = (int)c.k.size(0);
       p.page_size = (int)c.k.size(1);
       p.status = word(plan->status_for(q));
-      check(ae_launch_cache8_decode(P.kernel, &p, stream_of(q)), "ae_launch_cache8_decode");
+      const Tensor workspace = at::empty({P.workspace}, q.options().dtype(at::kByte));
+      p.workspace = workspace.data_ptr();
+      void* st = stream_of(q);
+      check(ae_launch_cache8_decode(P.kernel, &p, st), "ae_launch_cache8_decode");
+      if (ae_cache8_decode_merges(P.kernel, &p)) check(ae_launch_cache8_merge(P.merge, &p, st), "ae_launch_cache8_merge");
     }
   }
   py::gil_scoped_acquire gil;
@@ -1175,9 +1181,10 @@ PYBIND11_MODULE(_ae_host, m) {
     return std::make_shared<Cache8>(Cache8{std::move(k), std::move(v), std::move(ks), std::move(vs)});
   }));
   py::class_<Decode8Plan, std::shared_ptr<Decode8Plan>>(m, "Decode8Plan")
-      .def(py::init([](uint64_t kernel, bool bf16, int Hq, int Hkv, int Sq, int D, int DV, py::list custom) {
+      .def(py::init([](uint64_t kernel, uint64_t merge, bool bf16, int Hq, int Hkv, int Sq, int D, int DV, py::list custom) {
         auto p = std::make_shared<Decode8Plan>();
-        p->kernel = handle(kernel);
+        p->kernel = handle(kernel); p->merge = handle(merge);
+        p->workspace = ae_cache8_decode_workspace(p->kernel);
         p->dtype = bf16 ? at::kBFloat16 : at::kHalf;
         p->Hq = Hq; p->Hkv = Hkv; p->Sq = Sq; p->D = D; p->DV = DV;
         p->custom = customs_from(custom);

@@ -654,6 +654,74 @@ int ae_launch_cache8_write(void* module, const AeCache8WriteParams* p, void* str
   return launch(m, (unsigned)p->n_segments, (unsigned)p->H, 2, &a, stream);
 }
 
+// One CTA per SM; the table of cut units, then two partials of a row tile for each warp.
+static const int kC8Ctas = 148;
+static int64_t c8_cut_bytes() { return (kC8Ctas * (int64_t)sizeof(AeC8Cut) + 15) / 16 * 16; }
+
+int64_t ae_cache8_decode_workspace(void* module) {
+  const Module* m = (const Module*)module;
+  if (!m || m->cfg.kind != AE_KIND_CACHE8_DECODE) return 0;
+  return c8_cut_bytes() + (int64_t)kC8Ctas * 2 * (m->cfg.threads / 32 - 1) * m->cfg.reserved[0] * (m->cfg.head_dim_v + 2) * 4;
+}
+
+int ae_cache8_decode_merges(void* module, const AeCache8DecodeParams* p) {
+  const Module* m = (const Module*)module;
+  if (!m || !p || m->cfg.kind != AE_KIND_CACHE8_DECODE || p->Hkv < 1) return 1;
+  // few units that cannot be long are a CTA each
+  const int64_t rows = p->Hq > p->Hkv ? p->Hq / p->Hkv : p->Sq, rt = m->cfg.reserved[0], tile = m->cfg.reserved[2];
+  const int64_t units = (int64_t)p->B * p->Hkv * ((rows + rt - 1) / rt);
+  const int64_t tiles = ((int64_t)p->max_pages * p->page_size + tile - 1) / tile;
+  return units > kC8Ctas || tiles > (int64_t)m->cfg.reserved[4] * (m->cfg.threads / 32 - 1);
+}
+
+int ae_launch_cache8_merge(void* module, const AeCache8DecodeParams* p, void* stream) {
+  if (!module || !p || !p->o || !p->workspace || p->Hkv < 1) return AE_ERR_INVALID;
+  Module* m = (Module*)module;
+  if (m->cfg.kind != AE_KIND_CACHE8_MERGE) {
+    set_error("module kind does not match the entry point");
+    return AE_ERR_UNSUPPORTED;
+  }
+  int rc = ensure_loaded(m);
+  if (rc) return rc;
+  AeCache8MergeArgs a;
+  memset(&a, 0, sizeof a);
+  a.o = p->o;
+  a.cuts = (const AeC8Cut*)p->workspace;
+  a.part = (const float*)((const char*)p->workspace + c8_cut_bytes());
+  a.Hq = p->Hq;
+  a.gq = p->Hq / p->Hkv;
+  a.rows = a.gq > 1 ? a.gq : p->Sq;
+  int heads = 1;  // of a unit, at most
+  while (heads < m->cfg.reserved[0] && p->Hkv % (2 * heads) == 0) heads *= 2;
+  return launch_after(m, (unsigned)kC8Ctas, (unsigned)heads, 1, &a, stream);
+}
+
+// Codes [num_pages, page, H, D] seen as (d, slot, h, page): a box is min(page, tile) keys of one head.
+static int make_pages_map(AeTmaDesc* out, const void* base, const AeCache8DecodeParams* p, const int64_t st[3], int D, int tile,
+                          int heads) {
+  Driver& d = driver();
+  bool ok = (reinterpret_cast<uintptr_t>(base) & 15) == 0;
+  const int64_t n[3] = {p->num_pages, p->page_size, p->Hkv};
+  int64_t s[3];
+  for (int i = 0; i < 3; ++i) {
+    s[i] = n[i] > 1 ? st[i] : D;  // the stride of a single one is not used
+    ok = ok && s[i] > 0 && s[i] % 16 == 0 && s[i] < (int64_t)1 << 40;
+  }
+  if (!ok || p->num_pages < 1) {
+    set_error("8-bit decode: codes are 16-byte aligned, their strides positive multiples of 16 bytes below 2^40");
+    return AE_ERR_INVALID;
+  }
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)p->page_size, (cuuint64_t)p->Hkv, (cuuint64_t)p->num_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)s[1], (cuuint64_t)s[2], (cuuint64_t)s[0]};
+  cuuint32_t box[4] = {(cuuint32_t)D, (cuuint32_t)std::min(p->page_size, tile), (cuuint32_t)heads, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  AE_CU(d.cuTensorMapEncodeTiled(reinterpret_cast<CUtensorMap*>(out), CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims,
+                                 strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                 D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE));
+  return AE_OK;
+}
+
 int ae_launch_cache8_decode(void* module, const AeCache8DecodeParams* p, void* stream) {
   if (!module || !p || !p->q || !p->o || !p->k_codes || !p->v_codes || !p->k_scale || !p->v_scale || !p->block_table || !p->seq_lens)
     return AE_ERR_INVALID;
@@ -667,16 +735,13 @@ int ae_launch_cache8_decode(void* module, const AeCache8DecodeParams* p, void* s
   }
   AeCache8DecodeArgs a;
   memset(&a, 0, sizeof a);
-  a.q = p->q; a.o = p->o; a.k = p->k_codes; a.v = p->v_codes; a.ks = p->k_scale; a.vs = p->v_scale;
+  a.q = p->q; a.o = p->o; a.ks = p->k_scale; a.vs = p->v_scale;
   a.table = p->block_table; a.lens = p->seq_lens;
   a.q_sb = p->q_stride[0]; a.q_ss = p->q_stride[1]; a.q_sh = p->q_stride[2];
-  a.k_sp = p->k_codes_stride[0]; a.k_st = p->k_codes_stride[1]; a.k_sh = p->k_codes_stride[2];
-  a.v_sp = p->v_codes_stride[0]; a.v_st = p->v_codes_stride[1]; a.v_sh = p->v_codes_stride[2];
   a.ks_sp = p->k_scale_stride; a.vs_sp = p->v_scale_stride; a.table_stride = p->table_stride;
-  if (((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.o) | reinterpret_cast<uintptr_t>(a.k) |
-        reinterpret_cast<uintptr_t>(a.v)) & 15) ||
-      ((a.q_sb | a.q_ss | a.q_sh) & 7) || ((a.k_sp | a.k_st | a.k_sh | a.v_sp | a.v_st | a.v_sh) & 15)) {
-    set_error("8-bit decode: queries, codes, the output and their strides must be multiples of 16 bytes");
+  if (((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.o)) & 15) ||
+      ((a.q_sb | a.q_ss | a.q_sh) & 7)) {
+    set_error("8-bit decode: queries, their strides and the output must be multiples of 16 bytes");
     return AE_ERR_INVALID;
   }
   for (int i = 0; i < AE_MAX_CUSTOM; ++i) {
@@ -692,8 +757,33 @@ int ae_launch_cache8_decode(void* module, const AeCache8DecodeParams* p, void* s
   }
   rc = ensure_loaded(m);
   if (rc) return rc;
-  const int rt = m->cfg.reserved[0];  // query rows of a tile
-  return launch(m, (unsigned)((a.rows + rt - 1) / rt), (unsigned)p->Hkv, (unsigned)p->B, &a, stream);
+  while ((2 << a.team_log2) <= m->cfg.threads / 32 - 1 && p->Hkv % (2 << a.team_log2) == 0) ++a.team_log2;
+  for (int i = 0; i < 2; ++i) {
+    const int heads = i ? 1 << a.team_log2 : 1;
+    rc = make_pages_map(&a.tm_k[i], p->k_codes, p, p->k_codes_stride, m->cfg.head_dim, m->cfg.reserved[2], heads);
+    if (rc) return rc;
+    rc = make_pages_map(&a.tm_v[i], p->v_codes, p, p->v_codes_stride, m->cfg.head_dim_v, m->cfg.reserved[2], heads);
+    if (rc) return rc;
+  }
+  a.scales16 = !((reinterpret_cast<uintptr_t>(a.ks) | reinterpret_cast<uintptr_t>(a.vs)) & 15) && !((a.ks_sp | a.vs_sp) & 3);
+  const int rt = m->cfg.reserved[0], tile = m->cfg.reserved[2];  // query rows and keys of a tile
+  if (!p->workspace || (reinterpret_cast<uintptr_t>(p->workspace) & 15) || p->B > 16384) {
+    set_error("8-bit decode: a 16-byte aligned workspace, and at most 16384 rows");
+    return AE_ERR_INVALID;
+  }
+  a.cuts = (AeC8Cut*)p->workspace;
+  a.part = (float*)((char*)p->workspace + c8_cut_bytes());
+  a.row_tiles = (a.rows + rt - 1) / rt;
+  // the lengths are the device's: no more CTAs than full rows of the table would fill
+  const int64_t unit_tiles = (int64_t)p->B * std::max<int64_t>(1, ((int64_t)p->max_pages * p->page_size + tile - 1) / tile);
+  const int64_t units = (int64_t)p->Hkv * a.row_tiles, tiles = unit_tiles * units;
+  if (tiles > 0x7fffffff) {
+    set_error("8-bit decode: the block table holds too many keys for one launch");
+    return AE_ERR_INVALID;
+  }
+  a.single = !ae_cache8_decode_merges(m, p);
+  if (a.single) return launch(m, (unsigned)units, (unsigned)p->B, 1, &a, stream);
+  return launch(m, (unsigned)kC8Ctas, 1, 1, &a, stream);
 }
 
 static int fill_bwd_args(Module* m, const AeAttnBwdParams* p, AeAttnBwdArgs* a, int q_rows, int kv_rows) {

@@ -286,23 +286,40 @@ struct AeCache8WriteArgs {
 };
 
 // ---- decode over a paged 8-bit cache (kernel ae_cache8_decode) -----------------------------------
+struct AeC8Cut {  // of CTA c: the unit that begins in it and goes on in the CTAs behind it
+  int parts;       // CTAs that it lies in; 0: there is none
+  int b, h, rt;    // request, first head, row tile
+  int heads;
+};
 struct AeCache8DecodeArgs {
+  // [num_pages, page, Hkv, D] e4m3 seen as (d, slot, h, page), swizzle of D bytes; box {D, min(page, tile), 1, 1}, and with the heads of
+  // the largest team, 1 << team_log2
+  AeTmaDesc tm_k[2];
+  AeTmaDesc tm_v[2];
   const void* q;   // [B, Sq, Hq, D] 16 bits
   void* o;         // [B, Sq, Hq, DV] contiguous
-  const u8* k;     // [num_pages, page, Hkv, D] e4m3
-  const u8* v;
   const float* ks; // [num_pages, Hkv]
   const float* vs;
   const int* table;  // [B, max_pages]
   const int* lens;   // [B]
   i64 q_sb, q_ss, q_sh;
-  i64 k_sp, k_st, k_sh, v_sp, v_st, v_sh;
   i64 ks_sp, vs_sp, table_stride;
   const void* custom[AE_MAX_CUSTOM];
   i64 custom_st[AE_MAX_CUSTOM][4];
   int B, Hq, Hkv, gq, rows;  // gq query heads per kv head; rows of a unit: gq, or with gq == 1 the positions
   int max_pages, num_pages, page_log2;  // page_log2 4 ... 7
+  int row_tiles;   // of a kv head's query rows
+  int single;      // the grid is (heads x row tiles, rows), each CTA a unit of its own
+  int team_log2, scales16;  // scales16: four heads' scales of a page are 16 aligned bytes
+  float* part;     // [grid][2][warps][row tile * (DV + 2)]: the pieces of units that are cut between CTAs
+  AeC8Cut* cuts;   // [grid]
   u32* status;
+};
+struct AeCache8MergeArgs {  // kernel ae_cache8_merge
+  void* o;
+  const float* part;
+  const AeC8Cut* cuts;
+  int Hq, gq, rows;
 };
 
 // ---- UMMA / TMA probe kernels (bring-up checks, kernel ae_probe) -------------------

@@ -4,68 +4,95 @@
 //   s = score_mod(ks (q . k_code)),  p = exp(s - max),  o = sum p vs v_code / sum p
 //
 // Bound by HBM: a key and its value are D + DV bytes for at most 16 query rows (4 flops a byte and row), far below the tensor cores' rate, so
-// what counts is that the bytes come without a pause and that the work per byte is small.  Hence mma.sync on 16 x 8 x 16 tiles (query rows
-// x keys x dims): a warp works for itself, keys stay in the registers that the conversion wrote, scores leave the products in the layout in which
-// P enters the next, and no accumulator takes a trip through TMEM for 8 rows of use in 128.
+// what counts is that the bytes come without a pause and that the work per byte is small.  Hence mma.sync on 16 x 8 x 16 tiles with the
+// keys (and the value dims) as the 16 rows and the query rows as the 8 columns: a warp works for itself, codes go from shared memory through a
+// conversion straight into operand registers, and no accumulator takes a trip through TMEM for 8 used rows in 128.
 //
 // Precision: e4m3 is exact in fp16, so K and V enter the products as they are.  Each query row enters as fp16 times a power of two that
 // brings its largest value to [1, 2): exact for fp16 input, and for bf16 down to 2^-24 of that value.  P is fp16 in [0, 1].  Sums, maxima and the
 // scales are fp32.  The value scale goes into the exponent, p' = 2^(x + log2(vs) - m) with m the maximum of x + log2(vs): no page's values are
 // scaled after the product, and the row sum takes p' / vs.
 //
-// Layout of a warp's tile (AE_T keys, AE_T / 4 = KPT for each of the four lanes t of a quad): column n of score tile j is key
-// KPT (n / 2) + 2 j + n % 2, so lane t's scores of a row are keys KPT t ... KPT t + KPT - 1 in order, all in one page (a page has 16 slots or more):
-// one key scale, one value scale a lane.  The contraction over dims may take them in any order, so lane t takes dims
-// D/4 t ... of a key, whole 16-byte chunks.  Value dims likewise: column n of output tile m is dim DV/8 n + m.
+// Layout of a warp's tile of AE_T keys, lane = 4 g + t: row g + 8 h of score tile i is key 16 i + 8 h + g, so a lane has AE_T / 8 scores
+// each of query rows 2 t and 2 t + 1.  The contraction over dims may take them in any order, so lane t takes dims D/4 t ... of a key, whole
+// 16-byte chunks.  P goes from the accumulators' layout to the operand's by a transpose of 8 x 8 blocks in registers.  Row g + 8 h of output
+// tile m is value dim DV/8 g + 2 m + h: a lane ends with DV/8 dims in order of two query rows.
+//
+// Copies: a ninth warp fetches, a lane for each team of warps (below), a tile's keys and values as TMA boxes: the rows of one page (all of
+// them, or AE_T) of the team's heads, with the swizzle that the reads want.  Page numbers, addresses and barriers are then one lane's instructions
+// (200 of 572 a tile when each warp fetched for itself, 300 with 16-byte cp.async), and a box is large: 16 rows of one head at a time, pages of 16
+// keys took 125 us where pages of 64 took 95.
+//
+// Work split: a team of 1, 2, 4 or 8 warps takes the same tiles of as many neighbouring heads, whose keys lie side by side in a token's row of the
+// pool: read at one time they come out of DRAM as whole rows (722 MB of eight heads' pages took 172 us head by head, without any arithmetic,
+// and 128 us where the heads' pages were apart).  The tiles of all (request, heads, row tile) units stand in one line, which is cut into equal
+// intervals, one for each team of a persistent grid; a warp's next tiles are always under way, across the ends of requests too.  A unit that
+// lies in one interval is written at once.  What is cut is merged from fp32 partials: inside a CTA through shared memory, between CTAs by
+// ae_cache8_merge behind this kernel; the teams are as large as leaves it no more than 16 partials of a unit.  (Merged by the last CTA to arrive
+// instead, the partials of eight heads came to that one CTA in 30 us.)  Every CTA finds its interval from the lengths by itself, so the host needs
+// to know none of them.  Where the table says that few units cannot be long (args.single), each is a CTA's, without a search and a merge.
 //
 // Expects the forward prelude (AE_D, AE_DV, AE_BF16, AE_MASK_MODE 0 or 3, ae_score_mod, ae_mask), AE_RT (8 or 16: query rows of a
-// tile), AE_T, AE_WARPS.
+// tile), AE_T, AE_WARPS, AE_C8_SLOTS, AE_MIN_TILES (of a team).
 
-#define AE_KPT (AE_T / 4)
+#define AE_KPT (AE_T / 8)
+#define AE_NB (AE_RT / 8)      // column blocks: query rows 8 n ... 8 n + 7
 #define AE_KB (AE_T * AE_D)    // bytes of a tile's keys
 #define AE_VB (AE_T * AE_DV)
 #define AE_NEG_INF (-__int_as_float(0x7f800000))
 
-// Byte of 16-byte chunk c of row r in a tile of rows of W bytes.  Written a row's chunks at a time; read by a quarter warp as chunks 2 t (+ 1)
-// or t of two rows (keys), and as neighbouring chunks of the four rows KPT t + i (values): all eight in different banks.
+// Byte of 16-byte chunk c of row r in a tile of rows of W bytes, as TMA's swizzle of that width places it.  Read by a quarter warp as
+// chunks 2 t (+ 1) or t of rows 8 x + g (keys), and as chunks g (or 8-byte halves g) of rows 2 t + e (values): all in different banks.
 template <int W>
 AE_DEVICE u32 ae_c8_at(u32 r, u32 c) {
-  const u32 t = r / AE_KPT & 3u;
-  if constexpr (W == 128) return r * 128 + ((c ^ (t << 1) ^ (r & 1u)) << 4);
-  return (r ^ (t >> 1)) * 64 + ((c ^ ((t & 1u) << 1)) << 4);  // two rows of 64 bytes share the banks
-}
-AE_DEVICE void ae_cp16(u32 dst, const void* src, bool fetch) {  // zeros where `fetch` is false
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(fetch ? 16 : 0) : "memory");
+  if constexpr (W == 128) return r * 128 + ((c ^ (r & 7u)) << 4);
+  return r * 64 + ((c ^ (r >> 1 & 3u)) << 4);
 }
 AE_DEVICE u32 ae_e4m3_f16(u32 w, int half) {  // bytes 0, 1 or 2, 3 as a pair of fp16
-  u32 h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((u16)(half ? w >> 16 : w)));
-  return h;
+  u32 x;
+  if (half)
+    asm("{ .reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, h; }" : "=r"(x) : "r"(w));
+  else
+    asm("{ .reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, l; }" : "=r"(x) : "r"(w));
+  return x;
 }
 AE_DEVICE void ae_mma16816(float (&c)[4], u32 a0, u32 a1, u32 a2, u32 a3, u32 b0, u32 b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+AE_DEVICE u32 ae_transpose8(u32 x) {  // an 8 x 8 block of 16-bit values, row g's columns 2 t, 2 t + 1 in lane 4 g + t
+  u32 y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 
-// One request's query rows of a unit: fragments, running maxima (log2, with the value scale in) and sums, output.
-struct AeC8Rows {
-  u32 q[AE_D / 16][AE_RT / 4];  // [k step][low dims, high dims (of row g), the same of row g + 8]
-  float qs[AE_RT / 8];          // what a product is to be multiplied with
-  float m[AE_RT / 8], l[AE_RT / 8];
-  float o[AE_DV / 8][AE_RT / 4];  // [tile][2 (row / 8) + column]
+// Where the blocks of 16 keys of a head lie in a team's tile: boxes of min(page, AE_T) keys behind each other, in each the heads one after the
+// other.  In rows.
+struct AeC8Blocks {
+  int log2, heads;  // blocks of a box
+  AE_DEVICE int at(int i) const { return ((i >> log2) * heads << log2 | (i & ((1 << log2) - 1))) * 16; }
+  AE_DEVICE int head(int j) const { return j * (16 << log2); }
 };
 
-AE_DEVICE void ae_c8_begin(AeC8Rows& R, const AeCache8DecodeArgs& a, int b, int unit, int row0) {
+// One unit's query rows: operands, running maxima (log2, with the value scale in), sums and output of rows 8 n + 2 t + e.
+struct AeC8Rows {
+  u32 q[AE_NB][AE_D / 16][2];  // of row 8 n + g
+  float qs[AE_NB][2];          // what a product is to be multiplied with
+  float m[AE_NB][2], l[AE_NB][2];
+  float o[AE_NB][AE_DV / 16][4];  // [tile][2 h + e]
+};
+
+AE_DEVICE void ae_c8_begin(AeC8Rows& R, const AeCache8DecodeArgs& a, int b, int head, int row0) {
   const u32 g = lane_id() >> 2, t = lane_id() & 3u;
 #pragma unroll
-  for (int hf = 0; hf < AE_RT / 8; ++hf) {
-    const int r = row0 + (int)g + 8 * hf;
+  for (int n = 0; n < AE_NB; ++n) {
+    const int r = row0 + (int)g + 8 * n;
     u32 w[AE_D / 8];
 #pragma unroll
     for (int i = 0; i < AE_D / 8; ++i) w[i] = 0;
     if (r < a.rows) {
-      const i64 at = a.gq > 1 ? (i64)b * a.q_sb + (i64)(unit * a.gq + r) * a.q_sh : (i64)b * a.q_sb + (i64)r * a.q_ss + (i64)unit * a.q_sh;
+      const i64 at = (i64)b * a.q_sb + (a.gq > 1 ? (i64)(head * a.gq + r) * a.q_sh : (i64)r * a.q_ss + (i64)head * a.q_sh);
       const uint4* src = (const uint4*)((const u16*)a.q + at + t * (AE_D / 4));
 #pragma unroll
       for (int i = 0; i < AE_D / 32; ++i) {
@@ -80,148 +107,460 @@ AE_DEVICE void ae_c8_begin(AeC8Rows& R, const AeCache8DecodeArgs& a, int b, int 
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     u32 e = __float_as_uint(top) >> 23;      // 0: zero or below 2^-126; 255: an infinity, which stays one
     e = e < 1u ? 1u : e > 253u ? 127u : e;
-    const float f = __uint_as_float((254u - e) << 23);
-    R.qs[hf] = __uint_as_float(e << 23);
+    const float f = __uint_as_float((254u - e) << 23), qs = __uint_as_float(e << 23);
 #pragma unroll
-    for (int i = 0; i < AE_D / 8; ++i) R.q[i >> 1][2 * hf + (i & 1)] = pack2<0>(unpack_lo<AE_BF16>(w[i]) * f, unpack_hi<AE_BF16>(w[i]) * f);
-    R.m[hf] = AE_NEG_INF;
-    R.l[hf] = 0.f;
+    for (int i = 0; i < AE_D / 8; ++i) R.q[n][i >> 1][i & 1] = pack2<0>(unpack_lo<AE_BF16>(w[i]) * f, unpack_hi<AE_BF16>(w[i]) * f);
+#pragma unroll
+    for (int e2 = 0; e2 < 2; ++e2) {
+      R.qs[n][e2] = __shfl_sync(0xffffffffu, qs, 4 * (2 * t + e2));
+      R.m[n][e2] = AE_NEG_INF;
+      R.l[n][e2] = 0.f;
+    }
+#pragma unroll
+    for (int m = 0; m < AE_DV / 16; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) R.o[n][m][i] = 0.f;
   }
-#pragma unroll
-  for (int m = 0; m < AE_DV / 8; ++m)
-#pragma unroll
-    for (int i = 0; i < AE_RT / 4; ++i) R.o[m][i] = 0.f;
 }
 
 // The tile's scores, softmax step and P V.  `ks`, `vs`: the scales of the page that this lane's keys lie in; `kv0`: the tile's first key; keys
 // from `len` on are zeros in the tile and do not count.
-AE_DEVICE void ae_c8_tile(AeC8Rows& R, const u8* kt, const u8* vt, int kv0, int len, float ks, float vs, int b, int unit, int row0,
-                          const AeCache8DecodeArgs& a, const AeCustom& cu) {
+// Keys first (`keys`: the raw products), then the rest, each behind its own copy.
+AE_DEVICE void ae_c8_keys(const AeC8Rows& R, const u8* kt, const AeC8Blocks& blk, float (&s)[AE_NB][2][AE_KPT]) {
   const u32 g = lane_id() >> 2, t = lane_id() & 3u;
-  float s[AE_RT / 8][AE_KPT];
+  u32 w[AE_T / 16][2][AE_D / 16];
 #pragma unroll
-  for (int j = 0; j < AE_T / 8; ++j) {
-    float c[4] = {0.f, 0.f, 0.f, 0.f};
-    const u32 r = AE_KPT * (g >> 1) + 2 * j + (g & 1u);
-    u32 w[AE_D / 16];
+  for (int i = 0; i < AE_T / 16; ++i)
 #pragma unroll
-    for (int i = 0; i < AE_D / 64; ++i) {
-      const uint4 x = *(const uint4*)(kt + ae_c8_at<AE_D>(r, t * (AE_D / 64) + i));
-      w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < AE_D / 64; ++j) {
+        const uint4 x = *(const uint4*)(kt + blk.at(i) * AE_D + ae_c8_at<AE_D>(8 * h + g, t * (AE_D / 64) + j));
+        w[i][h][4 * j] = x.x; w[i][h][4 * j + 1] = x.y; w[i][h][4 * j + 2] = x.z; w[i][h][4 * j + 3] = x.w;
+      }
+  float c[AE_T / 16][AE_NB][4];
+#pragma unroll
+  for (int i = 0; i < AE_T / 16; ++i)
+#pragma unroll
+    for (int n = 0; n < AE_NB; ++n) c[i][n][0] = c[i][n][1] = c[i][n][2] = c[i][n][3] = 0.f;
+#pragma unroll
+  for (int k = 0; k < AE_D / 16; ++k)  // the score tiles side by side: products into one of them wait for each other
+#pragma unroll
+    for (int i = 0; i < AE_T / 16; ++i) {
+      u32 x[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        x[h] = ae_e4m3_f16(w[i][h][k], 0);
+        x[2 + h] = ae_e4m3_f16(w[i][h][k], 1);
+      }
+#pragma unroll
+      for (int n = 0; n < AE_NB; ++n) ae_mma16816(c[i][n], x[0], x[1], x[2], x[3], R.q[n][k][0], R.q[n][k][1]);
     }
 #pragma unroll
-    for (int k = 0; k < AE_D / 16; ++k) {
-      if constexpr (AE_RT == 16)
-        ae_mma16816(c, R.q[k][0], R.q[k][AE_RT / 4 - 2], R.q[k][1], R.q[k][AE_RT / 4 - 1], ae_e4m3_f16(w[k], 0), ae_e4m3_f16(w[k], 1));
-      else
-        ae_mma16816(c, R.q[k][0], 0u, R.q[k][1], 0u, ae_e4m3_f16(w[k], 0), ae_e4m3_f16(w[k], 1));
-    }
+  for (int i = 0; i < AE_T / 16; ++i)
 #pragma unroll
-    for (int hf = 0; hf < AE_RT / 8; ++hf) {
-      s[hf][2 * j] = c[2 * hf];
-      s[hf][2 * j + 1] = c[2 * hf + 1];
-    }
+    for (int n = 0; n < AE_NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        s[n][e][2 * i] = c[i][n][e];
+        s[n][e][2 * i + 1] = c[i][n][2 + e];
+      }
+}
+AE_DEVICE void ae_c8_weights(AeC8Rows& R, float (&s)[AE_NB][2][AE_KPT], u32 (&p)[AE_NB][AE_KPT], int kv0, int len, const float* scales, int heads, int b,
+                             int head, int row0, const AeCache8DecodeArgs& a, const AeCustom& cu) {
+  const u32 g = lane_id() >> 2, t = lane_id() & 3u;
+  const int k0 = kv0 + (int)g;
+  float ks[AE_T / 16], lv[AE_T / 16], iv[AE_T / 16];
+#pragma unroll
+  for (int i = 0; i < AE_T / 16; ++i) {
+    const float vs = scales[(AE_T / 16 + i) * heads];
+    ks[i] = scales[i * heads];
+    lv[i] = ae_log2(vs);
+    iv[i] = ae_rcp(vs);
   }
-  const int k0 = kv0 + (int)t * AE_KPT;
-  const float lv = ae_log2(vs), iv = 1.f / vs;
-  float osc[AE_RT / 8];
-  u32 p[AE_RT / 8][AE_KPT / 2];
+  const bool tail = kv0 + AE_T > len;
+  float osc[AE_NB][2];
 #pragma unroll
-  for (int hf = 0; hf < AE_RT / 8; ++hf) {
-    const int r = row0 + (int)g + 8 * hf;
-    const bool valid = r < a.rows;
-    const int h = a.gq > 1 ? unit * a.gq + (valid ? r : 0) : unit, q_idx = a.gq > 1 || !valid ? 0 : r;
-    const float f = R.qs[hf] * ks;
-    float top = AE_NEG_INF;
+  for (int n = 0; n < AE_NB; ++n) {
 #pragma unroll
-    for (int c = 0; c < AE_KPT; ++c) {
-      float x = ae_score_mod(s[hf][c] * f, b, h, q_idx, k0 + c, cu) * AE_LOG2E + lv;
+    for (int e = 0; e < 2; ++e) {
+      const int r = row0 + 8 * n + 2 * (int)t + e;
+      const bool valid = r < a.rows;
+      const int h = a.gq > 1 ? head * a.gq + (valid ? r : 0) : head, q_idx = a.gq > 1 || !valid ? 0 : r;
+      float (&x)[AE_KPT] = s[n][e];
+#pragma unroll
+      for (int c = 0; c < AE_KPT; ++c) {
+        x[c] = fmaf(ae_score_mod(x[c] * (R.qs[n][e] * ks[c / 2]), b, h, q_idx, k0 + 8 * c, cu), AE_LOG2E, lv[c / 2]);
 #if AE_MASK_MODE == 3
-      x = ae_mask(b, h, q_idx, k0 + c) ? x : AE_NEG_INF;
+        x[c] = ae_mask(b, h, q_idx, k0 + 8 * c) ? x[c] : AE_NEG_INF;
 #endif
-      x = k0 + c < len ? x : AE_NEG_INF;
-      s[hf][c] = x;
-      top = fmaxf(top, x);
+      }
+      if (tail) {
+#pragma unroll
+        for (int c = 0; c < AE_KPT; ++c) x[c] = k0 + 8 * c < len ? x[c] : AE_NEG_INF;
+      }
+      float top = x[0];
+#pragma unroll
+      for (int c = 1; c < AE_KPT; ++c) top = fmaxf(top, x[c]);
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float m = fmaxf(R.m[n][e], top), mu = m == AE_NEG_INF ? 0.f : m;  // nothing kept so far: p = 0
+      osc[n][e] = ae_exp2(R.m[n][e] - mu);
+      R.m[n][e] = m;
+      float l = R.l[n][e] * osc[n][e];  // this lane's keys; the lanes are added at the end
+#pragma unroll
+      for (int c = 0; c < AE_KPT; ++c) {
+        x[c] = ae_exp2(x[c] - mu);
+        l = fmaf(x[c], iv[c / 2], l);
+      }
+      R.l[n][e] = l;
     }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const float m = fmaxf(R.m[hf], top), mu = m == AE_NEG_INF ? 0.f : m;  // nothing kept so far: p = 0
-    osc[hf] = ae_exp2(R.m[hf] - mu);
-    R.m[hf] = m;
-    float sum = 0.f;
 #pragma unroll
-    for (int c = 0; c < AE_KPT; c += 2) {
-      const float x = ae_exp2(s[hf][c] - mu), y = ae_exp2(s[hf][c + 1] - mu);
-      sum += x + y;
-      p[hf][c / 2] = pack2<0>(x, y);
-    }
-    R.l[hf] = R.l[hf] * osc[hf] + sum * iv;  // this lane's keys; the quad's lanes are added at the end
+    for (int c = 0; c < AE_KPT; ++c) p[n][c] = ae_transpose8(pack2<0>(s[n][0][c], s[n][1][c]));
   }
-  if (__any_sync(0xffffffffu, osc[0] != 1.f || osc[AE_RT / 8 - 1] != 1.f)) {
+  bool grown = false;
 #pragma unroll
-    for (int m = 0; m < AE_DV / 8; ++m)
+  for (int n = 0; n < AE_NB; ++n) grown |= osc[n][0] != 1.f || osc[n][1] != 1.f;
+  if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-      for (int i = 0; i < AE_RT / 4; ++i) R.o[m][i] *= osc[i >> 1];
+    for (int n = 0; n < AE_NB; ++n)
+#pragma unroll
+      for (int m = 0; m < AE_DV / 16; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) R.o[n][m][i] *= osc[n][i & 1];
   }
+}
+AE_DEVICE void ae_c8_values(AeC8Rows& R, const u8* vt, const AeC8Blocks& blk, const u32 (&p)[AE_NB][AE_KPT]) {
+  const u32 g = lane_id() >> 2, t = lane_id() & 3u;
 #pragma unroll
   for (int k = 0; k < AE_T / 16; ++k) {
     constexpr int NW = AE_DV / 32;  // words of a key's values that this lane takes
-    u32 w[4][NW];
+    u32 w[4][NW];                   // keys 16 k + 2 t, the next, and 8 further on
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const u32 r = AE_KPT * t + 4 * k + i;
       if constexpr (AE_DV == 128) {
-        const uint4 x = *(const uint4*)(vt + ae_c8_at<AE_DV>(r, g));
+        const uint4 x = *(const uint4*)(vt + blk.at(k) * AE_DV + ae_c8_at<AE_DV>(8 * (i >> 1) + 2 * t + (i & 1), g));
         w[i][0] = x.x; w[i][1] = x.y; w[i][NW - 2] = x.z; w[i][NW - 1] = x.w;
-      } else {
-        const uint2 x = *(const uint2*)(vt + ae_c8_at<AE_DV>(r, g >> 1) + (g & 1u) * 8);
+      } else {  // odd t the other way round: two rows of 64 bytes share the banks
+        const uint2 x = *(const uint2*)(vt + blk.at(k) * AE_DV + ae_c8_at<AE_DV>(8 * (i >> 1) + 2 * t + ((i ^ t) & 1u), g >> 1) + (g & 1u) * 8);
         w[i][0] = x.x; w[i][1] = x.y;
       }
     }
+    const bool turned = AE_DV == 64 && (t & 1u);
 #pragma unroll
-    for (int n = 0; n < NW; ++n) {
+    for (int m = 0; m < AE_DV / 16; ++m) {  // two value dims of two keys in a word
+      const u32 sel = (m & 1) ? (turned ? 0x3726 : 0x7362) : (turned ? 0x1504 : 0x5140);
+      const u32 lo = __byte_perm(w[0][m / 2], w[1][m / 2], sel), hi = __byte_perm(w[2][m / 2], w[3][m / 2], sel);
+      const u32 x0 = ae_e4m3_f16(lo, 0), x1 = ae_e4m3_f16(lo, 1), x2 = ae_e4m3_f16(hi, 0), x3 = ae_e4m3_f16(hi, 1);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {  // two value dims of two keys in a word
-        const u32 b0 = __byte_perm(w[0][n], w[1][n], e ? 0x7362 : 0x5140), b1 = __byte_perm(w[2][n], w[3][n], e ? 0x7362 : 0x5140);
-#pragma unroll
-        for (int d = 0; d < 2; ++d) {
-          float (&o)[AE_RT / 4] = R.o[4 * n + 2 * e + d];
-          float c[4] = {o[0], o[1], AE_RT == 16 ? o[AE_RT / 4 - 2] : 0.f, AE_RT == 16 ? o[AE_RT / 4 - 1] : 0.f};
-          ae_mma16816(c, p[0][2 * k], AE_RT == 16 ? p[AE_RT / 8 - 1][2 * k] : 0u, p[0][2 * k + 1], AE_RT == 16 ? p[AE_RT / 8 - 1][2 * k + 1] : 0u,
-                      ae_e4m3_f16(b0, d), ae_e4m3_f16(b1, d));
-#pragma unroll
-          for (int i = 0; i < AE_RT / 4; ++i) o[i] = c[i];
-        }
-      }
+      for (int n = 0; n < AE_NB; ++n) ae_mma16816(R.o[n][m], x0, x1, x2, x3, p[n][2 * k], p[n][2 * k + 1]);
     }
   }
 }
 
-// A tile into shared memory: keys kv0 ... of the row, zeros from `len` on.  `page`: lane l holds the page of keys kv0 + 16 l ...
-template <int W>
-AE_DEVICE void ae_c8_fetch(u8* dst, const u8* pool, i64 sp, i64 st, int page_log2, int kv0, int len, int page) {
-  constexpr int CPR = W / 16, RPI = 32 / CPR;  // chunks of a row, rows of an instruction
-  const int c = (int)lane_id() % CPR, rr = (int)lane_id() / CPR;
+#define AE_SLB (AE_KB + AE_VB)  // a slot of the ring: a tile's keys and its values
+#define AE_SCF (AE_T / 8)        // and their scales
+#define AE_REC (AE_RT * (AE_DV + 2))  // floats of a partial: output, maxima, sums
+#define AE_C8_THREADS (AE_WARPS * 32 + 32)
+#define AE_SMEM_HEAD (AE_WARPS * AE_C8_SLOTS * AE_SLB)
+#define AE_SMEM_SCALE (AE_SMEM_HEAD + AE_WARPS * AE_REC * 4)
+#define AE_SMEM_INFO (AE_SMEM_SCALE + AE_WARPS * AE_C8_SLOTS * AE_SCF * 4)
+static_assert(AE_C8_SLOTS * AE_SLB >= AE_REC * 4, "a warp's last partial lies in its own slots");
+
+// A place in the line of tiles: request, heads, row tile, tile; the request's tiles and keys.
+struct AeC8Pos {
+  int b, h, rt, t, nt, len;  // h: heads of the team's size
+};
+struct AeC8Record {  // a cut piece
+  int b, h, rt;      // b = -1: none
+  int begin;         // the unit's first tile in the line
+  int from, to, nt;  // tiles of the unit in this piece, and of the whole
+  int pad;
+};
+#define AE_FEW 47
+struct AeC8Info {
+  u64 full[AE_WARPS][AE_C8_SLOTS], empty[AE_WARPS][AE_C8_SLOTS];  // of each team
+  AeC8Record rec[2 * AE_WARPS];  // of each team: the piece it began with (if it was begun before), the piece it ended in (if it goes on)
+  int longest, pad;
+  int before[AE_FEW + 1];  // tiles of one head's row tile in front of each of a few rows (of more: where the tiles will be)
+  AeCtaCtl ctl;
+};
+
+AE_DEVICE int ae_c8_len(const AeCache8DecodeArgs& a, int b) {
+  const i64 want = a.lens[b], most = (i64)a.max_pages << a.page_log2;
+  return (int)(want < 0 ? 0 : want > most ? most : want);
+}
+AE_DEVICE int ae_c8_tiles(int len) { return len > AE_T ? (len + AE_T - 1) / AE_T : 1; }  // a row without keys has its zeros to write
+
+AE_DEVICE void ae_c8_next(AeC8Pos& p, const AeCache8DecodeArgs& a, int team_log2) {
+  if (++p.t < p.nt) return;
+  p.t = 0;
+  if (++p.rt < a.row_tiles) return;
+  p.rt = 0;
+  if (++p.h < a.Hkv >> team_log2) return;
+  p.h = 0;
+  if (++p.b >= a.B) return;  // behind the last tile: not used
+  p.len = ae_c8_len(a, p.b);
+  p.nt = ae_c8_tiles(p.len);
+}
+
+AE_DEVICE bool ae_c8_test(u64* bar, u32 parity) {
+  u32 ok;
+  asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+               : "=r"(ok)
+               : "r"(smem_u32(bar)), "r"(parity)
+               : "memory");
+  return ok != 0;
+}
+AE_DEVICE void ae_cp4(u32 dst, const float* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
+AE_DEVICE void ae_cp16(u32 dst, const float* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+
+// The fetching warp: a lane for each team, whose interval is [n, n1) and begins at `p`.
+AE_DEVICE void ae_c8_fetch(const AeCache8DecodeArgs& a, u8* ring, float* scales, u64* full, u64* empty, AeC8Pos p, int n, int n1, int tl,
+                           const AeC8Blocks blk, AeCtaCtl* ctl) {
+  const int heads = 1 << tl, box = 16 << blk.log2;  // keys of a copy
+  const bool together = tl == a.team_log2;          // the team's heads are one box
+  int page[AE_T / 16];                              // of keys 16 i ... of the next tile
+  auto pages = [&]() {
+    const int* const row = a.table + (i64)p.b * a.table_stride;
 #pragma unroll
-  for (int i = 0; i < AE_T / RPI; ++i) {
-    const int r = i * RPI + rr;
-    const int pg = __shfl_sync(0xffffffffu, page, i * RPI / 16);
-    const i64 at = (i64)pg * sp + (i64)((kv0 + r) & ((1 << page_log2) - 1)) * st + c * 16;
-    const bool in = kv0 + r < len && pg >= 0;
-    ae_cp16(smem_u32(dst) + ae_c8_at<W>(r, c), pool + (in ? at : 0), in);
+    for (int i = 0; i < AE_T / 16; ++i) {
+      const i64 first = (i64)p.t * AE_T + 16 * i;
+      page[i] = n < n1 && first < p.len ? row[first >> a.page_log2] : -1;
+    }
+  };
+  pages();
+  int slot = 0, fetched = 0;
+  u32 parity = 1;  // a slot is free at first
+  i64 t0 = clock64();
+  while (__any_sync(0xffffffffu, n < n1)) {
+    const bool go = n < n1 && ae_c8_test(&empty[slot], parity);
+    if (!__any_sync(0xffffffffu, go)) {
+      // no team is done with a tile: again, within a limit
+      const bool late = ctl->abort || clock64() - t0 > AE_WAIT_CYCLES;
+      if (__any_sync(0xffffffffu, late)) {
+        if (ctl->abort == 0 && a.status) atomicCAS(a.status, 0u, AE_ST_TIMEOUT_BASE + 2u);
+        ctl->abort = 1;
+        break;
+      }
+      __nanosleep(64);
+      continue;
+    }
+    if (go) {
+      u8* const kt = ring + slot * heads * AE_SLB;
+      u8* const vt = kt + heads * AE_KB;
+      float* const sc = scales + slot * heads * AE_SCF;
+      const int kv0 = p.t * AE_T, head0 = p.h << tl;
+      u32 there = 0;  // blocks of 16 keys
+#pragma unroll
+      for (int i = 0; i < AE_T / 16; ++i) {
+        if (kv0 + 16 * i < p.len && (u32)page[i] < (u32)a.num_pages) {
+          there |= 1u << i;
+        } else {
+          for (int j = 0; j < heads; ++j) sc[i * heads + j] = sc[(AE_T / 16 + i) * heads + j] = 1.f;
+          if (kv0 + 16 * i < p.len) {  // a page that is not there: zeros
+            if (a.status) atomicOr(a.status, 0x1000u);
+            for (int j = 0; j < heads; ++j) {
+              const int row = blk.at(i) + blk.head(j);
+              for (int x = 0; x < AE_D; ++x) *(uint4*)(kt + row * AE_D + x * 16) = make_uint4(0, 0, 0, 0);
+              for (int x = 0; x < AE_DV; ++x) *(uint4*)(vt + row * AE_DV + x * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+          }
+        }
+      }
+      u32 boxes = there;  // the blocks that begin one
+      if (blk.log2 > 0) boxes &= blk.log2 > 1 ? 0x11111111u : 0x55555555u;
+      mbar_arrive_expect_tx(&full[slot], (u32)(__popc(boxes) * box * heads) * (AE_D + AE_DV));
+#pragma unroll
+      for (int i = 0; i < AE_T / 16; ++i) {
+        if (boxes >> i & 1u) {
+          const int row = (kv0 + 16 * i) & ((1 << a.page_log2) - 1);
+          if (together) {
+            tma_load_4d(kt + blk.at(i) * AE_D, &a.tm_k[1], &full[slot], 0, row, head0, page[i]);
+            tma_load_4d(vt + blk.at(i) * AE_DV, &a.tm_v[1], &full[slot], 0, row, head0, page[i]);
+          } else {
+            for (int j = 0; j < heads; ++j) {
+              tma_load_4d(kt + (blk.at(i) + blk.head(j)) * AE_D, &a.tm_k[0], &full[slot], 0, row, head0 + j, page[i]);
+              tma_load_4d(vt + (blk.at(i) + blk.head(j)) * AE_DV, &a.tm_v[0], &full[slot], 0, row, head0 + j, page[i]);
+            }
+          }
+        }
+        if (there >> i & 1u) {
+          const float *ks = a.ks + (i64)page[i] * a.ks_sp + head0, *vs = a.vs + (i64)page[i] * a.vs_sp + head0;
+          const u32 to = smem_u32(sc + i * heads), to2 = smem_u32(sc + (AE_T / 16 + i) * heads);
+          if (heads >= 4 && a.scales16) {
+            for (int j = 0; j < heads; j += 4) {
+              ae_cp16(to + j * 4, ks + j);
+              ae_cp16(to2 + j * 4, vs + j);
+            }
+          } else {
+            for (int j = 0; j < heads; ++j) {
+              ae_cp4(to + j * 4, ks + j);
+              ae_cp4(to2 + j * 4, vs + j);
+            }
+          }
+        }
+      }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[slot])) : "memory");
+      ++n;
+      ++fetched;
+      ae_c8_next(p, a, tl);
+      pages();
+      if (slot == AE_C8_SLOTS - 1) {
+        slot = 0;
+        parity ^= 1u;
+      } else {
+        ++slot;
+      }
+      t0 = clock64();
+    }
+    __syncwarp();
+  }
+  if (ctl->abort) {  // nothing may land in the shared memory of a CTA that has left
+    t0 = clock64();
+    for (int i = fetched > AE_C8_SLOTS ? fetched - AE_C8_SLOTS : 0; i < fetched; ++i)
+      while (!ae_c8_test(&full[i % AE_C8_SLOTS], (u32)(i / AE_C8_SLOTS) & 1u) && clock64() - t0 < AE_WAIT_CYCLES) {
+      }
   }
 }
 
-// One CTA per (request, unit, row tile): the warps take its tiles in turn and merge at the end.
-extern "C" __global__ void __launch_bounds__(AE_WARPS * 32) ae_cache8_decode(const __grid_constant__ AeCache8DecodeArgs a) {
-  extern __shared__ __align__(128) u8 smem_raw[];
-  const u32 warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
-  u8* const kt = smem_raw + warp * (AE_KB + AE_VB);
-  u8* const vt = kt + AE_KB;
-  float* const part = (float*)(smem_raw + AE_WARPS * (AE_KB + AE_VB));  // [warp][row][DV], then [warp][row] maxima and sums
-  float* const part_m = part + AE_WARPS * AE_RT * AE_DV;
-  float* const part_l = part_m + AE_WARPS * AE_RT;
-  const int b = blockIdx.z, unit = blockIdx.y, row0 = blockIdx.x * AE_RT;
+AE_DEVICE void ae_c8_store(const AeCache8DecodeArgs& a, int b, int h, int row, int d, float4 x, float l) {
+  if (row >= a.rows) return;
+  const i64 at = a.gq > 1 ? (i64)b * a.Hq + h * a.gq + row : ((i64)b * a.rows + row) * a.Hq + h;
+  const float f = l == 0.f ? 0.f : 1.f / l;  // l = 0: no kept key
+  if (l == 0.f) x = make_float4(0.f, 0.f, 0.f, 0.f);
+  *(uint2*)((u16*)a.o + at * AE_DV + d) = make_uint2(pack2<AE_BF16>(x.x * f, x.y * f), pack2<AE_BF16>(x.z * f, x.w * f));
+}
+
+// `put(row of the tile, dim, four values)` for the lane's output, then `end(row, m, l)`.
+template <class Put, class End>
+AE_DEVICE void ae_c8_out(AeC8Rows& R, Put&& put, End&& end) {
+  const int g = (int)(lane_id() >> 2), t = (int)(lane_id() & 3u);
+#pragma unroll
+  for (int n = 0; n < AE_NB; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) R.l[n][e] += __shfl_xor_sync(0xffffffffu, R.l[n][e], o);
+#pragma unroll
+      for (int m = 0; m < AE_DV / 16; m += 2) {
+        const float4 x = make_float4(R.o[n][m][e], R.o[n][m][2 + e], R.o[n][m + 1][e], R.o[n][m + 1][2 + e]);
+        put(8 * n + 2 * t + e, (AE_DV / 8) * g + 2 * m, x, R.l[n][e]);
+      }
+      if (g == 0) end(8 * n + 2 * t + e, R.m[n][e], R.l[n][e]);
+    }
+}
+struct AeC8Sum {
+  float m, l;
+  float4 o;
+};
+extern "C" __global__ void __launch_bounds__(AE_C8_THREADS, 1) ae_cache8_decode(const __grid_constant__ AeCache8DecodeArgs a) {
+  extern __shared__ u8 smem_dyn[];
+  u8* const smem_raw = smem_align1024(smem_dyn);
+  const int warp = (int)threadIdx.x >> 5, lane = (int)lane_id();
+  AeC8Info* const info = (AeC8Info*)(smem_raw + AE_SMEM_INFO);
+
+  // ---- the line of tiles, and this warp's interval [n0, n1) ----
+  int* const before = a.B <= AE_FEW ? info->before : (int*)smem_raw;
+  // (a barrier's initialisation takes 60 to 80 clk, one lane after the other: spread over the warps)
+  if (warp == AE_WARPS) {
+    if (lane == 0) {
+      info->ctl.abort = 0;
+      if (!a.single) a.cuts[blockIdx.x].parts = 0;
+    }
+  } else if (lane == 0) {
+    for (int i = 0; i < AE_C8_SLOTS; ++i) {
+      mbar_init(&info->full[warp][i], 2);  // the boxes, and the scales
+      if (a.single) mbar_init(&info->empty[warp][i], 1);
+    }
+    mbar_fence_init();
+    info->rec[2 * warp].b = info->rec[2 * warp + 1].b = -1;
+  }
+  const int cta = (int)blockIdx.x;
+  int tl = 0, teams = AE_WARPS, per = 1, more = 0;  // warps of a team, log2; teams of a CTA; tiles of a team, teams with one more
+  int team = warp, n0, n1, cta0 = 0;
+  AeC8Pos at;
+  auto cut = [&](int w) { return w * per + (w < more ? w : more); };  // first tile of team w of the grid
+  auto team_of = [&](int x) { return x < more * (per + 1) ? x / (per + 1) : more + (x - more * (per + 1)) / per; };
+  if (a.single) {  // a unit that cannot be long, by its row's place in the grid
+    at.b = blockIdx.y;
+    at.len = ae_c8_len(a, at.b);
+    at.nt = ae_c8_tiles(at.len);
+    at.h = a.row_tiles == 1 ? cta : cta / a.row_tiles;
+    at.rt = cta - at.h * a.row_tiles;
+    if (warp == 0 && lane == 0 && (a.lens[at.b] < 0 || (i64)a.lens[at.b] > (i64)a.max_pages << a.page_log2) && a.status) atomicOr(a.status, 0x800u);
+    if (warp == AE_WARPS) team = lane < AE_WARPS ? lane : 0;
+    n0 = at.nt * team / AE_WARPS;
+    n1 = at.nt * (team + 1) / AE_WARPS;
+    at.t = n0;
+  } else {
+    if (warp == 0) {
+      int sum = 0, longest = 0;
+      for (int b0 = 0; b0 < a.B; b0 += 32) {
+        const int b = b0 + lane;
+        int x = 0;
+        if (b < a.B) {
+          x = ae_c8_tiles(ae_c8_len(a, b));
+          if ((a.lens[b] < 0 || (i64)a.lens[b] > (i64)a.max_pages << a.page_log2) && a.status) atomicOr(a.status, 0x800u);
+        }
+        longest = longest > x ? longest : x;
+        int s = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, s, o);
+          if (lane >= o) s += y;
+        }
+        if (b < a.B) before[b] = sum + s - x;
+        sum += __shfl_sync(0xffffffffu, s, 31);
+      }
+      longest = __reduce_max_sync(0xffffffffu, longest);
+      if (lane == 0) {
+        before[a.B] = sum;
+        info->longest = longest;
+      }
+    }
+    __syncthreads();
+    // equal intervals of at least AE_MIN_TILES for each team, the first `more` one longer
+    for (int i = 1; i <= a.team_log2; ++i)
+      if ((i64)info->longest * gridDim.x <= (i64)16 * before[a.B] * (a.Hkv >> i) * a.row_tiles) tl = i;
+    const int units = (a.Hkv >> tl) * a.row_tiles, total = before[a.B] * units;
+    teams = AE_WARPS >> tl;
+    int n_team = (int)gridDim.x * teams;
+    if (n_team * AE_MIN_TILES > total) n_team = total < teams * AE_MIN_TILES ? teams : (total / AE_MIN_TILES) & ~(teams - 1);
+    per = total / n_team;
+    more = total - per * n_team;
+    ae_grid_trigger();  // the merge may come up beside
+    if (cta * teams >= n_team) return;
+    // a warp for its team, lane w of the last warp for team w
+    team = warp < AE_WARPS ? warp >> tl : lane < teams ? lane : 0;
+    cta0 = cut(cta * teams);
+    n0 = cut(cta * teams + team);
+    n1 = cut(cta * teams + team + 1);
+    int lo = 0, hi = a.B;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (before[mid] * units <= n0)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    at.b = lo;
+    at.len = ae_c8_len(a, lo);
+    at.nt = before[lo + 1] - before[lo];
+    const int in = n0 - before[lo] * units, u = in / at.nt;
+    at.t = in - u * at.nt;
+    at.h = a.row_tiles == 1 ? u : u / a.row_tiles;
+    at.rt = u - at.h * a.row_tiles;
+  }
+  const int mate = warp & ((1 << tl) - 1);
+  if (!a.single && warp < AE_WARPS && lane == 0) {
+    for (int i = warp; i < teams * AE_C8_SLOTS; i += AE_WARPS) mbar_init(&info->empty[0][0] + i, 1u << tl);
+    mbar_fence_init();
+  }
+  if (!a.single && a.B > AE_FEW) fence_proxy_async_smem();
+  __syncthreads();  // `before` has been read: the copies may come
+
   AeCustom cu;
 #pragma unroll
   for (int i = 0; i < AE_MAX_CUSTOM; ++i) {
@@ -229,63 +568,114 @@ extern "C" __global__ void __launch_bounds__(AE_WARPS * 32) ae_cache8_decode(con
 #pragma unroll
     for (int k = 0; k < 4; ++k) cu.st[i][k] = a.custom_st[i][k];
   }
-  i64 want = a.lens[b];
-  const i64 most = (i64)a.max_pages << a.page_log2;
-  if ((want > most || want < 0) && threadIdx.x == 0 && a.status) atomicOr(a.status, 0x800u);
-  const int len = (int)(want < 0 ? 0 : want > most ? most : want);
+  const AeC8Blocks blk = {(a.page_log2 < AE_T_LOG2 ? a.page_log2 : AE_T_LOG2) - 4, 1 << tl};
+  u8* const ring = smem_raw + (team << tl) * (AE_C8_SLOTS * AE_SLB);  // the team's
+  float* const scales = (float*)(smem_raw + AE_SMEM_SCALE) + (team << tl) * (AE_C8_SLOTS * AE_SCF);
+  auto slot_of = [&](int c, int later, int j) { return a.part + (((i64)c * 2 + later) * AE_WARPS + j) * AE_REC; };
+  auto part_of = [&](int i, int j) {  // record i's partial of the team's j-th head
+    const int w = ((i >> 1) << tl) + j;
+    return (i & 1) ? (float*)(smem_raw + w * (AE_C8_SLOTS * AE_SLB)) : (float*)(smem_raw + AE_SMEM_HEAD) + w * AE_REC;
+  };
+  if (warp == AE_WARPS) {
+    ae_c8_fetch(a, ring, scales, info->full[team], info->empty[team], at, n0, lane < teams ? n1 : n0, tl, blk, &info->ctl);
+  } else {
   AeC8Rows R;
-  ae_c8_begin(R, a, b, unit, row0);
-  for (int kv0 = (int)warp * AE_T; kv0 < len; kv0 += AE_WARPS * AE_T) {
-    int page = -1;
-    const i64 first = (i64)kv0 + 16 * (i64)lane;
-    if ((int)lane < AE_T / 16 && first < len) {
-      page = a.table[(i64)b * a.table_stride + (first >> a.page_log2)];
-      if ((u32)page >= (u32)a.num_pages) {
-        if (a.status) atomicOr(a.status, 0x1000u);
-        page = -1;
+  int from = 0, slot = 0;
+  u32 parity = 0;
+#pragma unroll 1
+  for (int n = n0; n < n1; ++n) {
+    const int row0 = at.rt * AE_RT, kv0 = at.t * AE_T, head = (at.h << tl) + mate;
+    if (n == n0 || at.t == 0) {
+      ae_c8_begin(R, a, at.b, head, row0);
+      from = at.t;
+    }
+    // a wait that gives up is reported; the CTA goes on to its end
+    mbar_wait_w(&info->full[team][slot], parity, &info->ctl, a.status, 1);
+    u8* const kt = ring + (slot << tl) * AE_SLB + blk.head(mate) * AE_D;
+    u8* const vt = ring + (slot << tl) * AE_SLB + (AE_KB << tl) + blk.head(mate) * AE_DV;
+    if (kv0 + AE_T > at.len) {  // what lies behind the row's keys may be anything, and a P of 0 makes a NaN of a NaN
+      for (int x = (at.len - kv0) * (AE_DV / 16) + lane; x < AE_T * (AE_DV / 16); x += 32)
+        *(uint4*)(vt + blk.at(x / AE_DV) * AE_DV + x % AE_DV * 16) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();  // before the next copy into the slot
+      __syncwarp();
+    }
+    float s[AE_NB][2][AE_KPT];
+    u32 p[AE_NB][AE_KPT];
+    ae_c8_keys(R, kt, blk, s);
+    ae_c8_weights(R, s, p, kv0, at.len, scales + (slot << tl) * AE_SCF + mate, 1 << tl, at.b, head, row0, a, cu);
+    ae_c8_values(R, vt, blk, p);
+    mbar_arrive_warp(&info->empty[team][slot]);
+    if (slot == AE_C8_SLOTS - 1) {
+      slot = 0;
+      parity ^= 1u;
+    } else {
+      ++slot;
+    }
+    const bool ends = at.t == at.nt - 1;
+    if (ends && from == 0) {
+      ae_c8_out(R, [&](int r, int d, float4 x, float l) { ae_c8_store(a, at.b, head, row0 + r, d, x, l); }, [](int, float, float) {});
+    } else if (ends || n == n1 - 1) {
+      // what was begun before is the team's first piece; what goes on is its last, and its copies have all been used.  A team that is the
+      // whole CTA has nothing to add to it.
+      const bool later = n - at.t >= cta0;
+      float* const part = teams == 1 ? slot_of(cta, later ? 1 : 0, mate) : part_of(2 * team + (ends ? 0 : 1), mate);
+      if (teams > 1 && tl > 0 && n == n1 - 1) named_bar_sync(1 + team, 32 << tl);  // the slots are the team's
+      ae_c8_out(R, [&](int r, int d, float4 x, float) { *(float4*)(part + r * AE_DV + d) = x; },
+                [&](int r, float m, float l) {
+                  part[AE_RT * AE_DV + r] = m;
+                  part[AE_RT * AE_DV + AE_RT + r] = l;
+                });
+      if (lane == 0 && mate == 0) {
+        if (teams > 1)
+          info->rec[2 * team + (ends ? 0 : 1)] = {at.b, at.h, at.rt, n - at.t, from, at.t + 1, at.nt, 0};
+        else if (later)
+          a.cuts[cta] = {team_of(n - at.t + at.nt - 1) - cta + 1, at.b, at.h << tl, at.rt, 1 << tl};
       }
     }
-    ae_c8_fetch<AE_D>(kt, a.k + (i64)unit * a.k_sh, a.k_sp, a.k_st, a.page_log2, kv0, len, page);
-    ae_c8_fetch<AE_DV>(vt, a.v + (i64)unit * a.v_sh, a.v_sp, a.v_st, a.page_log2, kv0, len, page);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    float ks = page >= 0 ? a.ks[(i64)page * a.ks_sp + unit] : 1.f, vs = page >= 0 ? a.vs[(i64)page * a.vs_sp + unit] : 1.f;
-    ks = __shfl_sync(0xffffffffu, ks, t * AE_KPT / 16);
-    vs = __shfl_sync(0xffffffffu, vs, t * AE_KPT / 16);
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncwarp();
-    ae_c8_tile(R, kt, vt, kv0, len, ks, vs, b, unit, row0, a, cu);
-    __syncwarp();
+    ae_c8_next(at, a, tl);
   }
-#pragma unroll
-  for (int hf = 0; hf < AE_RT / 8; ++hf) {
-    R.l[hf] += __shfl_xor_sync(0xffffffffu, R.l[hf], 1);
-    R.l[hf] += __shfl_xor_sync(0xffffffffu, R.l[hf], 2);
-    const u32 r = g + 8 * hf;
-    if (t == 0) {
-      part_m[warp * AE_RT + r] = R.m[hf];
-      part_l[warp * AE_RT + r] = R.l[hf];
-    }
-#pragma unroll
-    for (int m = 0; m < AE_DV / 8; ++m)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) part[(warp * AE_RT + r) * AE_DV + (AE_DV / 8) * (2 * t + e) + m] = R.o[m][2 * hf + e];
   }
+  if (teams == 1) return;
   __syncthreads();
-  for (int i = threadIdx.x; i < AE_RT * AE_DV / 2; i += AE_WARPS * 32) {
-    const int r = i / (AE_DV / 2), d = i % (AE_DV / 2) * 2;
-    if (row0 + r >= a.rows) continue;
-    float m = AE_NEG_INF;
-    for (int w = 0; w < AE_WARPS; ++w) m = fmaxf(m, part_m[w * AE_RT + r]);
-    float l = 0.f, x = 0.f, y = 0.f;
-    for (int w = 0; w < AE_WARPS; ++w) {
-      if (part_m[w * AE_RT + r] == AE_NEG_INF && part_l[w * AE_RT + r] == 0.f) continue;  // no kept key
-      const float f = ae_exp2(part_m[w * AE_RT + r] - m);
-      l += f * part_l[w * AE_RT + r];
-      x += f * part[(w * AE_RT + r) * AE_DV + d];
-      y += f * part[(w * AE_RT + r) * AE_DV + d + 1];
+
+  // ---- cut units: the pieces of this CTA, then of all CTAs ----
+  constexpr int ITEMS = AE_RT * (AE_DV / 4);
+  // records in a lane each; the pieces of a unit are those with the same first tile
+  AeC8Record rec = info->rec[lane < 2 * teams ? lane : 0];
+  u32 left = __ballot_sync(0xffffffffu, lane < 2 * teams && rec.b >= 0);
+  while (left) {
+    const int i = __ffs(left) - 1;
+    const AeC8Record first = info->rec[i];
+    const u32 has = __ballot_sync(0xffffffffu, rec.begin == first.begin) & left;
+    const int to = __shfl_sync(0xffffffffu, rec.to, 31 - __clz(has));
+    left &= ~has;
+    const bool whole = first.from == 0 && to == first.nt, later = first.begin >= cta0;
+    for (int x = (int)threadIdx.x; x < ITEMS << tl; x += AE_C8_THREADS) {
+      const int m0 = x / ITEMS, r = x % ITEMS / (AE_DV / 4), d = x % (AE_DV / 4) * 4;
+      if (first.rt * AE_RT + r >= a.rows) continue;
+      AeC8Sum s = {AE_NEG_INF, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+      for (u32 k = has; k; k &= k - 1) s.m = fmaxf(s.m, part_of(__ffs(k) - 1, m0)[AE_RT * AE_DV + r]);
+      for (u32 k = has; k; k &= k - 1) {
+        const float* const p = part_of(__ffs(k) - 1, m0);
+        const float m = p[AE_RT * AE_DV + r], l = p[AE_RT * AE_DV + AE_RT + r];
+        if (m == AE_NEG_INF && l == 0.f) continue;  // no kept key
+        const float f = ae_exp2(m - s.m);
+        const float4 o = *(const float4*)(p + r * AE_DV + d);
+        s.l += f * l;
+        s.o.x += f * o.x; s.o.y += f * o.y; s.o.z += f * o.z; s.o.w += f * o.w;
+      }
+      if (whole) {
+        ae_c8_store(a, first.b, (first.h << tl) + m0, first.rt * AE_RT + r, d, s.o, s.l);
+      } else {
+        float* const slot = slot_of(cta, later ? 1 : 0, m0);
+        *(float4*)(slot + r * AE_DV + d) = s.o;
+        if (d == 0) {
+          slot[AE_RT * AE_DV + r] = s.m;
+          slot[AE_RT * AE_DV + AE_RT + r] = s.l;
+        }
+      }
     }
-    if (l == 0.f) x = y = 0.f, l = 1.f;  // a row without a kept key
-    const i64 row = a.gq > 1 ? (i64)b * a.Hq + unit * a.gq + row0 + r : ((i64)b * a.rows + row0 + r) * a.Hq + unit;
-    *(u32*)((u16*)a.o + row * AE_DV + d) = pack2<AE_BF16>(x / l, y / l);
+    if (!whole && later && threadIdx.x == 0)  // it goes on: what the merge has to know
+      a.cuts[cta] = {team_of(first.begin + first.nt - 1) / teams - cta + 1, first.b, first.h << tl, first.rt, 1 << tl};
   }
 }

@@ -28,6 +28,7 @@ KIND_ATTN_BWD_FUSED, KIND_ATTN_BWD_CAST = 12, 13
 KIND_ATTN_FWD_PAIR = 14
 KIND_LINEAR_SEGMENTS = 15
 KIND_ATTN_PACKED, KIND_PLAN_PAGES, KIND_CACHE8_WRITE, KIND_CACHE8_DECODE = 16, 17, 18, 19
+KIND_CACHE8_MERGE = 20
 DTYPE_F16, DTYPE_BF16 = 0, 1
 
 
@@ -161,7 +162,7 @@ class Cache8DecodeParams(C.Structure):
                [("q_stride", _S3), ("k_codes_stride", _S3), ("v_codes_stride", _S3), ("k_scale_stride", C.c_int64),
                 ("v_scale_stride", C.c_int64), ("table_stride", C.c_int64), ("custom", C.c_void_p * AE_MAX_CUSTOM),
                 ("custom_stride", (C.c_int64 * 4) * AE_MAX_CUSTOM)] + \
-               [(n, C.c_int32) for n in ("B", "Hq", "Hkv", "Sq", "max_pages", "num_pages", "page_size")] + [("status", C.c_void_p)]
+               [(n, C.c_int32) for n in ("B", "Hq", "Hkv", "Sq", "max_pages", "num_pages", "page_size")] + [("status", C.c_void_p), ("workspace", C.c_void_p)]
 
 
 _lib = None
@@ -171,7 +172,8 @@ EXPORTS = ["ae_compile", "ae_module_from_cubin", "ae_module_cubin", "ae_query", 
            "ae_last_error", "ae_launch_attn_fwd", "ae_launch_attn_bwd_prep", "ae_launch_attn_bwd_dq",
            "ae_launch_attn_bwd_dkv", "ae_launch_attn_bwd_fused", "ae_launch_attn_bwd_dq_cast", "ae_launch_probe", "ae_launch_attn_bwd_static_scratch", "ae_launch_mla_decode", "ae_launch_mla_combine", "ae_launch_mla_decode_paged", "ae_launch_attn_decode", "ae_launch_decode_combine", "ae_launch_rowscale", "ae_launch_linear_fwd", "ae_launch_linear_states", "ae_launch_linear_bwd",
            "ae_launch_linear_segments", "ae_launch_attn_packed", "ae_launch_plan_pages", "ae_launch_cache8_write",
-           "ae_launch_cache8_decode"]
+           "ae_launch_cache8_decode", "ae_cache8_decode_workspace",
+           "ae_cache8_decode_merges", "ae_launch_cache8_merge"]
 
 
 def lib() -> C.CDLL:
@@ -212,6 +214,10 @@ def lib() -> C.CDLL:
             L.ae_launch_plan_pages.argtypes = [C.c_void_p, C.POINTER(PlanPagesParams), C.c_void_p]
             L.ae_launch_cache8_write.argtypes = [C.c_void_p, C.POINTER(Cache8WriteParams), C.c_void_p]
             L.ae_launch_cache8_decode.argtypes = [C.c_void_p, C.POINTER(Cache8DecodeParams), C.c_void_p]
+            L.ae_cache8_decode_workspace.argtypes = [C.c_void_p]
+            L.ae_cache8_decode_workspace.restype = C.c_int64
+            L.ae_cache8_decode_merges.argtypes = [C.c_void_p, C.POINTER(Cache8DecodeParams)]
+            L.ae_launch_cache8_merge.argtypes = [C.c_void_p, C.POINTER(Cache8DecodeParams), C.c_void_p]
             L.ae_launch_probe.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
                                           C.c_void_p, C.c_void_p]
             _lib = L

@@ -64,6 +64,7 @@ enum {
   AE_KIND_PLAN_PAGES = 17,
   AE_KIND_CACHE8_WRITE = 18,
   AE_KIND_CACHE8_DECODE = 19,
+  AE_KIND_CACHE8_MERGE = 20,
 };
 
 #define AE_MAX_CUSTOM_INPUTS 4
@@ -201,7 +202,9 @@ typedef struct AeCache8WriteParams {
 int ae_launch_cache8_write(void* module, const AeCache8WriteParams* p, void* stream);
 
 /* Softmax attention of Sq query positions a row (one with grouped heads) over the row's first seq_lens[b] cached keys.  A length
- * outside the table is cut to it (status 0x800), a page outside the pool counts as zeros (status 0x1000).  A row without keys gets zeros. */
+ * outside the table is cut to it (status 0x800), a page outside the pool counts as zeros (status 0x1000).  A row without keys gets zeros.
+ * `workspace`: ae_cache8_decode_workspace(module) bytes, 16-byte aligned, with any contents.  Where ae_cache8_decode_merges says so for these
+ * parameters, ae_launch_cache8_merge follows with the same ones. */
 typedef struct AeCache8DecodeParams {
   const void* q;             /* [B, Sq, Hq, D] */
   void* o;                   /* [B, Sq, Hq, DV] contiguous */
@@ -218,7 +221,11 @@ typedef struct AeCache8DecodeParams {
   int64_t custom_stride[AE_MAX_CUSTOM_INPUTS][4];
   int32_t B, Hq, Hkv, Sq, max_pages, num_pages, page_size; /* page_size: 16, 32, 64 or 128 */
   uint32_t* status;
+  void* workspace;
 } AeCache8DecodeParams;
+int64_t ae_cache8_decode_workspace(void* module);
+int ae_cache8_decode_merges(void* module, const AeCache8DecodeParams* p);
+int ae_launch_cache8_merge(void* module, const AeCache8DecodeParams* p, void* stream);
 int ae_launch_cache8_decode(void* module, const AeCache8DecodeParams* p, void* stream);
 
 /* ---- attention backward -----------------------------------------------------------
