@@ -572,8 +572,10 @@ int ae_launch_attn_packed(void* module, const AeAttnPackedParams* p, void* strea
   args.Sq = args.Skv = p->T;
   args.cu_seqlens = p->cu_seqlens;
   args.status = p->status;
-  // no more pairs than this whatever the lengths: a sequence of n positions has at most n / 256 + 1
-  const int64_t pairs = (int64_t)p->T / 256 + std::min(p->n_seq, p->T), ctas = pairs * p->Hq;
+  // no more blocks of rows than this whatever the lengths: a sequence of n positions has at most n / rows + 1
+  auto blocks = [&](int rows) { return (int64_t)p->T / rows + std::min(p->n_seq, p->T); };
+  args.pair_mode = blocks(128) * p->Hq <= 148 ? 2 : p->Hq / p->Hkv % 2 == 0 ? 1 : 0;
+  const int64_t ctas = blocks(args.pair_mode == 0 ? 256 : 128) * (args.pair_mode == 1 ? p->Hq / 2 : p->Hq);
   if (ctas > 0x7fffffff) {
     set_error("packed attention: too many q tiles for one launch");
     return AE_ERR_INVALID;

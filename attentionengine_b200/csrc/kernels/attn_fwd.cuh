@@ -115,11 +115,11 @@ AE_DEVICE int ae_causal_ntiles(int qt, int n_kt) {
 }
 
 #if AE_PACKED
-// The i-th q-tile pair of the packed sequences, by the length of its walk: the last pairs of the longest sequences first, so that the last
-// CTAs to start are the shortest.  The pairs behind pair L of their sequence number S(L) = sum over the sequences of max(0, pairs - 1 - L), so
-// the pair that is i-th has the L with S(L) <= i < S(L - 1), by bisection.  One warp; `at` = {sequence, pair, start, length}, or -1 for the
-// sequence where there are not that many.
-AE_DEVICE void ae_find_pair(int* at, int* pairs, const AeAttnFwdArgs& args, int i) {
+// The i-th block of `rows` query rows of the packed sequences, by the length of its walk: the last blocks of the longest sequences first, so that the
+// last CTAs to start are the shortest.  The blocks behind block L of their sequence number S(L) = sum over the sequences of
+// max(0, blocks - 1 - L), so the one that is i-th has the L with S(L) <= i < S(L - 1), by bisection.  One warp, a sequence in a lane (more than
+// 32: `more` in shared memory); `at` = {sequence, block, start, length}, or -1 for the sequence where there are not that many.
+AE_DEVICE void ae_find_block(int* at, int* more, const AeAttnFwdArgs& args, int i, int rows) {
   const int lane = (int)lane_id(), n = args.B, T = args.Sq;
   // positions outside the tensors would be a caller's mistake: reported, and cut to them
   auto span = [&](int b, int& start) {
@@ -129,39 +129,44 @@ AE_DEVICE void ae_find_pair(int* at, int* pairs, const AeAttnFwdArgs& args, int 
     const int end = s1 < start ? start : s1 > T ? T : s1;
     return end - start;
   };
-  int most = 0;
-  for (int b = lane; b < n; b += 32) {
-    int start;
-    const int p = (span(b, start) + 2 * AE_BM - 1) / (2 * AE_BM);
-    pairs[b] = p;
+  int start = 0, len = 0;
+  if (lane < n) len = span(lane, start);
+  const int mine = (len + rows - 1) / rows;
+  int most = mine;
+  for (int b = lane + 32; b < n; b += 32) {
+    int s;
+    const int p = (span(b, s) + rows - 1) / rows;
+    more[b] = p;
     most = most > p ? most : p;
   }
   most = __reduce_max_sync(0xffffffffu, most);
   __syncwarp();
   auto behind = [&](int L) {
-    int s = 0;
-    for (int b = lane; b < n; b += 32) s += pairs[b] - 1 > L ? pairs[b] - 1 - L : 0;
+    int s = mine - 1 > L ? mine - 1 - L : 0;
+    for (int b = lane + 32; b < n; b += 32) s += more[b] - 1 > L ? more[b] - 1 - L : 0;
     return __reduce_add_sync(0xffffffffu, s);
   };
-  int lo = -1, hi = most;  // S(lo) > i >= S(hi)
   if (behind(-1) <= i) {
     if (lane == 0) at[0] = -1;
     return;
   }
+  int lo = -1, hi = most, at_hi = 0;  // S(lo) > i >= S(hi) = at_hi
   while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (behind(mid) > i)
+    const int mid = (lo + hi) >> 1, s = behind(mid);
+    if (s > i) {
       lo = mid;
-    else
+    } else {
       hi = mid;
+      at_hi = s;
+    }
   }
-  int k = i - behind(hi);  // the k-th of the sequences that have a pair `hi`
+  int k = i - at_hi;  // the k-th of the sequences that have a block `hi`
   for (int b0 = 0; b0 < n; b0 += 32) {
-    const bool has = b0 + lane < n && pairs[b0 + lane] > hi;
+    const bool has = (b0 == 0 ? mine : b0 + lane < n ? more[b0 + lane] : 0) > hi;
     const u32 m = __ballot_sync(0xffffffffu, has);
     if (has && __popc(m & ((1u << lane) - 1u)) == k) {
-      int start;
-      at[3] = span(b0 + lane, start);
+      if (b0 > 0) len = span(b0 + lane, start);
+      at[3] = len;
       at[2] = start;
       at[1] = hi;
       at[0] = b0 + lane;
@@ -211,17 +216,45 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
 #define AE_SKV skv
 #elif AE_PACKED
 #define AE_SKV skv
+  // A CTA's two q tiles are one tile of two heads where a kv head's query heads are even in number: both walk the same kv tiles, and a
+  // sequence with an odd number of tiles leaves none alone (four prompts up to 8192 tokens: 848 -> 706 us).  Otherwise they are two neighbouring
+  // tiles of a head; and where all tiles find an SM of their own, there is one.  While one warp looks for the tiles, others make the barriers
+  // (60 to 80 clk each) and take the TMEM.
   int* const seq_at = (int*)(smem + AE_SMEM_SEQ);
-  if (warp == 0) ae_find_pair(seq_at, seq_at + 4, args, (int)blockIdx.x / args.Hq);
+  const int n_head = args.pair_mode == 1 ? args.Hq / 2 : args.Hq;
+  if (warp == 0) {
+    ae_find_block(seq_at, seq_at + 4, args, (int)blockIdx.x / n_head, args.pair_mode == 0 ? 2 * AE_BM : AE_BM);
+  } else if (warp <= 5 && lane == 0) {
+    u64* const bar = bars->q_full;  // and the others behind it
+    for (int i = (int)warp - 1; i < 6 + 2 * AE_STAGES; i += 5) mbar_init(bar + i, 1);
+    if (warp == 1) ctl->abort = 0;
+    mbar_fence_init();
+  } else if (warp == AE_ROW_WARPS) {
+    if (lane == 0) {
+      tma_prefetch_desc(&args.tm_q);
+      tma_prefetch_desc(&args.tm_k);
+      tma_prefetch_desc(&args.tm_v);
+    }
+  } else if (warp == AE_ROW_WARPS + 1) {
+    tmem_alloc(&ctl->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
   __syncthreads();
+  tc_fence_after_sync();
   const int b = seq_at[0];
-  if (b < 0) return;
-  const int hq = (int)blockIdx.x % args.Hq;
+  if (b < 0) {
+    if (warp == AE_ROW_WARPS + 1) tmem_dealloc(ctl->tmem_base, 512);
+    return;
+  }
+  const int hq = (int)blockIdx.x % n_head * (args.pair_mode == 1 ? 2 : 1);  // of tile 0
   const int hk = hq / (args.Hq / args.Hkv);
-  const int qt0 = 2 * seq_at[1];
+  const int qt0 = args.pair_mode == 0 ? 2 * seq_at[1] : seq_at[1];
   const int seq0 = seq_at[2];  // position of the sequence's first row in the tensors
   const int skv = seq_at[3];
   const int kt_off = 0;
+  // tile t: q tile qt0 + t next_qt, head hq + t next_h
+  const int next_qt = args.pair_mode == 0 ? 1 : args.pair_mode == 1 ? 0 : 1 << 24, next_h = args.pair_mode == 1 ? 1 : 0;
 #else
 #define AE_SKV args.Skv
   // One-dimensional grid: sections of args.sec (batch, q-head) units; inside a section all units' last q pair first, then
@@ -243,9 +276,12 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
 #else
   const int n_qt = args.n_qt, n_kt = args.n_kt, s_q = args.Sq;
   const int seq0 = 0;
+  constexpr int next_qt = 1, next_h = 0;  // tile t: q tile qt0 + t next_qt, head hq + t next_h
 #endif
   (void)n_kt;
   (void)s_q;
+  (void)next_qt;
+  (void)next_h;
 
 #ifdef AE_TRACE
   const bool tr_cta = blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
@@ -254,7 +290,7 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
   int n_steps;
 #if AE_MASK_MODE == 1
   int n_t0 = ae_causal_ntiles(qt0, n_kt);
-  int n_t1 = (qt0 + 1 < n_qt) ? ae_causal_ntiles(qt0 + 1, n_kt) : 0;
+  int n_t1 = (qt0 + next_qt < n_qt) ? ae_causal_ntiles(qt0 + next_qt, n_kt) : 0;
   n_steps = n_t0 > n_t1 ? n_t0 : n_t1;
 #elif AE_MASK_MODE == 2
   const u32* steps = (const u32*)(smem + AE_SMEM_STEPS);
@@ -265,7 +301,7 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
   n_steps = n_t0;
 #else
   int n_t0 = n_kt;
-  int n_t1 = (qt0 + 1 < n_qt) ? n_kt : 0;
+  int n_t1 = (qt0 + next_qt < n_qt) ? n_kt : 0;
   n_steps = n_kt;
 #endif
 
@@ -293,7 +329,7 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
 #if AE_MASK_MODE == 1
     // partial when the tile's last column exceeds the tile's first row
     if (walk.j * AE_BN + AE_BN - 1 > qt0 * AE_BM) st.flags |= 4u;
-    if (walk.j * AE_BN + AE_BN - 1 > (qt0 + 1) * AE_BM) st.flags |= 8u;
+    if (walk.j * AE_BN + AE_BN - 1 > (qt0 + next_qt) * AE_BM) st.flags |= 8u;
 #endif
     walk.j++;
     return true;
@@ -301,6 +337,7 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
   };
 
   // ---- setup ---------------------------------------------------------------------
+#if !AE_PACKED
   if (threadIdx.x == 0) {
     ctl->abort = 0;
     for (int i = 0; i < 2; ++i) {
@@ -324,6 +361,7 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
     }
     mbar_fence_init();
   }
+#endif
 #if AE_MASK_MODE == 2
   {
     // flag word per kv tile: bit t = tile t takes part, bit 2+t = it needs the element mask.  The lists come from the
@@ -379,6 +417,7 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
     }
   }
 #endif
+#if !AE_PACKED
   if (warp == AE_ROW_WARPS + 1) {
     tmem_alloc(&ctl->tmem_base, 512);
     tmem_relinquish();
@@ -386,6 +425,7 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+#endif
   const u32 tmem = ctl->tmem_base;
 #if AE_DECODE
   ae_grid_trigger();
@@ -410,12 +450,12 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
 #if AE_DECODE
         if (t > 0 && t * AE_BM >= args.rows) break;
 #else
-        if (qt0 + t >= n_qt) break;
+        if (qt0 + t * next_qt >= n_qt) break;
 #endif
         mbar_arrive_expect_tx(&bars->q_full[t], AE_Q_BYTES);
         for (int dh = 0; dh < AE_D / 64; ++dh)
           tma_load_bshd(smem + AE_SMEM_Q + t * AE_Q_BYTES + dh * (AE_BM * 128), &args.tm_q, &bars->q_full[t], dh * 64,
-                      hq, seq0 + (qt0 + t) * AE_BM, AE_PACKED ? 0 : b);
+                      hq + t * next_h, seq0 + (qt0 + t * next_qt) * AE_BM, AE_PACKED ? 0 : b);
       }
       AeKvStep st;
 #if AE_DECODE
@@ -637,7 +677,7 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
     const u32 lane_base = ((warp & 3) * 32) << 16;
     const u32 tm_s = tmem + (t ? TM_S1 : TM_S0) + lane_base;
     const u32 tm_o = tmem + (t ? TM_O1 : TM_O0) + lane_base;
-    const bool tile_valid = (qt0 + t) < n_qt;
+    const bool tile_valid = (qt0 + t * next_qt) < n_qt;
 #if AE_DECODE
     // packed rows: the query heads of the kv head's group (one query position), or the positions of one head;
     // rows past the last valid one compute on zero-filled Q with the indices of row 0 and are never stored
@@ -646,9 +686,9 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
     const int h_row = (args.gq > 1) ? hq * args.gq + (row_valid ? r_idx : 0) : hq;
     const int q_idx = (args.gq > 1 || !row_valid) ? 0 : r_idx;
 #else
-    const int q_idx = (qt0 + t) * AE_BM + (int)row;
+    const int q_idx = (qt0 + t * next_qt) * AE_BM + (int)row;
     const bool row_valid = q_idx < s_q;
-    const int h_row = hq;
+    const int h_row = hq + t * next_h;
 #endif
 
     AeCustom cu;
@@ -833,7 +873,7 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
           else if (args.final_rs[i])
             args.final_rs[i][((i64)b * args.Hq + h_row) * args.Sq + q_idx] = fr[i];
 #else
-          args.final_rs[i][((i64)(AE_PACKED ? 0 : b) * args.Hq + hq) * args.Sq + seq0 + q_idx] = fr[i];
+          args.final_rs[i][((i64)(AE_PACKED ? 0 : b) * args.Hq + h_row) * args.Sq + seq0 + q_idx] = fr[i];
 #endif
         }
       }
