@@ -49,7 +49,7 @@ class PagePlan(NamedTuple):
 
 @functools.lru_cache(maxsize=None)
 def _plan_kernel():
-    smem = 3 * (MAX_ROWS + 1) * 4 + 4 + 8 * 8
+    smem = 3 * (MAX_ROWS + 1) * 4 + 4 + 2 * 8 * 8 + 8
     cfg = rt.KernelConfig(kind=rt.KIND_PLAN_PAGES, threads=256, smem_bytes=smem)
     return rt.compile_module(rt.kernel_source("plan_pages.cuh", prelude=f"#define AE_PLAN_ROWS {MAX_ROWS}\n"), "ae_plan_pages", cfg)
 

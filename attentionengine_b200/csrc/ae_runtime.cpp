@@ -650,10 +650,16 @@ int ae_launch_cache8_write(void* module, const AeCache8WriteParams* p, void* str
     return AE_ERR_INVALID;
   }
   a.s_sp[0] = p->k_scale_stride; a.s_sp[1] = p->v_scale_stride;
-  a.n_tokens = p->n_tokens; a.num_pages = p->num_pages; a.bf16 = p->dtype == AE_DTYPE_BF16;
+  a.n_tokens = p->n_tokens; a.num_pages = p->num_pages; a.H = p->H; a.bf16 = p->dtype == AE_DTYPE_BF16;
   int rc = ensure_loaded(m);
   if (rc) return rc;
-  return launch(m, (unsigned)p->n_segments, (unsigned)p->H, 2, &a, stream);
+  // the heads of a segment side by side: their values are neighbours in memory
+  const int64_t ctas = (int64_t)p->n_segments * p->H;
+  if (ctas > 0x7fffffff) {
+    set_error("cache write: too many segments for one launch");
+    return AE_ERR_INVALID;
+  }
+  return launch(m, (unsigned)ctas, 2, 1, &a, stream);
 }
 
 // One CTA per SM; the table of cut units, then two partials of a row tile for each warp.

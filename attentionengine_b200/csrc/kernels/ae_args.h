@@ -283,7 +283,7 @@ struct AeCache8WriteArgs {
   i64 x_st[2], x_sh[2];               // element strides of x: token, head
   i64 c_sp[2], c_st[2], c_sh[2];      // of codes: page, token, head
   i64 s_sp[2];                        // of scales: page
-  int n_tokens, num_pages, bf16;
+  int n_tokens, num_pages, H, bf16;
 };
 
 // ---- decode over a paged 8-bit cache (kernel ae_cache8_decode) -----------------------------------

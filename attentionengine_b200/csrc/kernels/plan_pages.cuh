@@ -17,7 +17,8 @@ struct AePlanSmem {
   int cu[AE_PLAN_ROWS + 1];     // first new token of each row
   int take[AE_PLAN_ROWS + 1];   // first needed page
   int seg[AE_PLAN_ROWS + 1];    // first segment
-  i64 warp_sum[AE_PLAN_THREADS / 32];
+  i64 warp_sum[2][AE_PLAN_THREADS / 32];
+  u32 bad;
 };
 
 // Exclusive sum over the block; `total` is the whole.
@@ -29,7 +30,6 @@ AE_DEVICE i64 ae_block_scan(i64 x, i64* warp_sum, i64& total) {
     const i64 y = __shfl_up_sync(0xffffffffu, s, o);
     if ((int)lane >= o) s += y;
   }
-  __syncthreads();  // the sums of an earlier scan have been read
   if (lane == 31) warp_sum[warp] = s;
   __syncthreads();
   i64 before = 0;
@@ -61,8 +61,10 @@ extern "C" __global__ void __launch_bounds__(AE_PLAN_THREADS) ae_plan_pages(cons
   const int P = 1 << a.page_log2;
   const int per = (a.B + AE_PLAN_THREADS - 1) / AE_PLAN_THREADS;  // rows of a thread
   const int r0 = min((int)threadIdx.x * per, a.B), r1 = min(r0 + per, a.B);
+  const i64 head = max(*a.free_head, 0);
   u32 bad = 0;
   auto old_len = [&](int r) { return max(a.old_lens[r], 0); };
+  if (threadIdx.x == 0) sm.bad = 0;
 
   i64 sum = 0, total;
   for (int r = r0; r < r1; ++r) {
@@ -70,52 +72,48 @@ extern "C" __global__ void __launch_bounds__(AE_PLAN_THREADS) ae_plan_pages(cons
     if (n < 0 || a.old_lens[r] < 0) bad |= 8u;
     sum += max(n, 0);
   }
-  i64 at = ae_block_scan(sum, sm.warp_sum, total);
+  const i64 first = ae_block_scan(sum, sm.warp_sum[0], total);
   if (total > a.n_tokens) bad |= 4u;
-  for (int r = r0; r < r1; ++r) {
-    sm.cu[r] = (int)min(at, (i64)a.n_tokens);
-    at += max(a.new_lens[r], 0);
-  }
-  if (threadIdx.x == 0) sm.cu[a.B] = (int)min(total, (i64)a.n_tokens);
-  __syncthreads();
-
   // pages from `have` to `want`, segments: pages of the table that get a token
-  auto pages = [&](int r, int& have, int& want, int& n_seg, bool& outgrown) {
-    const i64 o = old_len(r), n = sm.cu[r + 1] - sm.cu[r];
+  auto pages = [&](int r, i64 n, int& need, int& n_seg, bool& outgrown) {
+    const i64 o = old_len(r);
     const i64 h = (o + P - 1) >> a.page_log2, w = (o + n + P - 1) >> a.page_log2;
-    have = (int)min(h, (i64)a.max_pages);
-    want = (int)min(w, (i64)a.max_pages);
+    need = (int)(min(w, (i64)a.max_pages) - min(h, (i64)a.max_pages));
     outgrown = w > a.max_pages;
     n_seg = n > 0 ? (int)(w - (o >> a.page_log2)) : 0;
   };
-  i64 need = 0, segs = 0, all_need, all_segs;
+  i64 at = first, mine = 0, all;  // needed pages, and segments above them
   for (int r = r0; r < r1; ++r) {
-    int have, want, n_seg;
+    const i64 from = min(at, (i64)a.n_tokens);
+    at += max(a.new_lens[r], 0);
+    sm.cu[r] = (int)from;
+    int need, n_seg;
     bool outgrown;
-    pages(r, have, want, n_seg, outgrown);
-    need += want - have;
-    segs += n_seg;
+    pages(r, min(at, (i64)a.n_tokens) - from, need, n_seg, outgrown);
+    mine += (i64)n_seg << 32 | (u32)need;
     if (outgrown) bad |= 2u;
   }
-  need = ae_block_scan(need, sm.warp_sum, all_need);
-  segs = ae_block_scan(segs, sm.warp_sum, all_segs);
+  mine = ae_block_scan(mine, sm.warp_sum[1], all);
+  at = first;
   for (int r = r0; r < r1; ++r) {
-    int have, want, n_seg;
+    const i64 from = min(at, (i64)a.n_tokens);
+    at += max(a.new_lens[r], 0);
+    int need, n_seg;
     bool outgrown;
-    pages(r, have, want, n_seg, outgrown);
-    sm.take[r] = (int)need;
-    sm.seg[r] = (int)segs;
-    need += want - have;
-    segs += n_seg;
+    pages(r, min(at, (i64)a.n_tokens) - from, need, n_seg, outgrown);
+    sm.take[r] = (int)(u32)mine;
+    sm.seg[r] = (int)(mine >> 32);
+    mine += (i64)n_seg << 32 | (u32)need;
   }
+  const int all_need = (int)(u32)all, all_segs = (int)(all >> 32);
   if (threadIdx.x == 0) {
-    sm.take[a.B] = (int)all_need;
-    sm.seg[a.B] = (int)all_segs;
+    sm.cu[a.B] = (int)min(total, (i64)a.n_tokens);
+    sm.take[a.B] = all_need;
+    sm.seg[a.B] = all_segs;
+    if (head + all_need > a.n_free) bad |= 1u;
   }
-  const i64 head = max(*a.free_head, 0);
-  if (head + all_need > a.n_free) bad |= 1u;
-  bad = (u32)__syncthreads_or(bad & 1u) | (u32)(__syncthreads_or(bad & 2u) ? 2 : 0) | (u32)(__syncthreads_or(bad & 4u) ? 4 : 0) |
-        (u32)(__syncthreads_or(bad & 8u) ? 8 : 0);
+  if (bad) atomicOr(&sm.bad, bad);
+  __syncthreads();
 
   // page i of row r, which may be one that this step takes
   auto page_of = [&](int r, i64 i) -> int {
@@ -154,8 +152,8 @@ extern "C" __global__ void __launch_bounds__(AE_PLAN_THREADS) ae_plan_pages(cons
     }
     a.segments[s] = e;
   }
-  for (i64 i = tid; i < all_need; i += step) {
-    const int r = ae_row_of(sm.take, a.B, (int)i);
+  for (int i = tid; i < all_need; i += step) {
+    const int r = ae_row_of(sm.take, a.B, i);
     const int have = (int)min((i64)((old_len(r) + (i64)P - 1) >> a.page_log2), (i64)a.max_pages);
     a.table[(i64)r * a.table_stride + have + (i - sm.take[r])] = head + i < a.n_free ? a.free_pages[head + i] : -1;
   }
@@ -165,6 +163,6 @@ extern "C" __global__ void __launch_bounds__(AE_PLAN_THREADS) ae_plan_pages(cons
   }
   if (tid == 0) {
     *a.head_out = (int)min(head + all_need, (i64)a.n_free);
-    *a.status = bad;
+    *a.status = sm.bad;
   }
 }
