@@ -67,7 +67,7 @@ class H100:
 
 
 _DYN_PROBE = 1024  # sequence length on which a dynamic-shape engine classifies its mask
-MAX_PACKED = 4096  # sequences of a packed call (AE_MAX_SEQ of attn_fwd.cuh)
+MAX_PACKED = 4096  # sequences of a packed call (AE_MAX_SEQ of attn_packed.cuh)
 MAX_LIST_KV_TILES = 2048  # kv tiles a block list may cover (AE_MAX_KT of attn_fwd.cuh): 262,144 keys
 
 _TORCH_DTYPES = {torch.float16: rt.DTYPE_F16, torch.bfloat16: rt.DTYPE_BF16}
@@ -121,12 +121,12 @@ class _AttnKernels:
         pair = int(os.environ.get("AE_B200_FWD_PAIR", self.tuned.get("fwd_pair", FWD_PAIR)))
         self.fwd_pair = bool(pair) and mask_mode in (0, 1, 3) and DV == 128 and D in (64, 128) and not packed
         if packed:
-            smem += 16 + 4 * MAX_PACKED  # where the CTA is, and the q-tile pairs of every sequence
+            smem += 4 * MAX_PACKED  # the blocks of query rows of every sequence
             cfg = rt.KernelConfig(kind=rt.KIND_ATTN_PACKED, dtype=dtype_tag, head_dim=D, head_dim_v=DV, threads=384, smem_bytes=smem,
                                   stages=stages, mask_mode=mask_mode)
             cfg.reserved[1] = len(low.final_names)
-            self.fwd_src = rt.kernel_source("attn_fwd.cuh", prelude=low.prelude_fwd, defines={"AE_PACKED": 1})
-            self.fwd = rt.compile_module(self.fwd_src, "ae_attn_fwd", cfg)
+            self.fwd_src = rt.kernel_source("attn_packed.cuh", prelude=low.prelude_fwd)
+            self.fwd = rt.compile_module(self.fwd_src, "ae_attn_packed", cfg)
         elif self.fwd_pair:
             pstages = int(os.environ.get("AE_B200_FWD_PAIR_STAGES", self.tuned.get("fwd_pair_stages", 5)))
             smem = 128 * D * 2 + pstages * (64 * D * 2 + 128 * 64 * 2) + 512 + 2048 + 1024

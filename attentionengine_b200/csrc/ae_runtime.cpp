@@ -575,12 +575,13 @@ int ae_launch_attn_packed(void* module, const AeAttnPackedParams* p, void* strea
   // no more blocks of rows than this whatever the lengths: a sequence of n positions has at most n / rows + 1
   auto blocks = [&](int rows) { return (int64_t)p->T / rows + std::min(p->n_seq, p->T); };
   args.pair_mode = blocks(128) * p->Hq <= 148 ? 2 : p->Hq / p->Hkv % 2 == 0 ? 1 : 0;
-  const int64_t ctas = blocks(args.pair_mode == 0 ? 256 : 128) * (args.pair_mode == 1 ? p->Hq / 2 : p->Hq);
-  if (ctas > 0x7fffffff) {
+  const int64_t items = blocks(args.pair_mode == 0 ? 256 : 128) * (args.pair_mode == 1 ? p->Hq / 2 : p->Hq);
+  if (items > 0x3fffffff) {
     set_error("packed attention: too many q tiles for one launch");
     return AE_ERR_INVALID;
   }
-  return launch(m, (unsigned)ctas, 1, 1, &args, stream);
+  args.n_items = (int)items;
+  return launch(m, (unsigned)std::min<int64_t>(items, 148), 1, 1, &args, stream);
 }
 
 static int page_log2_of(int page_size) {

@@ -68,11 +68,11 @@ struct AeAttnFwdArgs {
   int n_intervals;
   int* row_info;
   int in_cluster;  // the n_split (2 ... 8) CTAs of a unit are a cluster and merge their partials in it
-  // Packed sequences (the same kernel built with AE_PACKED): q, k, v, o are [T, H, D] as one batch row of Sq = Skv = T positions and
-  // sequence b of B is positions cu_seqlens[b] ... cu_seqlens[b + 1].  One CTA per (two q tiles, q-head) with pair_mode 0, per (q tile, two
-  // q-heads of a kv head) with 1, per (q tile, q-head) with 2; the tiles of all sequences are found from cu_seqlens.
+  // Packed sequences (attn_packed.cuh): q, k, v, o are [T, H, D] as one batch row of Sq = Skv = T positions and sequence b of B is positions
+  // cu_seqlens[b] ... cu_seqlens[b + 1].  An item is two q tiles of a head with pair_mode 0, a q tile of two heads of a kv head with 1, a q
+  // tile of a head with 2; there are at most n_items.
   const int* cu_seqlens;  // [B + 1]
-  int pair_mode;
+  int pair_mode, n_items;
 };
 
 // ---- attention backward ------------------------------------------------------------

@@ -28,12 +28,6 @@
 #if AE_DECODE && AE_MASK_MODE != 0 && AE_MASK_MODE != 3
 #error "the decode build takes no mask, or an element-wise one (mask mode 3)"
 #endif
-#ifndef AE_PACKED
-#define AE_PACKED 0  // 1: sequences of different lengths behind each other in one batch row (AeAttnFwdArgs::cu_seqlens)
-#endif
-#if AE_PACKED && (AE_DECODE || AE_MASK_MODE == 2)
-#error "the packed build is the prompt forward, and block lists are of one length"
-#endif
 #ifndef AE_NQ
 #define AE_NQ 2  // q tiles held in shared memory; 1 in a decode build whose head units have at most 128 rows (the
                  // space goes to a third K / V stage: more bytes in flight per SM while a tile's chain runs)
@@ -76,8 +70,6 @@
 #define AE_SMEM_BAR (AE_SMEM_V + AE_STAGES * AE_V_BYTES)
 #define AE_SMEM_STEPS (AE_SMEM_BAR + 512)  // mask mode 2 only: one word per kv tile
 #define AE_MAX_KT 2048                    // kv tiles a block list may cover (4 * AE_MAX_KT bytes of shared memory)
-#define AE_SMEM_SEQ (AE_SMEM_BAR + 512)  // packed build only: {sequence, pair, start, length}, then the q-tile pairs of each sequence
-#define AE_MAX_SEQ 4096
 
 struct AeFwdBars {
   u64 q_full[2];
@@ -113,69 +105,6 @@ AE_DEVICE int ae_causal_ntiles(int qt, int n_kt) {
   int n = qt + 1;
   return n < n_kt ? n : n_kt;
 }
-
-#if AE_PACKED
-// The i-th block of `rows` query rows of the packed sequences, by the length of its walk: the last blocks of the longest sequences first, so that the
-// last CTAs to start are the shortest.  The blocks behind block L of their sequence number S(L) = sum over the sequences of
-// max(0, blocks - 1 - L), so the one that is i-th has the L with S(L) <= i < S(L - 1), by bisection.  One warp, a sequence in a lane (more than
-// 32: `more` in shared memory); `at` = {sequence, block, start, length}, or -1 for the sequence where there are not that many.
-AE_DEVICE void ae_find_block(int* at, int* more, const AeAttnFwdArgs& args, int i, int rows) {
-  const int lane = (int)lane_id(), n = args.B, T = args.Sq;
-  // positions outside the tensors would be a caller's mistake: reported, and cut to them
-  auto span = [&](int b, int& start) {
-    const int s0 = args.cu_seqlens[b], s1 = args.cu_seqlens[b + 1];
-    if ((s0 < 0 || s1 < s0 || s1 > T || (b == 0 && s0 != 0) || (b == n - 1 && s1 != T)) && args.status) atomicOr(args.status, 0x2000u);
-    start = s0 < 0 ? 0 : s0 > T ? T : s0;
-    const int end = s1 < start ? start : s1 > T ? T : s1;
-    return end - start;
-  };
-  int start = 0, len = 0;
-  if (lane < n) len = span(lane, start);
-  const int mine = (len + rows - 1) / rows;
-  int most = mine;
-  for (int b = lane + 32; b < n; b += 32) {
-    int s;
-    const int p = (span(b, s) + rows - 1) / rows;
-    more[b] = p;
-    most = most > p ? most : p;
-  }
-  most = __reduce_max_sync(0xffffffffu, most);
-  __syncwarp();
-  auto behind = [&](int L) {
-    int s = mine - 1 > L ? mine - 1 - L : 0;
-    for (int b = lane + 32; b < n; b += 32) s += more[b] - 1 > L ? more[b] - 1 - L : 0;
-    return __reduce_add_sync(0xffffffffu, s);
-  };
-  if (behind(-1) <= i) {
-    if (lane == 0) at[0] = -1;
-    return;
-  }
-  int lo = -1, hi = most, at_hi = 0;  // S(lo) > i >= S(hi) = at_hi
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1, s = behind(mid);
-    if (s > i) {
-      lo = mid;
-    } else {
-      hi = mid;
-      at_hi = s;
-    }
-  }
-  int k = i - at_hi;  // the k-th of the sequences that have a block `hi`
-  for (int b0 = 0; b0 < n; b0 += 32) {
-    const bool has = (b0 == 0 ? mine : b0 + lane < n ? more[b0 + lane] : 0) > hi;
-    const u32 m = __ballot_sync(0xffffffffu, has);
-    if (has && __popc(m & ((1u << lane) - 1u)) == k) {
-      if (b0 > 0) len = span(b0 + lane, start);
-      at[3] = len;
-      at[2] = start;
-      at[1] = hi;
-      at[0] = b0 + lane;
-    }
-    k -= __popc(m);
-    if (k < 0) break;
-  }
-}
-#endif
 
 extern "C" __global__ void __launch_bounds__(AE_NTHREADS, 1)
 ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
@@ -214,47 +143,6 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
     staged = args.n_split > 1;
   }
 #define AE_SKV skv
-#elif AE_PACKED
-#define AE_SKV skv
-  // A CTA's two q tiles are one tile of two heads where a kv head's query heads are even in number: both walk the same kv tiles, and a
-  // sequence with an odd number of tiles leaves none alone (four prompts up to 8192 tokens: 848 -> 706 us).  Otherwise they are two neighbouring
-  // tiles of a head; and where all tiles find an SM of their own, there is one.  While one warp looks for the tiles, others make the barriers
-  // (60 to 80 clk each) and take the TMEM.
-  int* const seq_at = (int*)(smem + AE_SMEM_SEQ);
-  const int n_head = args.pair_mode == 1 ? args.Hq / 2 : args.Hq;
-  if (warp == 0) {
-    ae_find_block(seq_at, seq_at + 4, args, (int)blockIdx.x / n_head, args.pair_mode == 0 ? 2 * AE_BM : AE_BM);
-  } else if (warp <= 5 && lane == 0) {
-    u64* const bar = bars->q_full;  // and the others behind it
-    for (int i = (int)warp - 1; i < 6 + 2 * AE_STAGES; i += 5) mbar_init(bar + i, 1);
-    if (warp == 1) ctl->abort = 0;
-    mbar_fence_init();
-  } else if (warp == AE_ROW_WARPS) {
-    if (lane == 0) {
-      tma_prefetch_desc(&args.tm_q);
-      tma_prefetch_desc(&args.tm_k);
-      tma_prefetch_desc(&args.tm_v);
-    }
-  } else if (warp == AE_ROW_WARPS + 1) {
-    tmem_alloc(&ctl->tmem_base, 512);
-    tmem_relinquish();
-  }
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const int b = seq_at[0];
-  if (b < 0) {
-    if (warp == AE_ROW_WARPS + 1) tmem_dealloc(ctl->tmem_base, 512);
-    return;
-  }
-  const int hq = (int)blockIdx.x % n_head * (args.pair_mode == 1 ? 2 : 1);  // of tile 0
-  const int hk = hq / (args.Hq / args.Hkv);
-  const int qt0 = args.pair_mode == 0 ? 2 * seq_at[1] : seq_at[1];
-  const int seq0 = seq_at[2];  // position of the sequence's first row in the tensors
-  const int skv = seq_at[3];
-  const int kt_off = 0;
-  // tile t: q tile qt0 + t next_qt, head hq + t next_h
-  const int next_qt = args.pair_mode == 0 ? 1 : args.pair_mode == 1 ? 0 : 1 << 24, next_h = args.pair_mode == 1 ? 1 : 0;
 #else
 #define AE_SKV args.Skv
   // One-dimensional grid: sections of args.sec (batch, q-head) units; inside a section all units' last q pair first, then
@@ -271,38 +159,26 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
   const int kt_off = 0;
 #endif
 
-#if AE_PACKED
-  const int n_qt = (skv + AE_BM - 1) / AE_BM, n_kt = n_qt, s_q = skv;
-#else
-  const int n_qt = args.n_qt, n_kt = args.n_kt, s_q = args.Sq;
-  const int seq0 = 0;
-  constexpr int next_qt = 1, next_h = 0;  // tile t: q tile qt0 + t next_qt, head hq + t next_h
-#endif
-  (void)n_kt;
-  (void)s_q;
-  (void)next_qt;
-  (void)next_h;
-
 #ifdef AE_TRACE
   const bool tr_cta = blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0;
 #endif
   // ---- kv schedule (uniform over the CTA) ---------------------------------------
   int n_steps;
 #if AE_MASK_MODE == 1
-  int n_t0 = ae_causal_ntiles(qt0, n_kt);
-  int n_t1 = (qt0 + next_qt < n_qt) ? ae_causal_ntiles(qt0 + next_qt, n_kt) : 0;
+  int n_t0 = ae_causal_ntiles(qt0, args.n_kt);
+  int n_t1 = (qt0 + 1 < args.n_qt) ? ae_causal_ntiles(qt0 + 1, args.n_kt) : 0;
   n_steps = n_t0 > n_t1 ? n_t0 : n_t1;
 #elif AE_MASK_MODE == 2
   const u32* steps = (const u32*)(smem + AE_SMEM_STEPS);
   n_steps = 0;  // read from shared memory after the set-up barrier
 #elif AE_DECODE
   int n_t0 = dec_tiles;
-  int n_t1 = (1 < n_qt) ? n_t0 : 0;
+  int n_t1 = (1 < args.n_qt) ? n_t0 : 0;
   n_steps = n_t0;
 #else
-  int n_t0 = n_kt;
-  int n_t1 = (qt0 + next_qt < n_qt) ? n_kt : 0;
-  n_steps = n_kt;
+  int n_t0 = args.n_kt;
+  int n_t1 = (qt0 + 1 < args.n_qt) ? args.n_kt : 0;
+  n_steps = args.n_kt;
 #endif
 
   // step iterator: all roles call next() in lockstep order
@@ -329,7 +205,7 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
 #if AE_MASK_MODE == 1
     // partial when the tile's last column exceeds the tile's first row
     if (walk.j * AE_BN + AE_BN - 1 > qt0 * AE_BM) st.flags |= 4u;
-    if (walk.j * AE_BN + AE_BN - 1 > (qt0 + next_qt) * AE_BM) st.flags |= 8u;
+    if (walk.j * AE_BN + AE_BN - 1 > (qt0 + 1) * AE_BM) st.flags |= 8u;
 #endif
     walk.j++;
     return true;
@@ -337,7 +213,6 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
   };
 
   // ---- setup ---------------------------------------------------------------------
-#if !AE_PACKED
   if (threadIdx.x == 0) {
     ctl->abort = 0;
     for (int i = 0; i < 2; ++i) {
@@ -361,21 +236,20 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
     }
     mbar_fence_init();
   }
-#endif
 #if AE_MASK_MODE == 2
   {
     // flag word per kv tile: bit t = tile t takes part, bit 2+t = it needs the element mask.  The lists come from the
     // caller: a count or an entry outside the tile grid empties this CTA's walk and is reported through the status word.
     u32* tab = (u32*)(smem + AE_SMEM_STEPS);
-    const int* cnt_base = args.blk_cnt + ((i64)b * args.Hq + hq) * n_qt;
-    const int* idx_base = args.blk_idx + ((i64)b * args.Hq + hq) * n_qt * (i64)n_kt;
+    const int* cnt_base = args.blk_cnt + ((i64)b * args.Hq + hq) * args.n_qt;
+    const int* idx_base = args.blk_idx + ((i64)b * args.Hq + hq) * args.n_qt * (i64)args.n_kt;
     const int n_t0 = cnt_base[qt0];
-    const int n_t1 = (qt0 + 1 < n_qt) ? cnt_base[qt0 + 1] : 0;
-    const int* list0 = idx_base + (i64)qt0 * n_kt;
-    const int* list1 = idx_base + (i64)(qt0 + 1) * n_kt;
-    bool bad = n_kt > AE_MAX_KT || n_t0 < 0 || n_t0 > n_kt || n_t1 < 0 || n_t1 > n_kt;
+    const int n_t1 = (qt0 + 1 < args.n_qt) ? cnt_base[qt0 + 1] : 0;
+    const int* list0 = idx_base + (i64)qt0 * args.n_kt;
+    const int* list1 = idx_base + (i64)(qt0 + 1) * args.n_kt;
+    bool bad = args.n_kt > AE_MAX_KT || n_t0 < 0 || n_t0 > args.n_kt || n_t1 < 0 || n_t1 > args.n_kt;
     if (!bad)
-      for (int i = threadIdx.x; i < n_kt; i += AE_NTHREADS) tab[i] = 0u;
+      for (int i = threadIdx.x; i < args.n_kt; i += AE_NTHREADS) tab[i] = 0u;
     __syncthreads();
     if (!bad) {
       for (int i = threadIdx.x; i < n_t0 + n_t1; i += AE_NTHREADS) {
@@ -383,7 +257,7 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
         const u32 e = (u32)(second ? list1[i - n_t0] : list0[i]);
         const u32 kt = e & 0x3fffffffu;
         const u32 part = (e >> 30) & 1u;
-        if (kt >= (u32)n_kt)
+        if (kt >= (u32)args.n_kt)
           bad = true;
         else
           atomicOr(&tab[kt], second ? (2u | part << 3) : (1u | part << 2));
@@ -394,16 +268,16 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
       int n = 0;
       if (!any_bad) {
         // in-place compaction: entry kt moves to a position <= kt, and a chunk is read by every lane before it is written
-        for (int base = 0; base < n_kt; base += 32) {
+        for (int base = 0; base < args.n_kt; base += 32) {
           const int kt = base + (int)lane;
-          const u32 f = kt < n_kt ? tab[kt] : 0u;
+          const u32 f = kt < args.n_kt ? tab[kt] : 0u;
           const u32 m = __ballot_sync(0xffffffffu, f != 0u);
           if (f) {
             // A kv tile listed for one q tile only is still run for both (bits 4, 5: the other tile's P is zero):
             // the MMA and TMA roles then see the step pattern of an unmasked walk, whatever the lists hold.
             u32 g = f;
             if (!(f & 1u)) g |= 1u | 16u;
-            if (!(f & 2u) && qt0 + 1 < n_qt) g |= 2u | 32u;
+            if (!(f & 2u) && qt0 + 1 < args.n_qt) g |= 2u | 32u;
             tab[n + __popc(m & ((1u << lane) - 1u))] = (u32)kt | g << 24;
           }
           n += __popc(m);
@@ -417,7 +291,6 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
     }
   }
 #endif
-#if !AE_PACKED
   if (warp == AE_ROW_WARPS + 1) {
     tmem_alloc(&ctl->tmem_base, 512);
     tmem_relinquish();
@@ -425,7 +298,6 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-#endif
   const u32 tmem = ctl->tmem_base;
 #if AE_DECODE
   ae_grid_trigger();
@@ -450,12 +322,12 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
 #if AE_DECODE
         if (t > 0 && t * AE_BM >= args.rows) break;
 #else
-        if (qt0 + t * next_qt >= n_qt) break;
+        if (qt0 + t >= args.n_qt) break;
 #endif
         mbar_arrive_expect_tx(&bars->q_full[t], AE_Q_BYTES);
         for (int dh = 0; dh < AE_D / 64; ++dh)
           tma_load_bshd(smem + AE_SMEM_Q + t * AE_Q_BYTES + dh * (AE_BM * 128), &args.tm_q, &bars->q_full[t], dh * 64,
-                      hq + t * next_h, seq0 + (qt0 + t * next_qt) * AE_BM, AE_PACKED ? 0 : b);
+                      hq, (qt0 + t) * AE_BM, b);
       }
       AeKvStep st;
 #if AE_DECODE
@@ -463,8 +335,8 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
       auto kv_row = [&](int kt) { return args.block_table ? args.block_table[(i64)b * args.max_pages + kt] * AE_BN : kt * AE_BN; };
       const int kv_b = args.block_table ? 0 : b;
 #else
-      auto kv_row = [&](int kt) { return seq0 + kt * AE_BN; };
-      const int kv_b = AE_PACKED ? 0 : b;
+      auto kv_row = [&](int kt) { return kt * AE_BN; };
+      const int kv_b = b;
 #endif
       auto load_k = [&](int stage, int row0, u64* bar) {
         for (int dh = 0; dh < AE_D / 64; ++dh)
@@ -623,18 +495,6 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
       ok = mbar_wait_w(&bars->kv_full[stage], (n / AE_STAGES) & 1, ctl, args.status, 6) && !ctl->abort;
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-#if AE_PACKED
-      // The sequence ends inside this tile: the rows behind it are the next sequence's, whose values may be anything, and a P of 0 makes
-      // a NaN of an infinity.  Zeros in their place, as the copy fills them behind the end of a tensor.
-      if (cur.kt * AE_BN + AE_BN > AE_SKV) {
-        for (int r = AE_SKV - cur.kt * AE_BN + (int)(lane >> 3); r < AE_BN; r += 4)
-#pragma unroll
-          for (int dh = 0; dh < AE_DV / 64; ++dh)
-            *(uint4*)(smem + AE_SMEM_V + stage * AE_V_BYTES + dh * (AE_BN * 128) + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-#endif
       auto tile_step = [&](auto T, u32& np) {
         constexpr int t = decltype(T)::value;
         if (!(cur.flags & (1u << t))) return;
@@ -677,7 +537,7 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
     const u32 lane_base = ((warp & 3) * 32) << 16;
     const u32 tm_s = tmem + (t ? TM_S1 : TM_S0) + lane_base;
     const u32 tm_o = tmem + (t ? TM_O1 : TM_O0) + lane_base;
-    const bool tile_valid = (qt0 + t * next_qt) < n_qt;
+    const bool tile_valid = (qt0 + t) < args.n_qt;
 #if AE_DECODE
     // packed rows: the query heads of the kv head's group (one query position), or the positions of one head;
     // rows past the last valid one compute on zero-filled Q with the indices of row 0 and are never stored
@@ -686,9 +546,9 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
     const int h_row = (args.gq > 1) ? hq * args.gq + (row_valid ? r_idx : 0) : hq;
     const int q_idx = (args.gq > 1 || !row_valid) ? 0 : r_idx;
 #else
-    const int q_idx = (qt0 + t * next_qt) * AE_BM + (int)row;
-    const bool row_valid = q_idx < s_q;
-    const int h_row = hq + t * next_h;
+    const int q_idx = (qt0 + t) * AE_BM + (int)row;
+    const bool row_valid = q_idx < args.Sq;
+    const int h_row = hq;
 #endif
 
     AeCustom cu;
@@ -824,7 +684,7 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
     // tcgen05.ld is warp-collective: every lane of the warp runs it; only the stores are per-row.
     if (tile_valid) {
       const bool store = row_valid && ok;
-      u16* orow = (u16*)args.o + (AE_PACKED ? 0 : (i64)b * args.o_sb) + (i64)(seq0 + (store ? q_idx : 0)) * args.o_ss + (i64)h_row * args.o_sh;
+      u16* orow = (u16*)args.o + (i64)b * args.o_sb + (i64)(store ? q_idx : 0) * args.o_ss + (i64)h_row * args.o_sh;
 #if AE_DECODE
       // more than one split: this split's normalised O and final row scales go to fp32 staging, merged by the combine pass
       const i64 part_row = (i64)part_slot * ((i64)args.Sq * args.Hq) + (i64)q_idx * args.Hq + h_row;
@@ -873,7 +733,7 @@ ae_attn_fwd(const __grid_constant__ AeAttnFwdArgs args) {
           else if (args.final_rs[i])
             args.final_rs[i][((i64)b * args.Hq + h_row) * args.Sq + q_idx] = fr[i];
 #else
-          args.final_rs[i][((i64)(AE_PACKED ? 0 : b) * args.Hq + h_row) * args.Sq + seq0 + q_idx] = fr[i];
+          args.final_rs[i][((i64)b * args.Hq + hq) * args.Sq + q_idx] = fr[i];
 #endif
         }
       }

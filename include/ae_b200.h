@@ -60,7 +60,7 @@ enum {
   AE_KIND_ATTN_BWD_CAST = 13,
   AE_KIND_LINEAR_SEGMENTS = 15,
   AE_KIND_ATTN_FWD_PAIR = 14, /* kernel "ae_attn_fwd_pair": launched through ae_launch_attn_fwd */
-  AE_KIND_ATTN_PACKED = 16,   /* kernel "ae_attn_fwd" built for packed sequences */
+  AE_KIND_ATTN_PACKED = 16,
   AE_KIND_PLAN_PAGES = 17,
   AE_KIND_CACHE8_WRITE = 18,
   AE_KIND_CACHE8_DECODE = 19,
