@@ -188,6 +188,18 @@ struct AttnPlan : Plan {
   int D = 0, DV = 0, n_final = 0;
   bool uses_doosum = false;
   std::vector<Custom> custom;
+  // Counters of packed calls, a pair for each stream that the engine is called on: calls on one stream run in order and leave them at 0.
+  // A capturing call takes a pair of its own, cleared in the graph: its replays may run beside other calls.
+  std::vector<std::pair<void*, Tensor>> counters;
+  Tensor counters_for(const Tensor& like, void* stream) {
+    const auto ints = like.options().dtype(at::kInt);
+    if (capturing(stream)) return at::zeros({2}, ints);
+    std::lock_guard<std::mutex> lk(mu);
+    for (auto& c : counters)
+      if (c.first == stream && c.second.device() == like.device()) return c.second;
+    counters.emplace_back(stream, at::zeros({2}, ints));
+    return counters.back().second;
+  }
 };
 
 struct Dims {
@@ -391,7 +403,10 @@ py::object attn_packed(const std::shared_ptr<AttnPlan>& plan, const Tensor& q, c
       }
       p.n_seq = (int)cu.size(0) - 1; p.T = (int)T; p.Hq = (int)Hq; p.Hkv = (int)Hkv;
       p.status = word(plan->status_for(q));
-      check(ae_launch_attn_packed(plan->fwd, &p, stream_of(q)), "ae_launch_attn_packed");
+      void* st = stream_of(q);
+      const Tensor counters = plan->counters_for(q, st);
+      p.counters = (int32_t*)counters.data_ptr();
+      check(ae_launch_attn_packed(plan->fwd, &p, st), "ae_launch_attn_packed");
     }
   }
   py::gil_scoped_acquire gil;

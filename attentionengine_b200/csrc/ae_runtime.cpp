@@ -531,7 +531,7 @@ int ae_launch_attn_fwd(void* module, const AeAttnParams* p, void* stream) {
 }
 
 int ae_launch_attn_packed(void* module, const AeAttnPackedParams* p, void* stream) {
-  if (!module || !p || !p->q || !p->k || !p->v || !p->o || !p->cu_seqlens) return AE_ERR_INVALID;
+  if (!module || !p || !p->q || !p->k || !p->v || !p->o || !p->cu_seqlens || !p->counters) return AE_ERR_INVALID;
   Module* m = (Module*)module;
   int rc = check_attn_common(m, AE_KIND_ATTN_PACKED, p->n_seq, p->Hq, p->Hkv, p->T, p->T);
   if (rc) return rc;
@@ -581,6 +581,7 @@ int ae_launch_attn_packed(void* module, const AeAttnPackedParams* p, void* strea
     return AE_ERR_INVALID;
   }
   args.n_items = (int)items;
+  args.next_item = p->counters;
   return launch(m, (unsigned)std::min<int64_t>(items, 148), 1, 1, &args, stream);
 }
 

@@ -73,6 +73,7 @@ struct AeAttnFwdArgs {
   // tile of a head with 2; there are at most n_items.
   const int* cu_seqlens;  // [B + 1]
   int pair_mode, n_items;
+  int* next_item;  // [2]: items taken behind the first of each CTA, CTAs that are done; 0 between calls
 };
 
 // ---- attention backward ------------------------------------------------------------

@@ -7,9 +7,9 @@
 //   an odd number of tiles leaves none alone and no tile idles in the last step of a causal pair.  Otherwise they are two neighbouring tiles of a head;
 //   and where every tile finds an SM of its own, there is one (args.pair_mode).  Four prompts up to 8192 tokens, 32 heads of 128 dims: 848 us
 //   with two tiles of a head, 706 with two heads.
-// * The grid is persistent: a CTA takes items (blocks of query rows, heads) in turns, longest first, every second round backwards.  Barriers and
-//   TMEM are set up once; a warp of its own finds the next item from cu_seqlens while this one runs, and its first copies and products run under
-//   this item's last row work and epilogue.  One item a CTA spent 8000 clk around 4 to 5 steps of 3000 with twelve prompts up to 1500 tokens.
+// * The grid is persistent: a CTA takes the next item (a block of query rows, its heads) when it is in the last step of one, longest first.  Barriers
+//   and TMEM are set up once; a warp of its own finds the item from cu_seqlens, and its first copies and products run under this item's last row
+//   work and epilogue.  One item a CTA spent 8000 clk around 4 to 5 steps of 3000 with twelve prompts up to 1500 tokens.
 // * The rows behind a sequence's end are another sequence's: their scores are masked, and their values are overwritten with zeros in
 //   shared memory before P V (a P of 0 times an infinity is NaN).
 //
@@ -312,9 +312,16 @@ ae_attn_packed(const __grid_constant__ AeAttnFwdArgs args) {
       // =============================== finder of items ============================
       const int n_head = args.pair_mode == 1 ? args.Hq / 2 : args.Hq, grid = (int)gridDim.x;
       for (int k = 0;; ++k) {
+        int i = (int)blockIdx.x;
+        if (k > 0) {
+          // Taken as late as hides the search, at the beginning of the last step: who is done first has the next longest (by turns that were settled
+          // beforehand the longest CTA had 18 steps where the mean was 13.6).
+          if (!mbar_wait_w(&bars->q_free, (k - 1) & 1, ctl, args.status, 14)) break;
+          if (lane == 0 && args.n_items > grid) i = grid + atomicAdd(args.next_item, 1);
+          i = args.n_items > grid ? __shfl_sync(0xffffffffu, i, 0) : args.n_items;
+        }
         if (!mbar_wait_w(&bars->item_empty[k & 1], ((k >> 1) & 1) ^ 1, ctl, args.status, 10)) break;
         AePackItem& it = bars->item[k & 1];
-        const int i = k * grid + (k & 1 ? grid - 1 - (int)blockIdx.x : (int)blockIdx.x);
         if (i < args.n_items)
           ae_find_block(it, (int*)(smem + AE_SMEM_SEQ), args, i / n_head, args.pair_mode == 0 ? 2 * AE_BM : AE_BM, k == 0);
         else if (lane == 0)
@@ -457,5 +464,10 @@ ae_attn_packed(const __grid_constant__ AeAttnFwdArgs args) {
   if (warp == AE_ROW_WARPS + 1) {
     tc_fence_after_sync();
     tmem_dealloc(tmem, 512);
+  }
+  // the last CTA leaves the counters at 0 for the next call
+  if (threadIdx.x == 0 && args.n_items > (int)gridDim.x && atomicAdd(args.next_item + 1, 1) == (int)gridDim.x - 1) {
+    args.next_item[0] = 0;
+    args.next_item[1] = 0;
   }
 }

@@ -142,7 +142,8 @@ int ae_launch_attn_fwd(void* module, const AeAttnParams* p, void* stream);
 /* ---- packed prompts -------------------------------------------------------------
  * Sequences of different lengths behind each other: sequence b is positions cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of
  * every tensor, and attends to itself alone.  cu_seqlens starts at 0 and ends at T; other values set status 0x2000 and are
- * cut to the tensors.  The lengths are read on the device.  Module kind AE_KIND_ATTN_PACKED. */
+ * cut to the tensors.  The lengths are read on the device.  `counters`: two device words, zero before the first call with them and left
+ * so by every call; calls that may run at the same time take two each.  Module kind AE_KIND_ATTN_PACKED. */
 typedef struct AeAttnPackedParams {
   const void* q;             /* [T, Hq, D]   */
   const void* k;             /* [T, Hkv, D]  */
@@ -155,6 +156,7 @@ typedef struct AeAttnPackedParams {
   int64_t custom_stride[AE_MAX_CUSTOM_INPUTS][4]; /* over (sequence, h, q, kv); the last two 0 */
   int32_t n_seq, T, Hq, Hkv;                      /* n_seq: at most 4096 */
   uint32_t* status;
+  int32_t* counters;
 } AeAttnPackedParams;
 int ae_launch_attn_packed(void* module, const AeAttnPackedParams* p, void* stream);
 
