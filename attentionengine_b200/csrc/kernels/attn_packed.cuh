@@ -7,7 +7,7 @@
 //   an odd number of tiles leaves none alone and no tile idles in the last step of a causal pair.  Otherwise they are two neighbouring tiles of a head;
 //   and where every tile finds an SM of its own, there is one (args.pair_mode).  Four prompts up to 8192 tokens, 32 heads of 128 dims: 848 us
 //   with two tiles of a head, 706 with two heads.
-// * The grid is persistent: a CTA takes the next item (a block of query rows, its heads) when it is in the last step of one, longest first.  Barriers
+// * The grid is persistent: a CTA takes the next item (a block of query rows, its heads) near the end of one, longest first.  Barriers
 //   and TMEM are set up once; a warp of its own finds the item from cu_seqlens, and its first copies and products run under this item's last row
 //   work and epilogue.  One item a CTA spent 8000 clk around 4 to 5 steps of 3000 with twelve prompts up to 1500 tokens.
 // * The rows behind a sequence's end are another sequence's: their scores are masked, and their values are overwritten with zeros in
@@ -40,6 +40,7 @@ struct AePackItem {
 struct AePackBars {
   u64 q_full[2];
   u64 q_free;               // the item's last S GEMM has read Q
+  u64 near_end;             // the item is in its last but one step
   u64 s_full[2];
   u64 o_done[2];
   u64 kv_full[AE_STAGES];   // fill n of an item: V of its step n - 1 and K of step n
@@ -154,7 +155,7 @@ ae_attn_packed(const __grid_constant__ AeAttnFwdArgs args) {
   // barriers (60 to 80 clk each, so spread over the warps) and TMEM
   {
     u64* const bar = bars->q_full;  // and the others behind it, up to item_empty
-    const int n_bar = 7 + 2 * AE_STAGES + 4;
+    const int n_bar = 8 + 2 * AE_STAGES + 4;
     if (lane == 0)
       for (int i = (int)warp; i < n_bar; i += 12) mbar_init(bar + i, i >= n_bar - 2 ? AE_PACK_READERS : 1);
     if (threadIdx.x == 0) ctl->abort = 0;
@@ -269,6 +270,7 @@ ae_attn_packed(const __grid_constant__ AeAttnFwdArgs args) {
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           if (j == w.n_steps - 1) umma_commit_w(&bars->q_free);
+          if (j == (w.n_steps > 1 ? w.n_steps - 2 : 0)) mbar_arrive_warp(&bars->near_end);
           // The sequence ends inside this tile: zeros in the place of the next one's values, as the copy fills them behind the end of a tensor.
           if (j * AE_BN + AE_BN > w.len) {
             for (int r = w.len - j * AE_BN + (int)(lane >> 3); r < AE_BN; r += 4)
@@ -314,9 +316,9 @@ ae_attn_packed(const __grid_constant__ AeAttnFwdArgs args) {
       for (int k = 0;; ++k) {
         int i = (int)blockIdx.x;
         if (k > 0) {
-          // Taken as late as hides the search, at the beginning of the last step: who is done first has the next longest (by turns that were settled
-          // beforehand the longest CTA had 18 steps where the mean was 13.6).
-          if (!mbar_wait_w(&bars->q_free, (k - 1) & 1, ctl, args.status, 14)) break;
+          // Taken as late as hides the search, in the last but one step: who is done first has the next longest.  By turns that were settled beforehand
+          // the longest CTA had 18 steps where the mean was 13.6 (twelve prompts up to 1500 tokens: 45.0 us, so 42.0).
+          if (!mbar_wait_w(&bars->near_end, (k - 1) & 1, ctl, args.status, 14)) break;
           if (lane == 0 && args.n_items > grid) i = grid + atomicAdd(args.next_item, 1);
           i = args.n_items > grid ? __shfl_sync(0xffffffffu, i, 0) : args.n_items;
         }
