@@ -582,7 +582,7 @@ int ae_launch_attn_packed(void* module, const AeAttnPackedParams* p, void* strea
   }
   args.n_items = (int)items;
   args.next_item = p->counters;
-  return launch(m, (unsigned)std::min<int64_t>(items, 148), 1, 1, &args, stream);
+  return launch_after(m, (unsigned)std::min<int64_t>(items, 148), 1, 1, &args, stream);
 }
 
 static int page_log2_of(int page_size) {
@@ -619,7 +619,7 @@ int ae_launch_plan_pages(void* module, const AePlanPagesParams* p, void* stream)
   a.n_seg = p->n_segments;
   // two tokens a thread: the sums over the rows that every CTA makes cost more than its tokens
   const int64_t ctas = std::min<int64_t>(148, std::max<int64_t>(1, ((int64_t)p->n_tokens + 511) / 512));
-  return launch(m, (unsigned)ctas, 1, 1, &a, stream);
+  return launch_after(m, (unsigned)ctas, 1, 1, &a, stream);
 }
 
 int ae_launch_cache8_write(void* module, const AeCache8WriteParams* p, void* stream) {
@@ -661,7 +661,7 @@ int ae_launch_cache8_write(void* module, const AeCache8WriteParams* p, void* str
     set_error("cache write: too many segments for one launch");
     return AE_ERR_INVALID;
   }
-  return launch(m, (unsigned)ctas, 2, 1, &a, stream);
+  return launch_after(m, (unsigned)ctas, 2, 1, &a, stream);
 }
 
 // One CTA per SM; the table of cut units, then two partials of a row tile for each warp.
@@ -792,8 +792,8 @@ int ae_launch_cache8_decode(void* module, const AeCache8DecodeParams* p, void* s
     return AE_ERR_INVALID;
   }
   a.single = !ae_cache8_decode_merges(m, p);
-  if (a.single) return launch(m, (unsigned)units, (unsigned)p->B, 1, &a, stream);
-  return launch(m, (unsigned)kC8Ctas, 1, 1, &a, stream);
+  if (a.single) return launch_after(m, (unsigned)units, (unsigned)p->B, 1, &a, stream);
+  return launch_after(m, (unsigned)kC8Ctas, 1, 1, &a, stream);
 }
 
 static int fill_bwd_args(Module* m, const AeAttnBwdParams* p, AeAttnBwdArgs* a, int q_rows, int kv_rows) {

@@ -169,6 +169,8 @@ ae_attn_packed(const __grid_constant__ AeAttnFwdArgs args) {
   __syncthreads();
   tc_fence_after_sync();
   const u32 tmem = ctl->tmem_base;
+  ae_grid_wait();  // brought up under the kernel in front; nothing has been read or written outside this CTA so far
+  ae_grid_trigger();
   const u32 TM_S0 = 0, TM_S1 = 128, TM_O0 = 256, TM_O1 = 256 + AE_DV;
 
   if (warp >= AE_ROW_WARPS) {

@@ -467,7 +467,6 @@ extern "C" __global__ void __launch_bounds__(AE_C8_THREADS, 1) ae_cache8_decode(
   if (warp == AE_WARPS) {
     if (lane == 0) {
       info->ctl.abort = 0;
-      if (!a.single) a.cuts[blockIdx.x].parts = 0;
     }
   } else if (lane == 0) {
     for (int i = 0; i < AE_C8_SLOTS; ++i) {
@@ -477,6 +476,9 @@ extern "C" __global__ void __launch_bounds__(AE_C8_THREADS, 1) ae_cache8_decode(
     mbar_fence_init();
     info->rec[2 * warp].b = info->rec[2 * warp + 1].b = -1;
   }
+  ae_grid_wait();     // brought up under the kernel in front; nothing has been read or written outside this CTA so far
+  ae_grid_trigger();  // the merge may come up beside
+  if (!a.single && threadIdx.x == AE_WARPS * 32) a.cuts[blockIdx.x].parts = 0;
   const int cta = (int)blockIdx.x;
   int tl = 0, teams = AE_WARPS, per = 1, more = 0;  // warps of a team, log2; teams of a CTA; tiles of a team, teams with one more
   int team = warp, n0, n1, cta0 = 0;
@@ -530,7 +532,6 @@ extern "C" __global__ void __launch_bounds__(AE_C8_THREADS, 1) ae_cache8_decode(
     if (n_team * AE_MIN_TILES > total) n_team = total < teams * AE_MIN_TILES ? teams : (total / AE_MIN_TILES) & ~(teams - 1);
     per = total / n_team;
     more = total - per * n_team;
-    ae_grid_trigger();  // the merge may come up beside
     if (cta * teams >= n_team) return;
     // a warp for its team, lane w of the last warp for team w
     team = warp < AE_WARPS ? warp >> tl : lane < teams ? lane : 0;

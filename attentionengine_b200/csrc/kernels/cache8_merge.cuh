@@ -10,6 +10,7 @@
 extern "C" __global__ void __launch_bounds__(128) ae_cache8_merge(const __grid_constant__ AeCache8MergeArgs a) {
   __shared__ float wt[AE_FLY][AE_RT];
   ae_grid_wait();  // brought up under the decode kernel
+  ae_grid_trigger();
   const int c = blockIdx.x, j = blockIdx.y, tid = threadIdx.x;
   const AeC8Cut u = a.cuts[c];
   if (u.parts == 0 || j >= u.heads) return;

@@ -134,6 +134,8 @@ AE_DEVICE void ae_write_part(const AeCache8WriteArgs& a, const AePageSegment seg
 #define AE_W_CTAS (8 * 128 / AE_W_THREADS)  // 64 registers: more CTAs in flight (of 128 threads: 6 take 22.2 us, 8 20.4)
 extern "C" __global__ void __launch_bounds__(AE_W_THREADS, AE_W_CTAS) ae_cache8_write(const __grid_constant__ AeCache8WriteArgs a) {
   __shared__ u32 red[AE_W_THREADS / 32];
+  ae_grid_wait();  // brought up under the kernel in front
+  ae_grid_trigger();
   const AePageSegment seg = a.segments[blockIdx.x / a.H];
   // a segment without tokens, or one that a caller made up outside the pool or the tokens: nothing is written
   if (seg.tokens <= 0 || seg.page < 0 || seg.page >= a.num_pages || seg.slot < 0 || seg.slot >= AE_PAGE || seg.tokens > AE_PAGE - seg.slot || seg.token < 0 ||

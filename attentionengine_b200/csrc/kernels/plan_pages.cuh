@@ -58,6 +58,8 @@ AE_DEVICE int ae_row_of(const int* first, int B, int i) {
 extern "C" __global__ void __launch_bounds__(AE_PLAN_THREADS) ae_plan_pages(const __grid_constant__ AePlanPagesArgs a) {
   extern __shared__ u8 smem_raw[];
   AePlanSmem& sm = *(AePlanSmem*)smem_raw;
+  ae_grid_wait();  // brought up under the kernel in front
+  ae_grid_trigger();
   const int P = 1 << a.page_log2;
   const int per = (a.B + AE_PLAN_THREADS - 1) / AE_PLAN_THREADS;  // rows of a thread
   const int r0 = min((int)threadIdx.x * per, a.B), r1 = min(r0 + per, a.B);
