@@ -29,6 +29,11 @@ AE_DEVICE u32 ae_e4m3x2(float lo, float hi) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
+AE_DEVICE u32 ae_e4m3x2_half(u32 x, u32 factor) {  // of a pair of fp16 times a pair
+  u16 r;
+  asm("{ .reg .b32 y; mul.rn.f16x2 y, %1, %2; cvt.rn.satfinite.e4m3x2.f16x2 %0, y; }" : "=h"(r) : "r"(x), "r"(factor));
+  return r;
+}
 AE_DEVICE void ae_from_e4m3x2(u32 w, float& lo, float& hi) {
   u32 h;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((u16)w));
@@ -59,13 +64,18 @@ AE_DEVICE void ae_write_part(const AeCache8WriteArgs& a, const AePageSegment seg
   const u16* const x = (const u16*)a.x[which] + (i64)h * a.x_sh[which];
   u8* const codes = a.codes[which] + (i64)seg.page * a.c_sp[which] + (i64)h * a.c_sh[which];
   float* const scale = a.scales[which] + (i64)seg.page * a.s_sp[which] + h;
-  const int n = seg.tokens * CPR;
+  // a thread's chunks lie RPI rows apart, in the same column
+  constexpr int RPI = AE_W_THREADS / CPR;
+  static_assert(AE_W_THREADS % CPR == 0, "whole rows");
+  const int row = (int)threadIdx.x / CPR, col = (int)threadIdx.x % CPR * 8, n = seg.tokens - row;  // chunk i is there if i RPI < n
+  const u16* src = x + (i64)(seg.token + row) * a.x_st[which] + col;
+  const i64 src_step = (i64)RPI * a.x_st[which];
   uint4 w[AE_W_PER];
 #pragma unroll
   for (int i = 0; i < AE_W_PER; ++i) {
-    const int c = i * AE_W_THREADS + (int)threadIdx.x;
     w[i] = make_uint4(0, 0, 0, 0);
-    if (c < n) w[i] = *(const uint4*)(x + (i64)(seg.token + c / CPR) * a.x_st[which] + (c % CPR) * 8);
+    if (i * RPI < n) w[i] = *(const uint4*)src;
+    src += src_step;
   }
   const float before = *scale;
   u32 top = 0;
@@ -112,21 +122,35 @@ AE_DEVICE void ae_write_part(const AeCache8WriteArgs& a, const AePageSegment seg
     }
   }
   const float inv = 1.f / s;  // a power of two
+  u8* dst = codes + (i64)(seg.slot + row) * a.c_st[which] + col;
+  const i64 dst_step = (i64)RPI * a.c_st[which];
+  // fp16 is scaled as it is where the factor is one of fp16's normal numbers: exact down to 2^-14, and what is smaller is the code 0
+  const bool halves = !BF16 && !special && inv <= 32768.f && inv >= 6.103515625e-5f;
+  if (halves) {
+    const u32 inv2 = pack2<0>(inv, inv);
 #pragma unroll
-  for (int i = 0; i < AE_W_PER; ++i) {
-    const int c = i * AE_W_THREADS + (int)threadIdx.x;
-    if (c >= n) continue;
-    const u32 u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-    u32 r[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      r[k] = ae_e4m3x2(unpack_lo<BF16>(u[k]) * inv, unpack_hi<BF16>(u[k]) * inv);
-      if (special) {  // the conversion saturates; an infinity is to be NaN
-        if ((u[k] & 0x7fffu) == INF) r[k] |= 0x7fu;
-        if ((u[k] >> 16 & 0x7fffu) == INF) r[k] |= 0x7f00u;
-      }
+    for (int i = 0; i < AE_W_PER; ++i) {
+      if (i * RPI < n)
+        *(uint2*)dst = make_uint2(ae_e4m3x2_half(w[i].x, inv2) | ae_e4m3x2_half(w[i].y, inv2) << 16,
+                                  ae_e4m3x2_half(w[i].z, inv2) | ae_e4m3x2_half(w[i].w, inv2) << 16);
+      dst += dst_step;
     }
-    *(uint2*)(codes + (i64)(seg.slot + c / CPR) * a.c_st[which] + (c % CPR) * 8) = make_uint2(r[0] | r[1] << 16, r[2] | r[3] << 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < AE_W_PER; ++i) {
+      const u32 u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+      u32 r[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        r[k] = ae_e4m3x2(unpack_lo<BF16>(u[k]) * inv, unpack_hi<BF16>(u[k]) * inv);
+        if (special) {  // the conversion saturates; an infinity is to be NaN
+          if ((u[k] & 0x7fffu) == INF) r[k] |= 0x7fu;
+          if ((u[k] >> 16 & 0x7fffu) == INF) r[k] |= 0x7f00u;
+        }
+      }
+      if (i * RPI < n) *(uint2*)dst = make_uint2(r[0] | r[1] << 16, r[2] | r[3] << 16);
+      dst += dst_step;
+    }
   }
   if (threadIdx.x == 0) *scale = s;
 }

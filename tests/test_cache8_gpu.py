@@ -12,7 +12,7 @@ import torch
 
 import cache8_ref as ref
 import parity
-from attentionengine_b200 import AttentionEngine, CustomIO, PagedCache8, examples, meta_tensor
+from attentionengine_b200 import AttentionEngine, CustomIO, PagedCache8, examples, meta_tensor, plan_pages
 from attentionengine_b200.runtime import AeError
 
 pytestmark = pytest.mark.gpu
@@ -71,6 +71,16 @@ def test_write_special_values(dtype):
     write_and_compare(cache, x, x.flip(0), segments)
     write_and_compare(cache, x * 0, x * 0, [[1, 0, 0, 1]])  # inf * 0: NaN everywhere it was infinite
     assert cache.k_scale[1].tolist() == [2.0 ** -64] * 2
+
+
+@pytest.mark.parametrize("dtype,exponents", [("fp16", [13, 0, -6, -7, -8, -9, -14, -20]), ("bf16", [100, 20, 0, -7, -9, -40, -70, -110])])
+def test_write_magnitudes(dtype, exponents):
+    """Pages from the top of the type's range to its bottom, small values beside large ones in each: where a scale's reciprocal is a number of
+    the type and where it is not, and scales at their lower bound."""
+    cache = PagedCache8(len(exponents), 32, 2, 64)
+    x = torch.cat([values((32, 2, 64), torch.float32, 50 + i, spread=3.0).clamp(-3, 3) * 2.0 ** e for i, e in enumerate(exponents)]).to(DT[dtype])
+    assert x.isfinite().all()
+    write_and_compare(cache, x, -x.flip(1), [[i, 0, 32 * i, 32] for i in range(len(exponents))])
 
 
 def test_a_page_that_grows_token_by_token():
@@ -356,6 +366,50 @@ def test_refusals():
 
 
 # ------------------------------------------------------------------------------------------------------------ a serving loop
+def test_a_step_in_a_graph():
+    """Plan, write and decode of a step captured as one graph, each brought up under the one in front; replayed with other lengths, keys and queries
+    it gives what the calls give."""
+    Hq, Hkv, D, page, B, dtype = 16, 4, 128, 32, 5, torch.bfloat16
+    g = torch.Generator().manual_seed(3)
+    k, v, ks, vs = filled(60, page, Hkv, D, D, 9)
+    eng = engine(Hq, Hkv, 1, D, D, dtype)
+    free, head, one = ints(list(range(40, 60))), ints([0]), ints([1] * B)
+    table, lens = ints([[8 * b + i if i < 7 else 0 for i in range(10)] for b in range(B)]), ints([1] * B)
+    q, nk, nv = (torch.zeros(B, h, D, dtype=dtype, device="cuda") for h in (Hq, Hkv, Hkv))
+
+    def step(cache, table):
+        plan = plan_pages(lens, one, table, free, head, page, B)
+        cache.write(nk, nv, plan.segments)
+        return plan, eng.decode_cache8(q.unsqueeze(1), cache, plan.block_table, plan.seq_lens)
+
+    def fresh():
+        return PagedCache8.from_tensors(*(t.clone() for t in (k, v, ks, vs)))
+
+    in_graph, its_table = fresh(), table.clone()
+    step(in_graph, its_table)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan, o = step(in_graph, its_table)
+    for now in ([1, 31, 32, 95, 200], [224, 223, 1, 64, 63], [96, 128, 7, 33, 160]):
+        lens.copy_(ints(now))
+        for t in (q, nk, nv):
+            t.copy_(torch.randn(t.shape, generator=g))
+        for a, b in zip((in_graph.k, in_graph.v, in_graph.k_scale, in_graph.v_scale), (k, v, ks, vs)):
+            a.copy_(b)
+        its_table.copy_(table)
+        graph.replay()
+        apart, want_table = fresh(), table.clone()
+        want_plan, want = step(apart, want_table)
+        torch.cuda.synchronize()
+        assert torch.equal(o, want) and torch.equal(its_table, want_table)
+        assert all(torch.equal(x, y) for x, y in zip(plan, want_plan))
+        for a, b in zip((in_graph.k, in_graph.v, in_graph.k_scale, in_graph.v_scale), (apart.k, apart.v, apart.k_scale, apart.v_scale)):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        plan.check()
+    eng.check_status()
+
+
 def test_a_served_layer_from_prompts_to_tokens():
     """examples.PagedLayers: prompts of different lengths, then tokens one by one, the pages running over several times; two layers share the
     pages.  Prompts against 64 bits on the 16-bit keys, tokens on the cached ones."""
