@@ -173,7 +173,7 @@ class PagedCache8:
 
 @functools.lru_cache(maxsize=None)
 def _write_kernel(page: int, D: int, DV: int):
-    threads = 256 if page * max(D, DV) >= 128 * 128 else 128
+    threads = max(32, page * max(D, DV) // 64)  # 64 values each: the kernel's comment
     cfg = rt.KernelConfig(kind=rt.KIND_CACHE8_WRITE, head_dim=D, head_dim_v=DV, threads=threads)
     src = rt.kernel_source("cache8_write.cuh", defines={"AE_PAGE": page, "AE_D": D, "AE_DV": DV, "AE_W_THREADS": threads})
     return rt.compile_module(src, "ae_cache8_write", cfg)
@@ -249,7 +249,7 @@ class CacheDecode8:
         cfg = rt.KernelConfig(kind=rt.KIND_CACHE8_DECODE, dtype=rt.DTYPE_BF16 if self.dtype == torch.bfloat16 else rt.DTYPE_F16,
                               head_dim=self.D, head_dim_v=self.DV, threads=32 * warps + 32, smem_bytes=smem, stages=slots,
                               mask_mode=self.low.defines["AE_MASK_MODE"])
-        cfg.reserved[0], cfg.reserved[2], cfg.reserved[3], cfg.reserved[4] = self.rt, tile, least, single
+        cfg.reserved[0], cfg.reserved[2], cfg.reserved[4] = self.rt, tile, single
         self.src = rt.kernel_source("cache8_decode.cuh", prelude=self.low.prelude_fwd, defines={
             "AE_RT": self.rt, "AE_T": tile, "AE_T_LOG2": tile.bit_length() - 1, "AE_WARPS": warps, "AE_C8_SLOTS": slots, "AE_MIN_TILES": least})
         merge_cfg = rt.KernelConfig(kind=rt.KIND_CACHE8_MERGE, dtype=cfg.dtype, head_dim=self.D, head_dim_v=self.DV, threads=128)

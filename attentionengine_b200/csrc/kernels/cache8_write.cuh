@@ -10,7 +10,9 @@
 // values are neighbours in memory.  A page is at most 128 x 128 values: the CTA holds its 16-bit values in registers between the maximum and the
 // rounding, one pass over the data.  Bound by HBM (2 bytes in and 1 out a value) once the instructions are few: the maximum is taken of the
 // 16-bit patterns without their sign, two at a time, and infinities are looked for again only where that maximum is one (or a NaN).
-// 16029 tokens of 8 heads of 128 dims (98.5 MB): 26.2 us value by value in fp32, 20.4 us so.  For a step of single tokens, latency.
+// A thread has 64 of a full page's values, eight loads on their way: 16029 tokens of 8 heads of 128 dims (98.5 MB) take 18.5 us in pages of 64
+// (5.3 TB/s; 26.2 value by value in fp32), 19.1 in pages of 32 and 19.3 in pages of 16; with half the values a thread, 20.5 (pages of 32) and
+// 20.7 (of 16), with twice as many 23.5 (of 64 and of 32).  For a step of single tokens, latency.
 #define AE_W_MAXD (AE_D > AE_DV ? AE_D : AE_DV)
 #define AE_W_CHUNKS (AE_PAGE * (AE_W_MAXD / 8))                                 // 16-byte chunks of a full page's values
 #define AE_W_PER ((AE_W_CHUNKS + AE_W_THREADS - 1) / AE_W_THREADS)
@@ -155,7 +157,7 @@ AE_DEVICE void ae_write_part(const AeCache8WriteArgs& a, const AePageSegment seg
   if (threadIdx.x == 0) *scale = s;
 }
 
-#define AE_W_CTAS (8 * 128 / AE_W_THREADS)  // 64 registers: more CTAs in flight (of 128 threads: 6 take 22.2 us, 8 20.4)
+#define AE_W_CTAS (8 * 128 / AE_W_THREADS)  // 64 registers a thread (pages of 128: 18.9 us, 20.0 with 85)
 extern "C" __global__ void __launch_bounds__(AE_W_THREADS, AE_W_CTAS) ae_cache8_write(const __grid_constant__ AeCache8WriteArgs a) {
   __shared__ u32 red[AE_W_THREADS / 32];
   ae_grid_wait();  // brought up under the kernel in front
