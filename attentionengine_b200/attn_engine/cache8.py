@@ -244,14 +244,14 @@ class CacheDecode8:
         # the room) fill an SM's shared memory.  Measured with 64 ragged rows of up to 16384 keys, 128 dims: 6 warps of four tiles 182 us,
         # 8 of three 158, 12 of two 165, 4 of three 64-key tiles 185 (cp.async; 120 since the copies are a warp's of their own).
         # A team takes two tiles at least; a unit of up to four tiles a warp is a CTA's (`single`).
-        tile, warps, slots, least, single = 4096 // max(self.D, self.DV), 8, 3 if self.rt == 8 else 2, 2, 4
+        tile, warps, fetch, slots, least, single = 4096 // max(self.D, self.DV), 8, 4, 3 if self.rt == 8 else 2, 2, 4
         smem = warps * slots * (tile * (self.D + self.DV) + tile // 8 * 4 + 16) + warps * (self.rt * (self.DV + 2) * 4 + 64) + 208 + 1024
         cfg = rt.KernelConfig(kind=rt.KIND_CACHE8_DECODE, dtype=rt.DTYPE_BF16 if self.dtype == torch.bfloat16 else rt.DTYPE_F16,
-                              head_dim=self.D, head_dim_v=self.DV, threads=32 * warps + 32, smem_bytes=smem, stages=slots,
+                              head_dim=self.D, head_dim_v=self.DV, threads=32 * (warps + fetch), smem_bytes=smem, stages=slots,
                               mask_mode=self.low.defines["AE_MASK_MODE"])
-        cfg.reserved[0], cfg.reserved[2], cfg.reserved[4] = self.rt, tile, single
+        cfg.reserved[0], cfg.reserved[2], cfg.reserved[3], cfg.reserved[4] = self.rt, tile, warps, single
         self.src = rt.kernel_source("cache8_decode.cuh", prelude=self.low.prelude_fwd, defines={
-            "AE_RT": self.rt, "AE_T": tile, "AE_T_LOG2": tile.bit_length() - 1, "AE_WARPS": warps, "AE_C8_SLOTS": slots, "AE_MIN_TILES": least})
+            "AE_RT": self.rt, "AE_T": tile, "AE_T_LOG2": tile.bit_length() - 1, "AE_WARPS": warps, "AE_FETCH": fetch, "AE_C8_SLOTS": slots, "AE_MIN_TILES": least})
         merge_cfg = rt.KernelConfig(kind=rt.KIND_CACHE8_MERGE, dtype=cfg.dtype, head_dim=self.D, head_dim_v=self.DV, threads=128)
         merge_cfg.reserved[0] = warps
         self.merge_src = rt.kernel_source("cache8_merge.cuh", defines={

@@ -671,7 +671,7 @@ static int64_t c8_cut_bytes() { return (kC8Ctas * (int64_t)sizeof(AeC8Cut) + 15)
 int64_t ae_cache8_decode_workspace(void* module) {
   const Module* m = (const Module*)module;
   if (!m || m->cfg.kind != AE_KIND_CACHE8_DECODE) return 0;
-  return c8_cut_bytes() + (int64_t)kC8Ctas * 2 * (m->cfg.threads / 32 - 1) * m->cfg.reserved[0] * (m->cfg.head_dim_v + 2) * 4;
+  return c8_cut_bytes() + (int64_t)kC8Ctas * 2 * m->cfg.reserved[3] * m->cfg.reserved[0] * (m->cfg.head_dim_v + 2) * 4;
 }
 
 int ae_cache8_decode_merges(void* module, const AeCache8DecodeParams* p) {
@@ -681,7 +681,7 @@ int ae_cache8_decode_merges(void* module, const AeCache8DecodeParams* p) {
   const int64_t rows = p->Hq > p->Hkv ? p->Hq / p->Hkv : p->Sq, rt = m->cfg.reserved[0], tile = m->cfg.reserved[2];
   const int64_t units = (int64_t)p->B * p->Hkv * ((rows + rt - 1) / rt);
   const int64_t tiles = ((int64_t)p->max_pages * p->page_size + tile - 1) / tile;
-  return units > kC8Ctas || tiles > (int64_t)m->cfg.reserved[4] * (m->cfg.threads / 32 - 1);
+  return units > kC8Ctas || tiles > (int64_t)m->cfg.reserved[4] * m->cfg.reserved[3];
 }
 
 int ae_launch_cache8_merge(void* module, const AeCache8DecodeParams* p, void* stream) {
@@ -767,7 +767,7 @@ int ae_launch_cache8_decode(void* module, const AeCache8DecodeParams* p, void* s
   }
   rc = ensure_loaded(m);
   if (rc) return rc;
-  while ((2 << a.team_log2) <= m->cfg.threads / 32 - 1 && p->Hkv % (2 << a.team_log2) == 0) ++a.team_log2;
+  while ((2 << a.team_log2) <= m->cfg.reserved[3] && p->Hkv % (2 << a.team_log2) == 0) ++a.team_log2;
   for (int i = 0; i < 2; ++i) {
     const int heads = i ? 1 << a.team_log2 : 1;
     rc = make_pages_map(&a.tm_k[i], p->k_codes, p, p->k_codes_stride, m->cfg.head_dim, m->cfg.reserved[2], heads);

@@ -18,10 +18,12 @@
 // 16-byte chunks.  P goes from the accumulators' layout to the operand's by a transpose of 8 x 8 blocks in registers.  Row g + 8 h of output
 // tile m is value dim DV/8 g + 2 m + h: a lane ends with DV/8 dims in order of two query rows.
 //
-// Copies: a ninth warp fetches, a lane for each team of warps (below), a tile's keys and values as TMA boxes: the rows of one page (all of
-// them, or AE_T) of the team's heads, with the swizzle that the reads want.  Page numbers, addresses and barriers are then one lane's instructions
-// (200 of 572 a tile when each warp fetched for itself, 300 with 16-byte cp.async), and a box is large: 16 rows of one head at a time, pages of 16
-// keys took 125 us where pages of 64 took 95.
+// Copies: warps of their own fetch a tile's keys and values as TMA boxes: the rows of one page (all of them, or AE_T) of a team's heads (below), with the
+// swizzle that the reads want.  Page numbers, addresses and barriers are then those warps' instructions (200 of 572 a tile when each warp fetched for
+// itself, 300 with 16-byte cp.async), and a box is large: 16 rows of one head at a time, pages of 16 keys took 125 us where pages of 64 took 95.  There
+// are four of them, which costs no registers (an SM's quarter has three warps either way): a copy takes one some 600 clk, and with one kv head, eight
+// teams, one fetching warp took 43 us where two take 29 and four 23; with one team it makes no difference.  A warp of a single unit (below) fetches its
+// few tiles itself, their pages read together: 9.4 us for 700 keys, 10.0 by the fetching warps.
 //
 // Work split: a team of 1, 2, 4 or 8 warps takes the same tiles of as many neighbouring heads, whose keys lie side by side in a token's row of the
 // pool: read at one time they come out of DRAM as whole rows (722 MB of eight heads' pages took 172 us head by head, without any arithmetic,
@@ -33,7 +35,7 @@
 // to know none of them.  Where the table says that few units cannot be long (args.single), each is a CTA's, without a search and a merge.
 //
 // Expects the forward prelude (AE_D, AE_DV, AE_BF16, AE_MASK_MODE 0 or 3, ae_score_mod, ae_mask), AE_RT (8 or 16: query rows of a
-// tile), AE_T, AE_WARPS, AE_C8_SLOTS, AE_MIN_TILES (of a team).
+// tile), AE_T, AE_WARPS, AE_C8_SLOTS, AE_FETCH, AE_MIN_TILES (of a team).
 
 #define AE_KPT (AE_T / 8)
 #define AE_NB (AE_RT / 8)      // column blocks: query rows 8 n ... 8 n + 7
@@ -261,7 +263,7 @@ AE_DEVICE void ae_c8_values(AeC8Rows& R, const u8* vt, const AeC8Blocks& blk, co
 #define AE_SLB (AE_KB + AE_VB)  // a slot of the ring: a tile's keys and its values
 #define AE_SCF (AE_T / 8)        // and their scales
 #define AE_REC (AE_RT * (AE_DV + 2))  // floats of a partial: output, maxima, sums
-#define AE_C8_THREADS (AE_WARPS * 32 + 32)
+#define AE_C8_THREADS ((AE_WARPS + AE_FETCH) * 32)
 #define AE_SMEM_HEAD (AE_WARPS * AE_C8_SLOTS * AE_SLB)
 #define AE_SMEM_SCALE (AE_SMEM_HEAD + AE_WARPS * AE_REC * 4)
 #define AE_SMEM_INFO (AE_SMEM_SCALE + AE_WARPS * AE_C8_SLOTS * AE_SCF * 4)
@@ -315,98 +317,132 @@ AE_DEVICE bool ae_c8_test(u64* bar, u32 parity) {
 AE_DEVICE void ae_cp4(u32 dst, const float* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
 AE_DEVICE void ae_cp16(u32 dst, const float* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 
-// The fetching warp: a lane for each team, whose interval is [n, n1) and begins at `p`.
-AE_DEVICE void ae_c8_fetch(const AeCache8DecodeArgs& a, u8* ring, float* scales, u64* full, u64* empty, AeC8Pos p, int n, int n1, int tl,
-                           const AeC8Blocks blk, AeCtaCtl* ctl) {
-  const int heads = 1 << tl, box = 16 << blk.log2;  // keys of a copy
-  const bool together = tl == a.team_log2;          // the team's heads are one box
-  int page[AE_T / 16];                              // of keys 16 i ... of the next tile
-  auto pages = [&]() {
-    const int* const row = a.table + (i64)p.b * a.table_stride;
+// Copies of a tile of keys kv0 ... and of its scales into a slot, by a whole warp.  `page`: the page of keys 16 i ... of the tile, the same in every lane.
+// The boxes are one lane's, the scales AE_C8_HANDS lanes': 64 ragged rows of up to 16384 keys take 122 us, 150 when one lane copies them all.
+#define AE_C8_HANDS 8
+AE_DEVICE void ae_c8_copy(const AeCache8DecodeArgs& a, u8* kt, float* sc, u64* full, int kv0, int head0, int len, const int (&page)[AE_T / 16], int tl,
+                          const AeC8Blocks& blk) {
+  const int lane = (int)lane_id(), heads = 1 << tl, box = 16 << blk.log2;  // box: keys of a copy
+  u8* const vt = kt + heads * AE_KB;
+  u32 want = 0, there = 0;  // blocks of 16 keys
+#pragma unroll
+  for (int i = 0; i < AE_T / 16; ++i) {
+    if (kv0 + 16 * i >= len) continue;
+    want |= 1u << i;
+    if ((u32)page[i] < (u32)a.num_pages) there |= 1u << i;
+  }
+  auto page_of = [&](int i) {
+    int x = page[0];
+#pragma unroll
+    for (int k = 1; k < AE_T / 16; ++k) x = i == k ? page[k] : x;
+    return x;
+  };
+  if (there != (1u << AE_T / 16) - 1u) {
+    for (int x = lane; x < AE_T / 8 << tl; x += 32)
+      if (!(there >> ((x >> tl) & (AE_T / 16 - 1)) & 1u)) sc[x] = 1.f;
+    if (want != there) {  // a page that is not there: zeros
+      if (lane == 0 && a.status) atomicOr(a.status, 0x1000u);
+      for (int i = 0; i < AE_T / 16; ++i) {
+        if (!((want & ~there) >> i & 1u)) continue;
+        for (int j = 0; j < heads; ++j) {
+          const int row = blk.at(i) + blk.head(j);
+          for (int x = lane; x < AE_D; x += 32) *(uint4*)(kt + row * AE_D + x * 16) = make_uint4(0, 0, 0, 0);
+          for (int x = lane; x < AE_DV; x += 32) *(uint4*)(vt + row * AE_DV + x * 16) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      fence_proxy_async_smem();
+    }
+    __syncwarp();  // what was written comes before the arrival below
+  }
+  u32 boxes = there;  // the blocks that begin one
+  if (blk.log2 > 0) boxes &= blk.log2 > 1 ? 0x11111111u : 0x55555555u;
+  if (elect_one()) {
+    mbar_arrive_expect_tx(full, (u32)(__popc(boxes) * box * heads) * (AE_D + AE_DV));
 #pragma unroll
     for (int i = 0; i < AE_T / 16; ++i) {
-      const i64 first = (i64)p.t * AE_T + 16 * i;
-      page[i] = n < n1 && first < p.len ? row[first >> a.page_log2] : -1;
+      if (!(boxes >> i & 1u)) continue;
+      const int row = (kv0 + 16 * i) & ((1 << a.page_log2) - 1);
+      if (tl == a.team_log2) {  // the heads are one box
+        tma_load_4d(kt + blk.at(i) * AE_D, &a.tm_k[1], full, 0, row, head0, page[i]);
+        tma_load_4d(vt + blk.at(i) * AE_DV, &a.tm_v[1], full, 0, row, head0, page[i]);
+      } else {
+        for (int j = 0; j < heads; ++j) {
+          tma_load_4d(kt + (blk.at(i) + blk.head(j)) * AE_D, &a.tm_k[0], full, 0, row, head0 + j, page[i]);
+          tma_load_4d(vt + (blk.at(i) + blk.head(j)) * AE_DV, &a.tm_v[0], full, 0, row, head0 + j, page[i]);
+        }
+      }
     }
-  };
-  pages();
+  }
+  __syncwarp();
+  if (lane < AE_C8_HANDS) {
+    const int log2 = tl >= 2 && a.scales16 ? tl - 2 : tl;  // copies of a block's scales
+    for (int x = lane; x < AE_T / 8 << log2; x += AE_C8_HANDS) {
+      const int i = (x >> log2) & (AE_T / 16 - 1), j = x & ((1 << log2) - 1), v = x >> log2 >= AE_T / 16;
+      if (!(there >> i & 1u)) continue;
+      const float* const src = v ? a.vs + (i64)page_of(i) * a.vs_sp + head0 : a.ks + (i64)page_of(i) * a.ks_sp + head0;
+      if (log2 < tl)
+        ae_cp16(smem_u32(sc + 4 * x), src + 4 * j);
+      else
+        ae_cp4(smem_u32(sc + x), src + j);
+    }
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(full)) : "memory");
+  }
+  __syncwarp();
+}
+// Pages of a tile's blocks of 16 keys.
+AE_DEVICE void ae_c8_pages(int (&page)[AE_T / 16], const AeCache8DecodeArgs& a, const AeC8Pos& p, bool is) {
+  const int* const row = a.table + (i64)p.b * a.table_stride;
+#pragma unroll
+  for (int i = 0; i < AE_T / 16; ++i) {
+    const i64 first = (i64)p.t * AE_T + 16 * i;
+    page[i] = is && first < p.len ? row[first >> a.page_log2] : -1;
+  }
+}
+// After a wait that gave up: nothing may land in the shared memory of a CTA that has left.
+AE_DEVICE void ae_c8_drain(u64* full, int fetched) {
+  const i64 t0 = clock64();
+  for (int i = fetched > AE_C8_SLOTS ? fetched - AE_C8_SLOTS : 0; i < fetched; ++i)
+    while (!ae_c8_test(&full[i % AE_C8_SLOTS], (u32)(i / AE_C8_SLOTS) & 1u) && clock64() - t0 < AE_WAIT_CYCLES) {
+    }
+}
+
+// A fetching warp, for teams `first`, first + AE_FETCH ...: a lane finds a team's tiles, whose interval is [n, n1) and begins at `p`; the copies are
+// the whole warp's.
+AE_DEVICE void ae_c8_fetch(const AeCache8DecodeArgs& a, u8* smem_raw, AeC8Info* info, int first, AeC8Pos p, int n, int n1, int tl,
+                           const AeC8Blocks blk) {
+  const int lane = (int)lane_id(), team = lane * AE_FETCH + first < AE_WARPS >> tl ? lane * AE_FETCH + first : 0;
+  int page[AE_T / 16];  // of the next tile
+  ae_c8_pages(page, a, p, n < n1);
   int slot = 0, fetched = 0;
   u32 parity = 1;  // a slot is free at first
   i64 t0 = clock64();
   while (__any_sync(0xffffffffu, n < n1)) {
-    const bool go = n < n1 && ae_c8_test(&empty[slot], parity);
-    if (!__any_sync(0xffffffffu, go)) {
+    const bool go = n < n1 && ae_c8_test(&info->empty[team][slot], parity);
+    const u32 due = __ballot_sync(0xffffffffu, go);
+    if (due == 0) {
       // no team is done with a tile: again, within a limit
-      const bool late = ctl->abort || clock64() - t0 > AE_WAIT_CYCLES;
+      const bool late = info->ctl.abort || clock64() - t0 > AE_WAIT_CYCLES;
       if (__any_sync(0xffffffffu, late)) {
-        if (ctl->abort == 0 && a.status) atomicCAS(a.status, 0u, AE_ST_TIMEOUT_BASE + 2u);
-        ctl->abort = 1;
+        if (info->ctl.abort == 0 && a.status) atomicCAS(a.status, 0u, AE_ST_TIMEOUT_BASE + 2u);
+        info->ctl.abort = 1;
         break;
       }
-      __nanosleep(64);
+      __nanosleep(300);
       continue;
     }
+    for (u32 left = due; left; left &= left - 1) {
+      const int w = __ffs(left) - 1, mine = w * AE_FETCH + first, at = __shfl_sync(0xffffffffu, slot, w), s = (mine << tl) * AE_C8_SLOTS + (at << tl);
+      int pg[AE_T / 16];
+#pragma unroll
+      for (int i = 0; i < AE_T / 16; ++i) pg[i] = __shfl_sync(0xffffffffu, page[i], w);
+      ae_c8_copy(a, smem_raw + s * AE_SLB, (float*)(smem_raw + AE_SMEM_SCALE) + s * AE_SCF, &info->full[mine][at],
+                 __shfl_sync(0xffffffffu, p.t, w) * AE_T, __shfl_sync(0xffffffffu, p.h, w) << tl, __shfl_sync(0xffffffffu, p.len, w), pg, tl, blk);
+    }
     if (go) {
-      u8* const kt = ring + slot * heads * AE_SLB;
-      u8* const vt = kt + heads * AE_KB;
-      float* const sc = scales + slot * heads * AE_SCF;
-      const int kv0 = p.t * AE_T, head0 = p.h << tl;
-      u32 there = 0;  // blocks of 16 keys
-#pragma unroll
-      for (int i = 0; i < AE_T / 16; ++i) {
-        if (kv0 + 16 * i < p.len && (u32)page[i] < (u32)a.num_pages) {
-          there |= 1u << i;
-        } else {
-          for (int j = 0; j < heads; ++j) sc[i * heads + j] = sc[(AE_T / 16 + i) * heads + j] = 1.f;
-          if (kv0 + 16 * i < p.len) {  // a page that is not there: zeros
-            if (a.status) atomicOr(a.status, 0x1000u);
-            for (int j = 0; j < heads; ++j) {
-              const int row = blk.at(i) + blk.head(j);
-              for (int x = 0; x < AE_D; ++x) *(uint4*)(kt + row * AE_D + x * 16) = make_uint4(0, 0, 0, 0);
-              for (int x = 0; x < AE_DV; ++x) *(uint4*)(vt + row * AE_DV + x * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-          }
-        }
-      }
-      u32 boxes = there;  // the blocks that begin one
-      if (blk.log2 > 0) boxes &= blk.log2 > 1 ? 0x11111111u : 0x55555555u;
-      mbar_arrive_expect_tx(&full[slot], (u32)(__popc(boxes) * box * heads) * (AE_D + AE_DV));
-#pragma unroll
-      for (int i = 0; i < AE_T / 16; ++i) {
-        if (boxes >> i & 1u) {
-          const int row = (kv0 + 16 * i) & ((1 << a.page_log2) - 1);
-          if (together) {
-            tma_load_4d(kt + blk.at(i) * AE_D, &a.tm_k[1], &full[slot], 0, row, head0, page[i]);
-            tma_load_4d(vt + blk.at(i) * AE_DV, &a.tm_v[1], &full[slot], 0, row, head0, page[i]);
-          } else {
-            for (int j = 0; j < heads; ++j) {
-              tma_load_4d(kt + (blk.at(i) + blk.head(j)) * AE_D, &a.tm_k[0], &full[slot], 0, row, head0 + j, page[i]);
-              tma_load_4d(vt + (blk.at(i) + blk.head(j)) * AE_DV, &a.tm_v[0], &full[slot], 0, row, head0 + j, page[i]);
-            }
-          }
-        }
-        if (there >> i & 1u) {
-          const float *ks = a.ks + (i64)page[i] * a.ks_sp + head0, *vs = a.vs + (i64)page[i] * a.vs_sp + head0;
-          const u32 to = smem_u32(sc + i * heads), to2 = smem_u32(sc + (AE_T / 16 + i) * heads);
-          if (heads >= 4 && a.scales16) {
-            for (int j = 0; j < heads; j += 4) {
-              ae_cp16(to + j * 4, ks + j);
-              ae_cp16(to2 + j * 4, vs + j);
-            }
-          } else {
-            for (int j = 0; j < heads; ++j) {
-              ae_cp4(to + j * 4, ks + j);
-              ae_cp4(to2 + j * 4, vs + j);
-            }
-          }
-        }
-      }
-      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[slot])) : "memory");
       ++n;
       ++fetched;
       ae_c8_next(p, a, tl);
-      pages();
+      ae_c8_pages(page, a, p, n < n1);
       if (slot == AE_C8_SLOTS - 1) {
         slot = 0;
         parity ^= 1u;
@@ -417,12 +453,7 @@ AE_DEVICE void ae_c8_fetch(const AeCache8DecodeArgs& a, u8* ring, float* scales,
     }
     __syncwarp();
   }
-  if (ctl->abort) {  // nothing may land in the shared memory of a CTA that has left
-    t0 = clock64();
-    for (int i = fetched > AE_C8_SLOTS ? fetched - AE_C8_SLOTS : 0; i < fetched; ++i)
-      while (!ae_c8_test(&full[i % AE_C8_SLOTS], (u32)(i / AE_C8_SLOTS) & 1u) && clock64() - t0 < AE_WAIT_CYCLES) {
-      }
-  }
+  if (info->ctl.abort) ae_c8_drain(info->full[team], fetched);
 }
 
 AE_DEVICE void ae_c8_store(const AeCache8DecodeArgs& a, int b, int h, int row, int d, float4 x, float l) {
@@ -464,15 +495,11 @@ extern "C" __global__ void __launch_bounds__(AE_C8_THREADS, 1) ae_cache8_decode(
   // ---- the line of tiles, and this warp's interval [n0, n1) ----
   int* const before = a.B <= AE_FEW ? info->before : (int*)smem_raw;
   // (a barrier's initialisation takes 60 to 80 clk, one lane after the other: spread over the warps)
-  if (warp == AE_WARPS) {
-    if (lane == 0) {
-      info->ctl.abort = 0;
-    }
+  if (warp >= AE_WARPS) {
+    if (warp == AE_WARPS && lane < 4) tma_prefetch_desc(lane < 2 ? &a.tm_k[lane] : &a.tm_v[lane - 2]);
+    if (warp == AE_WARPS && lane == 0) info->ctl.abort = 0;
   } else if (lane == 0) {
-    for (int i = 0; i < AE_C8_SLOTS; ++i) {
-      mbar_init(&info->full[warp][i], 2);  // the boxes, and the scales
-      if (a.single) mbar_init(&info->empty[warp][i], 1);
-    }
+    for (int i = 0; i < AE_C8_SLOTS; ++i) mbar_init(&info->full[warp][i], 1 + AE_C8_HANDS);  // the boxes, and the scales
     mbar_fence_init();
     info->rec[2 * warp].b = info->rec[2 * warp + 1].b = -1;
   }
@@ -492,7 +519,6 @@ extern "C" __global__ void __launch_bounds__(AE_C8_THREADS, 1) ae_cache8_decode(
     at.h = a.row_tiles == 1 ? cta : cta / a.row_tiles;
     at.rt = cta - at.h * a.row_tiles;
     if (warp == 0 && lane == 0 && (a.lens[at.b] < 0 || (i64)a.lens[at.b] > (i64)a.max_pages << a.page_log2) && a.status) atomicOr(a.status, 0x800u);
-    if (warp == AE_WARPS) team = lane < AE_WARPS ? lane : 0;
     n0 = at.nt * team / AE_WARPS;
     n1 = at.nt * (team + 1) / AE_WARPS;
     at.t = n0;
@@ -533,8 +559,9 @@ extern "C" __global__ void __launch_bounds__(AE_C8_THREADS, 1) ae_cache8_decode(
     per = total / n_team;
     more = total - per * n_team;
     if (cta * teams >= n_team) return;
-    // a warp for its team, lane w of the last warp for team w
-    team = warp < AE_WARPS ? warp >> tl : lane < teams ? lane : 0;
+    // a warp for its team, a lane of the fetching warps for each of theirs
+    const int theirs = lane * AE_FETCH + warp - AE_WARPS;
+    team = warp < AE_WARPS ? warp >> tl : theirs < teams ? theirs : 0;
     cta0 = cut(cta * teams);
     n0 = cut(cta * teams + team);
     n1 = cut(cta * teams + team + 1);
@@ -577,14 +604,30 @@ extern "C" __global__ void __launch_bounds__(AE_C8_THREADS, 1) ae_cache8_decode(
     const int w = ((i >> 1) << tl) + j;
     return (i & 1) ? (float*)(smem_raw + w * (AE_C8_SLOTS * AE_SLB)) : (float*)(smem_raw + AE_SMEM_HEAD) + w * AE_REC;
   };
-  if (warp == AE_WARPS) {
-    ae_c8_fetch(a, ring, scales, info->full[team], info->empty[team], at, n0, lane < teams ? n1 : n0, tl, blk, &info->ctl);
+  if (warp >= AE_WARPS) {
+    const int first = warp - AE_WARPS;
+    if (!a.single) ae_c8_fetch(a, smem_raw, info, first, at, n0, lane * AE_FETCH + first < teams ? n1 : n0, tl, blk);
   } else {
   AeC8Rows R;
+  int pages = 0, fetched = n0;  // of a single unit: lane i's page of keys 16 i ... of the warp's tiles
+  if (a.single) {
+    const i64 first = (i64)n0 * AE_T + 16 * lane;
+    pages = first < at.len && first < (i64)n1 * AE_T ? a.table[(i64)at.b * a.table_stride + (first >> a.page_log2)] : -1;
+  }
   int from = 0, slot = 0;
   u32 parity = 0;
 #pragma unroll 1
   for (int n = n0; n < n1; ++n) {
+    if (a.single) {
+      __syncwarp();  // the tile in front has been used
+      for (; fetched < n1 && fetched < n + AE_C8_SLOTS; ++fetched) {
+        int pg[AE_T / 16];
+#pragma unroll
+        for (int i = 0; i < AE_T / 16; ++i) pg[i] = __shfl_sync(0xffffffffu, pages, (fetched - n0) * (AE_T / 16) + i);
+        const int x = (fetched - n0) % AE_C8_SLOTS;
+        ae_c8_copy(a, ring + x * AE_SLB, scales + x * AE_SCF, &info->full[team][x], fetched * AE_T, at.h, at.len, pg, 0, blk);
+      }
+    }
     const int row0 = at.rt * AE_RT, kv0 = at.t * AE_T, head = (at.h << tl) + mate;
     if (n == n0 || at.t == 0) {
       ae_c8_begin(R, a, at.b, head, row0);
@@ -605,7 +648,7 @@ extern "C" __global__ void __launch_bounds__(AE_C8_THREADS, 1) ae_cache8_decode(
     ae_c8_keys(R, kt, blk, s);
     ae_c8_weights(R, s, p, kv0, at.len, scales + (slot << tl) * AE_SCF + mate, 1 << tl, at.b, head, row0, a, cu);
     ae_c8_values(R, vt, blk, p);
-    mbar_arrive_warp(&info->empty[team][slot]);
+    if (!a.single) mbar_arrive_warp(&info->empty[team][slot]);
     if (slot == AE_C8_SLOTS - 1) {
       slot = 0;
       parity ^= 1u;
@@ -633,8 +676,9 @@ extern "C" __global__ void __launch_bounds__(AE_C8_THREADS, 1) ae_cache8_decode(
           a.cuts[cta] = {team_of(n - at.t + at.nt - 1) - cta + 1, at.b, at.h << tl, at.rt, 1 << tl};
       }
     }
-    ae_c8_next(at, a, tl);
+    if (n < n1 - 1) ae_c8_next(at, a, tl);
   }
+  if (a.single && info->ctl.abort) ae_c8_drain(info->full[team], fetched - n0);
   }
   if (teams == 1) return;
   __syncthreads();
