@@ -362,9 +362,9 @@ AE_DEVICE void ae_c8_copy(const AeCache8DecodeArgs& a, u8* kt, float* sc, u64* f
     for (int i = 0; i < AE_T / 16; ++i) {
       if (!(boxes >> i & 1u)) continue;
       const int row = (kv0 + 16 * i) & ((1 << a.page_log2) - 1);
-      if (tl == a.team_log2) {  // the heads are one box
-        tma_load_4d(kt + blk.at(i) * AE_D, &a.tm_k[1], full, 0, row, head0, page[i]);
-        tma_load_4d(vt + blk.at(i) * AE_DV, &a.tm_v[1], full, 0, row, head0, page[i]);
+      if (tl == 0 || tl == a.team_log2) {  // the heads are one box
+        tma_load_4d(kt + blk.at(i) * AE_D, &a.tm_k[tl != 0], full, 0, row, head0, page[i]);
+        tma_load_4d(vt + blk.at(i) * AE_DV, &a.tm_v[tl != 0], full, 0, row, head0, page[i]);
       } else {
         for (int j = 0; j < heads; ++j) {
           tma_load_4d(kt + (blk.at(i) + blk.head(j)) * AE_D, &a.tm_k[0], full, 0, row, head0 + j, page[i]);
@@ -618,6 +618,11 @@ extern "C" __global__ void __launch_bounds__(AE_C8_THREADS, 1) ae_cache8_decode(
   u32 parity = 0;
 #pragma unroll 1
   for (int n = n0; n < n1; ++n) {
+    const int row0 = at.rt * AE_RT, kv0 = at.t * AE_T, head = (at.h << tl) + mate;
+    if (n == n0 || at.t == 0) {
+      ae_c8_begin(R, a, at.b, head, row0);
+      from = at.t;
+    }
     if (a.single) {
       __syncwarp();  // the tile in front has been used
       for (; fetched < n1 && fetched < n + AE_C8_SLOTS; ++fetched) {
@@ -627,11 +632,6 @@ extern "C" __global__ void __launch_bounds__(AE_C8_THREADS, 1) ae_cache8_decode(
         const int x = (fetched - n0) % AE_C8_SLOTS;
         ae_c8_copy(a, ring + x * AE_SLB, scales + x * AE_SCF, &info->full[team][x], fetched * AE_T, at.h, at.len, pg, 0, blk);
       }
-    }
-    const int row0 = at.rt * AE_RT, kv0 = at.t * AE_T, head = (at.h << tl) + mate;
-    if (n == n0 || at.t == 0) {
-      ae_c8_begin(R, a, at.b, head, row0);
-      from = at.t;
     }
     // a wait that gives up is reported; the CTA goes on to its end
     mbar_wait_w(&info->full[team][slot], parity, &info->ctl, a.status, 1);
@@ -699,14 +699,21 @@ extern "C" __global__ void __launch_bounds__(AE_C8_THREADS, 1) ae_cache8_decode(
       const int m0 = x / ITEMS, r = x % ITEMS / (AE_DV / 4), d = x % (AE_DV / 4) * 4;
       if (first.rt * AE_RT + r >= a.rows) continue;
       AeC8Sum s = {AE_NEG_INF, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
-      for (u32 k = has; k; k &= k - 1) s.m = fmaxf(s.m, part_of(__ffs(k) - 1, m0)[AE_RT * AE_DV + r]);
-      for (u32 k = has; k; k &= k - 1) {
-        const float* const p = part_of(__ffs(k) - 1, m0);
-        const float m = p[AE_RT * AE_DV + r], l = p[AE_RT * AE_DV + AE_RT + r];
-        if (m == AE_NEG_INF && l == 0.f) continue;  // no kept key
-        const float f = ae_exp2(m - s.m);
-        const float4 o = *(const float4*)(p + r * AE_DV + d);
-        s.l += f * l;
+      float m[2 * AE_WARPS], l[2 * AE_WARPS];  // all pieces' reads on their way together
+#pragma unroll
+      for (int k = 0; k < 2 * AE_WARPS; ++k) {
+        const float* const p = part_of(k, m0) + AE_RT * AE_DV + r;
+        m[k] = has >> k & 1u ? p[0] : AE_NEG_INF;
+        l[k] = has >> k & 1u ? p[AE_RT] : 0.f;
+        s.m = fmaxf(s.m, m[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < 2 * AE_WARPS; ++k) {
+        const bool none = m[k] == AE_NEG_INF && l[k] == 0.f;  // no kept key, or not of this unit
+        const float f = none ? 0.f : ae_exp2(m[k] - s.m);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!none) o = *(const float4*)(part_of(k, m0) + r * AE_DV + d);
+        s.l += f * l[k];
         s.o.x += f * o.x; s.o.y += f * o.y; s.o.z += f * o.z; s.o.w += f * o.w;
       }
       if (whole) {
