@@ -22,7 +22,8 @@
 // swizzle that the reads want.  Page numbers, addresses and barriers are then those warps' instructions (200 of 572 a tile when each warp fetched for
 // itself, 300 with 16-byte cp.async), and a box is large: 16 rows of one head at a time, pages of 16 keys took 125 us where pages of 64 took 95.  There
 // are four of them, which costs no registers (an SM's quarter has three warps either way): a copy takes one some 600 clk, and with one kv head, eight
-// teams, one fetching warp took 43 us where two take 29 and four 23; with one team it makes no difference.  A warp of a single unit (below) fetches its
+// teams, one fetching warp took 43 us where two take 29 and four 22; with one team it makes no difference.  What they do not need of their registers the
+// others get (16 query rows of one kv head: 38 us, 30 so).  A warp of a single unit (below) fetches its
 // few tiles itself, their pages read together: 9.4 us for 700 keys, 10.0 by the fetching warps.
 //
 // Work split: a team of 1, 2, 4 or 8 warps takes the same tiles of as many neighbouring heads, whose keys lie side by side in a token's row of the
@@ -267,6 +268,7 @@ AE_DEVICE void ae_c8_values(AeC8Rows& R, const u8* vt, const AeC8Blocks& blk, co
 #define AE_SMEM_HEAD (AE_WARPS * AE_C8_SLOTS * AE_SLB)
 #define AE_SMEM_SCALE (AE_SMEM_HEAD + AE_WARPS * AE_REC * 4)
 #define AE_SMEM_INFO (AE_SMEM_SCALE + AE_WARPS * AE_C8_SLOTS * AE_SCF * 4)
+static_assert(AE_WARPS == 8 && AE_FETCH == 4, "three warpgroups, and their registers");
 static_assert(AE_C8_SLOTS * AE_SLB >= AE_REC * 4, "a warp's last partial lies in its own slots");
 
 // A place in the line of tiles: request, heads, row tile, tile; the request's tiles and keys.
@@ -605,9 +607,12 @@ extern "C" __global__ void __launch_bounds__(AE_C8_THREADS, 1) ae_cache8_decode(
     return (i & 1) ? (float*)(smem_raw + w * (AE_C8_SLOTS * AE_SLB)) : (float*)(smem_raw + AE_SMEM_HEAD) + w * AE_REC;
   };
   if (warp >= AE_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     const int first = warp - AE_WARPS;
     if (!a.single) ae_c8_fetch(a, smem_raw, info, first, at, n0, lane * AE_FETCH + first < teams ? n1 : n0, tl, blk);
-  } else {
+    return;
+  }
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");  // 8 x 208 + 4 x 88 = 12 x 168
   AeC8Rows R;
   int pages = 0, fetched = n0;  // of a single unit: lane i's page of keys 16 i ... of the warp's tiles
   if (a.single) {
@@ -679,9 +684,8 @@ extern "C" __global__ void __launch_bounds__(AE_C8_THREADS, 1) ae_cache8_decode(
     if (n < n1 - 1) ae_c8_next(at, a, tl);
   }
   if (a.single && info->ctl.abort) ae_c8_drain(info->full[team], fetched - n0);
-  }
   if (teams == 1) return;
-  __syncthreads();
+  named_bar_sync(15, AE_WARPS * 32);
 
   // ---- cut units: the pieces of this CTA, then of all CTAs ----
   constexpr int ITEMS = AE_RT * (AE_DV / 4);
@@ -695,7 +699,7 @@ extern "C" __global__ void __launch_bounds__(AE_C8_THREADS, 1) ae_cache8_decode(
     const int to = __shfl_sync(0xffffffffu, rec.to, 31 - __clz(has));
     left &= ~has;
     const bool whole = first.from == 0 && to == first.nt, later = first.begin >= cta0;
-    for (int x = (int)threadIdx.x; x < ITEMS << tl; x += AE_C8_THREADS) {
+    for (int x = (int)threadIdx.x; x < ITEMS << tl; x += AE_WARPS * 32) {
       const int m0 = x / ITEMS, r = x % ITEMS / (AE_DV / 4), d = x % (AE_DV / 4) * 4;
       if (first.rt * AE_RT + r >= a.rows) continue;
       AeC8Sum s = {AE_NEG_INF, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
