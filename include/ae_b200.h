@@ -206,7 +206,8 @@ int ae_launch_cache8_write(void* module, const AeCache8WriteParams* p, void* str
 /* Softmax attention of Sq query positions a row (one with grouped heads) over the row's first seq_lens[b] cached keys.  A length
  * outside the table is cut to it (status 0x800), a page outside the pool counts as zeros (status 0x1000).  A row without keys gets zeros.
  * `workspace`: ae_cache8_decode_workspace(module) bytes, 16-byte aligned, with any contents.  Where ae_cache8_decode_merges says so for these
- * parameters, ae_launch_cache8_merge follows with the same ones. */
+ * parameters, ae_launch_cache8_merge follows with the same ones.  The module's config: reserved[0] query rows and [2] keys of a tile, [3] warps that
+ * multiply, [4] tiles a warp at most where a CTA does a unit alone; the merge's: reserved[0] those warps. */
 typedef struct AeCache8DecodeParams {
   const void* q;             /* [B, Sq, Hq, D] */
   void* o;                   /* [B, Sq, Hq, DV] contiguous */
