@@ -160,6 +160,7 @@ ae_attn_packed(const __grid_constant__ AeAttnFwdArgs args) {
       for (int i = (int)warp; i < n_bar; i += 12) mbar_init(bar + i, i >= n_bar - 2 ? AE_PACK_READERS : 1);
     if (threadIdx.x == 0) ctl->abort = 0;
     if (lane == 0) mbar_fence_init();
+    if (warp == AE_ROW_WARPS && lane < 3) tma_prefetch_desc(lane == 0 ? &args.tm_q : lane == 1 ? &args.tm_k : &args.tm_v);
   }
   if (warp == AE_ROW_WARPS + 1) {
     tmem_alloc(&ctl->tmem_base, 512);
@@ -178,9 +179,6 @@ ae_attn_packed(const __grid_constant__ AeAttnFwdArgs args) {
     if (warp == AE_ROW_WARPS) {
       // =============================== TMA producer ===============================
       if (lane == 0) {
-        tma_prefetch_desc(&args.tm_q);
-        tma_prefetch_desc(&args.tm_k);
-        tma_prefetch_desc(&args.tm_v);
         u32 fill = 0;
         AePackWork w;
         for (u32 k = 0;; ++k) {
