@@ -24,7 +24,7 @@
 // are four of them, which costs no registers (an SM's quarter has three warps either way): a copy takes one some 600 clk, and with one kv head, eight
 // teams, one fetching warp took 43 us where two take 29 and four 22; with one team it makes no difference.  What they do not need of their registers the
 // others get (16 query rows of one kv head: 38 us, 30 so).  A warp of a single unit (below) fetches its
-// few tiles itself, their pages read together: 9.4 us for 700 keys, 10.0 by the fetching warps.
+// few tiles itself, their pages read together: 9.4 us for 700 keys, 10.0 by the fetching warps (8.3 since the pieces' reads go together too).
 //
 // Work split: a team of 1, 2, 4 or 8 warps takes the same tiles of as many neighbouring heads, whose keys lie side by side in a token's row of the
 // pool: read at one time they come out of DRAM as whole rows (722 MB of eight heads' pages took 172 us head by head, without any arithmetic,
