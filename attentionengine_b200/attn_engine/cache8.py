@@ -242,8 +242,8 @@ class CacheDecode8:
     def _build(self):
         # 32 keys a tile at 128 dims, 64 at 64: 8 KB; eight warps with three tiles under way each (two where the partials of 16 query rows need
         # the room) fill an SM's shared memory.  Measured with 64 ragged rows of up to 16384 keys, 128 dims: 6 warps of four tiles 182 us,
-        # 8 of three 158, 12 of two 165, 4 of three 64-key tiles 185 (cp.async; 121 since the copies are those of warps of their own, for which the four fetching ones stand).
-        # A team takes two tiles at least; a unit of up to four tiles a warp is a CTA's (`single`).
+        # 8 of three 158, 12 of two 165, 4 of three 64-key tiles 185 (cp.async by each warp;
+        # 8 of three take 121 now that four warps only fetch).  A team takes two tiles at least; a unit of up to four tiles a warp is a CTA's (`single`).
         tile, warps, fetch, slots, least, single = 4096 // max(self.D, self.DV), 8, 4, 3 if self.rt == 8 else 2, 2, 4
         smem = warps * slots * (tile * (self.D + self.DV) + tile // 8 * 4 + 16) + warps * (self.rt * (self.DV + 2) * 4 + 64) + 208 + 1024
         cfg = rt.KernelConfig(kind=rt.KIND_CACHE8_DECODE, dtype=rt.DTYPE_BF16 if self.dtype == torch.bfloat16 else rt.DTYPE_F16,
