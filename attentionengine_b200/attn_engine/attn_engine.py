@@ -18,7 +18,7 @@ import torch
 
 from .. import runtime as rt
 from ..core.transform.core import (CustomIO, SymbolicArray, SymbolScalar, Var, block_mask_counts)
-from ..lower.cuda_lower import LoweredAttention, lower_attention
+from ..lower.cuda_lower import LoweredAttention, lower_attention, mask_is_causal
 from . import attn_bwd
 
 
@@ -273,10 +273,9 @@ class AttentionEngine:
         if extern_block_mask:
             mask_mode = 2
         elif packed and mask_mod is not None:
-            # positions count from the start of each sequence and lengths are the call's: causal bounds, or element by element
-            probe = block_mask_counts(mask_mod, 2, 2, _DYN_PROBE, _DYN_PROBE, "cpu", 128, 128)
-            causal_cnt = block_mask_counts(lambda b, h, q, kv: q >= kv, 1, 1, _DYN_PROBE, _DYN_PROBE, "cpu", 128, 128)
-            mask_mode = 1 if probe.shape[:2] == (1, 1) and torch.equal(probe, causal_cnt) else 3
+            # positions count from the start of each sequence and lengths are the call's: causal bounds where the mask is that
+            # comparison itself, element by element otherwise
+            mask_mode = 1 if infer_mask and mask_is_causal(mask_mod) else 3
         elif mask_mod is not None:
             if infer_mask and not dynamic:
                 cnt = block_mask_counts(mask_mod, B, Hq, Sq, Skv, "cpu", 128, 128)

@@ -529,6 +529,58 @@ def _trace_mask(mask_mod: Optional[Callable]) -> Optional[str]:
     return _e(out)
 
 
+class _Diff:
+    """An integer combination of q_idx and kv_idx, or a comparison of two (``>= 0``), for ``mask_is_causal``."""
+
+    def __init__(self, q, kv, c, holds=False):
+        self.v, self.holds = (q, kv, c), holds
+
+    @classmethod
+    def _of(cls, o):
+        if isinstance(o, cls) and not o.holds:
+            return o.v
+        if isinstance(o, int) and not isinstance(o, bool):
+            return (0, 0, o)
+        raise TypeError
+
+    def _plus(self, o, s, t, c=0, holds=False):  # s * self + t * o + c
+        return _Diff(*(s * x + t * y + z for x, y, z in zip(self._of(self), self._of(o), (0, 0, c))), holds)
+
+    __add__ = __radd__ = lambda a, o: a._plus(o, 1, 1)
+    __sub__ = lambda a, o: a._plus(o, 1, -1)
+    __rsub__ = lambda a, o: a._plus(o, -1, 1)
+    __ge__ = lambda a, o: a._plus(o, 1, -1, 0, True)
+    __gt__ = lambda a, o: a._plus(o, 1, -1, -1, True)
+    __le__ = lambda a, o: a._plus(o, -1, 1, 0, True)
+    __lt__ = lambda a, o: a._plus(o, -1, 1, -1, True)
+    __hash__ = None
+
+    def __invert__(self):
+        if not self.holds:
+            raise TypeError
+        q, kv, c = self.v
+        return _Diff(-q, -kv, -c - 1, True)
+
+    def __bool__(self):
+        raise TypeError
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        if getattr(func, "__name__", "") != "logical_not":
+            raise TypeError
+        return ~args[0]
+
+
+def mask_is_causal(mask_mod: Callable) -> bool:
+    """Whether ``mask_mod`` is the comparison q_idx >= kv_idx, in any spelling by sums and differences: known for every length.  (Counts on a
+    short sequence cannot tell it from a window or a chunk longer than that sequence.)"""
+    try:
+        r = mask_mod(object(), object(), _Diff(1, 0, 0), _Diff(0, 1, 0))
+    except Exception:  # any other operation, b and h among them
+        return False
+    return isinstance(r, _Diff) and r.holds and r.v == (1, -1, 0)
+
+
 _LD16 = """
 template <int kBf16>
 AE_DEVICE float ae_ld16(const void* p, i64 idx) {
