@@ -66,7 +66,6 @@ class H100:
     always targets B200."""
 
 
-_DYN_PROBE = 1024  # sequence length on which a dynamic-shape engine classifies its mask
 MAX_PACKED = 4096  # sequences of a packed call (AE_MAX_SEQ of attn_packed.cuh)
 MAX_LIST_KV_TILES = 2048  # kv tiles a block list may cover (AE_MAX_KT of attn_fwd.cuh): 262,144 keys
 
@@ -291,11 +290,9 @@ class AttentionEngine:
                     self.block_mask = (cnt > 0).to(torch.int8).expand(B, Hq, cnt.shape[2], cnt.shape[3])
             elif infer_mask:
                 # Dynamic shapes (named dims, reference: lower.py:626-629): the kernels do not depend on B, H or S, only
-                # the tile lists do.  The mask is classified on a probe shape: exactly causal there -> analytic bounds
-                # for every length; anything else -> lists, built per runtime shape at the first call with it.
-                probe = block_mask_counts(mask_mod, 2, 2, _DYN_PROBE, _DYN_PROBE, "cpu", 128, 128)
-                causal_cnt = block_mask_counts(lambda b, h, q, kv: q >= kv, 1, 1, _DYN_PROBE, _DYN_PROBE, "cpu", 128, 128)
-                mask_mode = 1 if probe.shape[:2] == (1, 1) and torch.equal(probe, causal_cnt) else 2
+                # the tile lists do.  The causal comparison itself -> analytic bounds for every length; anything else -> lists,
+                # built per runtime shape at the first call with it.
+                mask_mode = 1 if mask_is_causal(mask_mod) else 2
             else:
                 mask_mode = 3  # no block information: visit every tile, mask every element
         self.mask_mode = mask_mode

@@ -43,3 +43,13 @@ def test_other_comparisons(mask):
 
 def test_no_inference_when_the_caller_asks_for_none():
     assert make(examples.causal_mask, infer_mask=False).mask_mode == 3
+
+
+@pytest.mark.parametrize("name", list(LIKE_CAUSAL))
+def test_padded_batches_of_named_lengths(name):
+    """Engines of named dims: tile lists for the length of the call, which see what a mask does there."""
+    eng = make(LIKE_CAUSAL[name], packed=False)
+    assert eng.mask_mode == 2 and make(examples.causal_mask, packed=False).mask_mode == 1
+    if name == "window_1024":
+        count, index = (x.tolist() for x in eng._ensure_lists("cpu", None, 1, 2, 1536, 1536)[:2])
+        assert count[0][0] == [min(i + 1, 9) for i in range(12)] and [x & 0xffff for x in index[0][0][11][:9]] == list(range(3, 12))

@@ -35,3 +35,25 @@ def test_sequences_longer_than_the_window(name, infer):
     for n in lens:  # each sequence by itself: a long one does not hide a short one's error
         parity.check("o", o[at:at + n], want[at:at + n], torch.float16, stages=2)
         at += n
+
+
+@pytest.mark.parametrize("name", list(MASKS))
+def test_padded_batches_of_named_lengths(name):
+    """The same masks in an engine of named dims, forward and gradients (stages: P, output; for the gradients P and dS beside)."""
+    mask, S = MASKS[name], 1700
+    m = [meta_tensor("B", "H", "S", 64, dtype=torch.float16) for _ in range(3)]
+    eng = AttentionEngine(m, CustomIO({}), score_mod=lambda s, c, b, h, q, kv: s * 0.125, mask_mod=mask, online_func=examples.OnlineSoftmax())
+    g = torch.Generator().manual_seed(2)
+    q, k, v, d_o = (torch.randn(1, S, 2, 64, generator=g).half().cuda() for _ in range(4))
+    got = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = eng(*got)
+    grads = torch.autograd.grad(o, got, d_o)
+    eng.check_status()
+    i = torch.arange(S, device="cuda")
+    ref = [t.double().requires_grad_() for t in (q, k, v)]
+    x, y, z = (t.transpose(1, 2) for t in ref)
+    s = (x @ y.transpose(2, 3) * 0.125).masked_fill(~mask(0, 0, i[:, None], i[None, :]), -math.inf)
+    want = (torch.softmax(s, -1) @ z).transpose(1, 2)
+    parity.check("o", o, want, torch.float16, stages=2)
+    for name, a, b in zip(("dq", "dk", "dv"), grads, torch.autograd.grad(want, ref, d_o.double())):
+        parity.check(name, a, b, torch.float16, stages=3)
