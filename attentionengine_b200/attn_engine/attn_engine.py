@@ -223,6 +223,9 @@ class AttentionEngine:
         self.packed = bool(packed)
         if packed and (kv_shared or extern_block_mask or cache_dtype is not None):
             raise NotImplementedError("packed sequences go with neither kv_shared, extern_block_mask nor cache_dtype")
+        if packed and mask_mod is not None and str(mask_value).strip() not in ("-inf", "-float('inf')"):
+            # another value leaves the scores as they are, to be weighed by custom inputs over positions, which packed engines do not take
+            raise NotImplementedError(f"mask_value {mask_value!r}: packed sequences are masked with -inf")
         if cache_dtype is not None:
             from .cache8 import E4M3, CacheDecode8
             if cache_dtype != E4M3:

@@ -53,3 +53,9 @@ def test_padded_batches_of_named_lengths(name):
     if name == "window_1024":
         count, index = (x.tolist() for x in eng._ensure_lists("cpu", None, 1, 2, 1536, 1536)[:2])
         assert count[0][0] == [min(i + 1, 9) for i in range(12)] and [x & 0xffff for x in index[0][0][11][:9]] == list(range(3, 12))
+
+
+def test_a_mask_that_would_not_be_applied_is_refused():
+    with pytest.raises(NotImplementedError, match="-inf"):
+        make(examples.causal_mask, mask_value="0")
+    make(None, mask_value="0")
