@@ -313,7 +313,7 @@ class AttentionEngine:
         stages = int(tuned_config.get("stages", 2))
         low = lower_attention(score_mod, mask_mod, online_func, self.custom_fwd_inputs, D=D, DV=DV,
                               bf16=self.dtype == torch.bfloat16, mask_mode=mask_mode, stages=stages,
-                              mask_value=mask_value)
+                              mask_value=mask_value, packed=packed)
         self.lowered = low
         if packed and any(d > 1 for sp in low.custom for d in sp.dim_slots):
             raise NotImplementedError("custom inputs over positions are not read beside packed sequences: batch and heads only")

@@ -15,7 +15,7 @@
 //
 // Bound by the tensor cores at 128 dims (2048 clk of products a step; what is left are the hand-overs), and by the exponentials, as many clk, at 64.
 //
-// Expects the forward prelude (AE_D, AE_DV, AE_BF16, AE_STAGES, AE_MASK_MODE 0, 1 or 3, AE_NFINAL, AE_O_SCALE_ONE, AeRow and its functions).
+// Expects the forward prelude (AE_D, AE_DV, AE_BF16, AE_STAGES, AE_MASK_MODE 0, 1 or 3, AE_NFINAL, AE_O_SCALE_ONE, AE_PACK_SCORES, AeRow and its functions).
 
 #define AE_BM 128
 #define AE_BN 128
@@ -373,13 +373,22 @@ ae_attn_packed(const __grid_constant__ AeAttnFwdArgs args) {
         float s[AE_BN];
         tmem_ld_f32x128(tm_s, s);
         const int kv0 = j * AE_BN;
-        // Compile-time columns and selects, as in attn_fwd.cuh.  Under a causal mask of -inf the sequence's end needs none of its own: a row inside
-        // the sequence keeps no key behind itself.
-#if !(AE_MASK_MODE == 1 && AE_MASK_NEG_INF)
+        // Keys behind the sequence's end do not count, whatever score_mod makes of them.  Compile-time columns and selects, as in attn_fwd.cuh.
+#if AE_PACK_SCORES == 1  // score_mod may not keep -inf (a tanh, a slope of the caller's): behind it the mask and the end
+#pragma unroll
+        for (int c = 0; c < AE_BN; ++c) s[c] = ae_score_mod(s[c], w.b, h_row, q_idx, kv0 + c, cu);
+#endif
+#if AE_PACK_SCORES == 2  // not a softmax: left out of the row reductions, and P 0
+        st.lim = w.len - kv0;
+        if (st.lim < AE_BN) {
+#pragma unroll
+          for (int c = 0; c < AE_BN; ++c) s[c] = c < st.lim ? s[c] : 0.f;
+        }
+#elif AE_MASK_MODE != 1  // (under a causal mask a row inside the sequence keeps no key behind itself)
         if (kv0 + AE_BN > w.len) {
           const int lim = w.len - kv0;
 #pragma unroll
-          for (int c = 0; c < AE_BN; ++c) s[c] = c < lim ? s[c] : (AE_MASK_NEG_INF ? -__int_as_float(0x7f800000) : 0.f);
+          for (int c = 0; c < AE_BN; ++c) s[c] = c < lim ? s[c] : -__int_as_float(0x7f800000);
         }
 #endif
 #if AE_MASK_MODE != 0 && AE_MASK_NEG_INF  // (additive mask value 0: scores stay as they are)
@@ -408,6 +417,12 @@ ae_attn_packed(const __grid_constant__ AeAttnFwdArgs args) {
 #endif
           } else {
             // P -> TMEM (16-bit pairs, column c / 2 holds kv columns c, c + 1), a block of 64 columns at a time
+#if AE_PACK_SCORES == 2
+            if (st.lim < AE_BN) {
+#pragma unroll
+              for (int c = kb * 64; c < kb * 64 + 64; ++c) p[c] = c < st.lim ? p[c] : 0.f;
+            }
+#endif
             u32 pk[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) pk[i] = pack2<AE_BF16>(p[kb * 64 + 2 * i], p[kb * 64 + 2 * i + 1]);

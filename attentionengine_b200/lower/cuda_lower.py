@@ -88,6 +88,7 @@ class Emitter:
         self.aff: dict[int, tuple] = {}               # id(value) -> (base (expr, kind), a Scal|None, b Scal|None)
         self.used_leaves: set[str] = set()
         self.lazy_max: dict[int, int] = {}  # id(Max node) -> index of the operand that is the previous state
+        self.limit: Optional[str] = None    # C++ expression: row reductions take the columns below it
         # packed f32x2 multiply-add / add in the tile loops: off unless AE_B200_PACKED=1 (measured 1 - 4 % slower in the
         # forward kernel: the pack / unpack moves cost what the halved instruction count saves)
         self.packed = tile_mode == "array" and os.environ.get("AE_B200_PACKED", "0") == "1"
@@ -231,7 +232,10 @@ class Emitter:
         if self.tile_mode != "array":
             raise NotImplementedError("row reduction outside of online_fwd")
         name = self._tmp()
-        if self.packed and t == "ReduceSum":  # N is a multiple of 8 (asserted in the functor)
+        if self.limit is not None:
+            src, neutral = src_of_c, "-__int_as_float(0x7f800000)" if t == "ReduceMax" else "0.f"
+            src_of_c = lambda col: f"({col} < {self.limit} ? {src(col)} : {neutral})"  # noqa: E731
+        elif self.packed and t == "ReduceSum":  # N is a multiple of 8 (asserted in the functor)
             # (the three-input max of PTX assembles under nvcc 12.9 but not under NVRTC 12.9, so the maximum stays scalar)
             if True:
                 self.lines.append("u64 " + ", ".join(f"{name}_{i} = 0ull" for i in range(4)) + ";")
@@ -665,6 +669,44 @@ def _lazy_max_is_invariant(online_func, raw, t_scores, rs_in, new_scores, new_rs
         return False
 
 
+def drops_neg_inf(online_func) -> bool:
+    """Whether the traced recurrence passes over columns of -inf: tile by tile over random scores, with such columns among them and
+    without, it gives the same output.  So does a softmax, also one with a term of its own in the sum; a function whose P is the score
+    itself does not."""
+    from .torch_eval import evaluate
+    try:
+        g = torch.Generator().manual_seed(13)
+        R, N, T, DV = 8, 16, 4, 4
+        tiles = [torch.randn(R, N, generator=g, dtype=torch.float64) * (1 + 2 * t) for t in range(T)]
+        vals = [torch.randn(N, DV, generator=g, dtype=torch.float64) for _ in range(T)]
+        rs = {k: SymbolScalar(k, Var(k), shape_idx=["block_M"]) for k in online_func.online_rowscales}
+        x = SymbolicArray("scores", Var("scores"), shape_idx=["block_M", "block_N"])
+        idx = [SymbolScalar(n, Var(n), require_grad=False) for n in ("b", "h", "q_idx")]
+        at = dict(zip(map(id, idx), (1.0, 2.0, torch.arange(R, dtype=torch.float64).view(R, 1))))
+        p_sym, rs_new, osc_sym = online_func.online_fwd(x, dict(rs), *idx)
+        o_sym = SymbolicArray("o", Var("o"), shape_idx=["block_M", "dimv"])
+        o_new, _ = online_func.online_fwd_epilogue(o_sym, rs, *idx)
+
+        def run(spare: int):
+            state = {k: torch.full((R, 1), float(str(v.code.name if v.code.type == "Var" else v.code.value).replace("inf", "1e30")),
+                                   dtype=torch.float64) for k, v in online_func.online_rowscales.items()}
+            o = torch.zeros(R, DV, dtype=torch.float64)
+            for s, v in zip(tiles, vals):
+                env, cache = {id(rs[k]): state[k] for k in rs} | at, {}
+                env[id(x)] = torch.cat([torch.full((R, spare), -torch.inf, dtype=torch.float64), s], 1)
+                p, osc = torch.as_tensor(evaluate(p_sym, env, cache)), evaluate(osc_sym, env, cache)
+                state = {k: torch.as_tensor(evaluate(e, env, cache), dtype=torch.float64).expand(R, 1) for k, e in rs_new.items()}
+                o = o * osc + p @ torch.cat([torch.ones(spare, DV, dtype=torch.float64), v])
+            env = {id(rs[k]): state[k] for k in rs} | at
+            env[id(o_sym)] = o
+            return torch.as_tensor(evaluate(o_new, env))
+
+        a, b = run(0), run(5)
+        return bool(torch.isfinite(b).all()) and torch.allclose(a, b, rtol=1e-9, atol=1e-9)
+    except Exception:  # what the evaluator cannot run is not taken for such a recurrence
+        return False
+
+
 def _split_recurrence(em: Emitter, p_expr: str, o_expr: str):
     """The emitted statements of online_fwd in three parts: what the row scalars behind P and o_scale need (``pre``), the
     element-wise statements that make P from them (``tiles``: (array name, element expression)), which may run column block by
@@ -695,8 +737,14 @@ def _split_recurrence(em: Emitter, p_expr: str, o_expr: str):
     return text["pre"], [(f"t{n}", em.tile_exprs[f"t{n}"]) for n in sorted(groups) if part[n] == "tiles"], text["post"]
 
 
+def _keeps_neg_inf(out, raw, env, idx_env) -> bool:
+    """Whether a traced score_mod is the raw score, times a positive constant, plus what does not depend on the key: -inf stays -inf."""
+    base, a, b = Emitter(dict(env), idx_env, n_cols="N").affine(out)
+    return base == env[id(raw)] and (a is None or (a.val is not None and a.val > 0))
+
+
 def lower_attention(score_mod, mask_mod, online_func, custom_fwd_inputs: CustomIO, *, D: int, DV: int, bf16: bool,
-                    mask_mode: int, stages: int = 2, mask_value: str = "-inf") -> LoweredAttention:
+                    mask_mode: int, stages: int = 2, mask_value: str = "-inf", packed: bool = False) -> LoweredAttention:
     """Trace the user callables and produce the kernel preludes.
 
     Order of operations per score tile follows the reference forward kernel
@@ -704,6 +752,11 @@ def lower_attention(score_mod, mask_mod, online_func, custom_fwd_inputs: CustomI
     online_fwd -> rescale O by o_scale -> O += P V; after the loop online_fwd_epilogue.  The backward
     fragments follow attn_tl.py:348-403: score_mod, OnlineFunc.forward with the saved final
     rowscales, OnlineFunc.backward (its ``scores`` argument is P), score_mod's derivative.
+
+    ``packed`` sequences end inside a tile, and what stands behind the end must not count whatever ``score_mod`` makes of it.  How the
+    kernel leaves it out (AE_PACK_SCORES): 0, where the recurrence passes over -inf and score_mod keeps it: a raw score of -inf;
+    1, where score_mod may not keep it (a bounded one, a factor that may be 0): score_mod first, then -inf, masks included; 2, for other
+    recurrences: row reductions over the columns that are there, and P of the others is 0.
     """
     specs = custom_specs(custom_fwd_inputs)
     idx_env = {"b": ("(float)b", "uniform"), "h": ("(float)h", "uniform"), "q_idx": ("(float)q_idx", "row"),
@@ -744,6 +797,8 @@ def lower_attention(score_mod, mask_mod, online_func, custom_fwd_inputs: CustomI
     row_struct = "struct AeRow {\n"
     if state_names:
         row_struct += "  float " + ", ".join(f"st_{k}" for k in state_names) + ";\n"
+    if packed:
+        row_struct += "  int lim;  // columns of this tile that are there (AE_PACK_SCORES 2)\n"
     row_struct += ("#if AE_RSPLIT > 1\n  volatile float* xch; u32 xme, xother, xbar, xn, xphase;\n#endif\n")
     row_struct += "  AE_DEVICE void init() {" + " ".join(
         f"st_{k} = {_flit(state_init[k])};" for k in state_names) + " }\n};\n"
@@ -768,16 +823,23 @@ def lower_attention(score_mod, mask_mod, online_func, custom_fwd_inputs: CustomI
     raw, t_scores = trace_score_mod()
     rs_in = {}
     env = _custom_env(specs, custom_fwd_inputs, bf16, "array")
+    env[id(raw)] = ("s[{c}]", "tile")
+    arr_idx_env = dict(idx_env)
+    arr_idx_env["kv_idx"] = ("(float)(kv0 + {c})", "tile")
+    pack_scores = 0
+    if packed:
+        pack_scores = 2 if not drops_neg_inf(online_func) else 0 if _keeps_neg_inf(t_scores, raw, env, arr_idx_env) else 1
+        if pack_scores == 1:  # the kernel hands over what score_mod has made
+            t_scores = raw
     for k in state_names:
         v = SymbolScalar(k, Var(k), shape_idx=["block_M"])
         rs_in[k] = v
         env[id(v)] = (f"st.st_{k}", "row")
-    env[id(raw)] = ("s[{c}]", "tile")
     new_scores, new_rs, o_scale = online_func.online_fwd(t_scores, dict(rs_in), sym_idx("b"), sym_idx("h"),
                                                           sym_idx("q_idx"))
-    arr_idx_env = dict(idx_env)
-    arr_idx_env["kv_idx"] = ("(float)(kv0 + {c})", "tile")
     em = Emitter(env, arr_idx_env, n_cols="N")
+    if pack_scores == 2:
+        em.limit = "st.lim"
     lazy = _lazy_max_candidates(rs_in, new_rs)
     if lazy and not specs and _lazy_max_is_invariant(online_func, raw, t_scores, rs_in, new_scores, new_rs, o_scale, lazy):
         em.lazy_max = lazy
@@ -882,6 +944,8 @@ def lower_attention(score_mod, mask_mod, online_func, custom_fwd_inputs: CustomI
         "AE_DS_USES_S": int(ds_uses_s),
         "AE_MASK_NEG_INF": int(str(mask_value).strip() in ("-inf", "-float('inf')")),
     }
+    if packed:
+        defines["AE_PACK_SCORES"] = pack_scores
     head = ("".join(f"#define {k} {v}\n" for k, v in defines.items())
             + "#ifndef AE_RSPLIT\n#define AE_RSPLIT 1  // threads per score row in the kernel that includes this\n#endif\n#ifndef AE_XCH_ROWS\n#define AE_XCH_ROWS 128  // rows that exchange partial reductions\n#endif\n"
             + "struct AeCustom;\n")
