@@ -20,6 +20,7 @@ from .. import runtime as rt
 from ..core.transform.core import (CustomIO, SymbolicArray, SymbolScalar, Var, block_mask_counts)
 from ..lower.cuda_lower import LoweredAttention, lower_attention, mask_is_causal
 from . import attn_bwd
+from .cache8 import refuse_gradients
 
 
 class OnlineFunc:
@@ -528,8 +529,6 @@ class AttentionEngine:
                 raise ValueError(f"{name} must be [T, H, D] with a contiguous last dimension")
             if t.device != q.device:
                 raise ValueError(f"{name} is on {t.device}, q on {q.device}")
-            if t.requires_grad and torch.is_grad_enabled():
-                raise NotImplementedError(f"{name} requires a gradient: packed sequences are forward only")
         if (q.shape[2], k.shape[2], v.shape[2]) != (self.D, self.D, self.DV) or k.shape[:2] != v.shape[:2] or k.shape[0] != q.shape[0] or \
                 k.shape[1] == 0 or q.shape[1] % k.shape[1] or q.shape[1] == 0:
             raise ValueError("q / k / v must be [T, Hq, D], [T, Hkv, D], [T, Hkv, DV] with the engine's head dims and Hq a multiple of Hkv")
@@ -540,6 +539,8 @@ class AttentionEngine:
             raise ValueError(f"cu_seqlens must be contiguous int32 [sequences + 1] beside q, with 1 to {MAX_PACKED} sequences")
         if len(custom) != len(self.lowered.custom):
             raise TypeError(f"expected {len(self.lowered.custom)} custom input(s) {[s.name for s in self.lowered.custom]}, got {len(custom)}")
+        refuse_gradients("packed sequences are", [("q", q), ("k", k), ("v", v)] +
+                         [(f"custom input {sp.name}", t) for sp, t in zip(self.lowered.custom, custom)])
         raise ValueError("tensors do not fit this engine")
 
     def _launch_bwd(self, q, k, v, o, d_o, finals, custom, lists=None):

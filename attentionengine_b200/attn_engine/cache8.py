@@ -78,6 +78,15 @@ def _ints(name, t, dim, device):
         raise ValueError(f"{name} must be int32 with {dim} dimension(s), the last contiguous")
 
 
+def refuse_gradients(what: str, named):
+    """Raise if one of ``named``, (name, tensor) pairs, wants a gradient of a call that has none, or carries a tangent."""
+    for name, t in named:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError(f"{name} requires a gradient: {what} forward only")
+        if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} has a tangent: {what} without derivatives")
+
+
 def _refuse_plan(old_lens, new_lens, block_table, free_pages, free_head, page_size, n_tokens):
     for name, t, dim in (("old_lens", old_lens, 1), ("new_lens", new_lens, 1), ("block_table", block_table, 2),
                          ("free_pages", free_pages, 1), ("free_head", free_head, 1)):
@@ -290,6 +299,5 @@ class CacheDecode8:
             raise ValueError(f"block_table must be [{B}, pages] and seq_lens [{B}]")
         if len(custom) != len(self.low.custom):
             raise TypeError(f"expected {len(self.low.custom)} custom input(s) {[s.name for s in self.low.custom]}, got {len(custom)}")
-        if q.requires_grad and torch.is_grad_enabled():
-            raise NotImplementedError("q requires a gradient: decode over a cache is forward only")
+        refuse_gradients("decode over a cache is", [("q", q)] + [(f"custom input {sp.name}", t) for sp, t in zip(self.low.custom, custom)])
         raise ValueError("tensors do not fit this engine")

@@ -145,6 +145,13 @@ bool needs_function(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 
+// Whether a call that is forward only takes these: custom inputs count as the others do.
+bool forward_only(std::initializer_list<const Tensor*> ts, const std::vector<Tensor>& custom) {
+  bool ok = !wants_grad(ts) && !needs_function(ts);
+  for (const Tensor& c : custom) ok = ok && !wants_grad({&c}) && !needs_function({&c});
+  return ok;
+}
+
 std::vector<Tensor> tensors_of(const py::handle& seq) {
   std::vector<Tensor> out;
   if (seq.is_none()) return out;
@@ -383,7 +390,7 @@ py::object attn_packed(const std::shared_ptr<AttnPlan>& plan, const Tensor& q, c
       v.size(0) != T || v.size(1) != Hkv || !good_ints(cu, 1, q) || cu.size(0) < 2 || cu.size(0) > 4097)
     return py::none();
   std::vector<Tensor> C = tensors_of(custom);
-  if (!row_customs(P.custom, C, cu.size(0) - 1, Hq) || wants_grad({&q, &k, &v}) || needs_function({&q, &k, &v})) return py::none();
+  if (!row_customs(P.custom, C, cu.size(0) - 1, Hq) || !forward_only({&q, &k, &v}, C)) return py::none();
   py::gil_scoped_release nogil;
   c10::cuda::CUDAGuard guard(q.device());
   at::AutoGradMode no_grad(false);
@@ -480,7 +487,7 @@ bool cache8_write(uint64_t kernel, const std::shared_ptr<Cache8>& cache, const T
       return false;
   if (k.scalar_type() != v.scalar_type() || k.size(0) != v.size(0) || k.size(0) > 0x7fffffff || k.size(2) != c.k.size(3) ||
       v.size(2) != c.v.size(3) || !good_ints(segments, 2, c.k) || segments.size(1) != 4 || (segments.size(0) > 1 && segments.stride(0) != 4) ||
-      segments.size(0) > 0x7fffffff || wants_grad({&k, &v}) || needs_function({&k, &v}))
+      segments.size(0) > 0x7fffffff || !forward_only({&k, &v}, {}))
     return false;
   py::gil_scoped_release nogil;
   c10::cuda::CUDAGuard guard(k.device());
@@ -518,7 +525,7 @@ py::object decode8(const std::shared_ptr<Decode8Plan>& plan, const std::shared_p
       lens.size(0) != B || B > 16384)
     return py::none();
   std::vector<Tensor> C = tensors_of(custom);
-  if (!row_customs(P.custom, C, B, P.Hq) || wants_grad({&q}) || needs_function({&q})) return py::none();
+  if (!row_customs(P.custom, C, B, P.Hq) || !forward_only({&q}, C)) return py::none();
   py::gil_scoped_release nogil;
   c10::cuda::CUDAGuard guard(q.device());
   at::AutoGradMode no_grad(false);
