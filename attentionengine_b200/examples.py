@@ -225,7 +225,8 @@ def retention_engine(B, H, S, D, DV, dtype):
 
 class PagedLayers:
     """The attention of a server's layers over paged 8-bit caches: ``prompts`` admits a batch of requests of different lengths, ``tokens``
-    takes one more token for each.  The layers share the pages' numbers, so one plan serves a step; nothing is read back."""
+    takes one more token for each.  The layers share the pages' numbers, so one plan serves a step; nothing is read back.  A prompt attends to itself
+    alone, so ``prompts`` is the first step: rows that hold tokens cannot get another one (a later turn, a part of a long prompt)."""
 
     def __init__(self, n_layers, Hq, Hkv, D, dtype, rows, num_pages, page_size, max_len, device="cuda"):
         self.page_size, self.rows = page_size, rows
@@ -237,8 +238,10 @@ class PagedLayers:
         self.table, self.lens = torch.zeros(rows, -(-max_len // page_size), **ints), torch.zeros(rows, **ints)
         self.one = torch.ones(rows, **ints)
         self.status = torch.zeros(1, **ints)
+        self.begun = False
 
     def _plan(self, new_lens, n_tokens):
+        self.begun = True
         plan = plan_pages(self.lens, new_lens, self.table, self.free, self.head, self.page_size, n_tokens)
         self.lens, self.head = plan.seq_lens, plan.free_head
         self.status |= plan.status
@@ -246,6 +249,8 @@ class PagedLayers:
 
     def prompts(self, layers, new_lens):
         """``layers``: (q, k, v) of every layer, [T, heads, D] with the requests' tokens behind each other; returns the layers' outputs."""
+        if self.begun:
+            raise NotImplementedError("rows hold tokens already: new prompts would attend to themselves alone, without what is cached")
         plan = self._plan(new_lens, layers[0][0].shape[0])
         out = []
         for cache, (q, k, v) in zip(self.caches, layers):
