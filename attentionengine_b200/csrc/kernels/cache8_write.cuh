@@ -3,8 +3,9 @@
 // The scale is the smallest power of two s with amax / s <= 448 (the largest e4m3 value), at least 2^-64; codes are x / s rounded to
 // nearest even.  A power of two, because e4m3 is a floating-point format: any scale gives the same relative precision, and with this
 // one x / s is exact, so the only rounding is the one to e4m3; and when a page that goes on needs a coarser scale, the codes that are there are
-// multiplied by a power of two, which changes none of them but at the bottom of the range.  amax takes the finite values: an infinity or a
-// NaN becomes NaN and does not take the others' precision.
+// multiplied by a power of two, which changes none of them but at the bottom of the range.  (Where a page came with another scale, both are
+// rounded once all the same: ae_sticky.)  amax takes the finite values: an infinity or a NaN becomes NaN and does not take the others'
+// precision.
 //
 // One CTA per (segment, head, K or V) owns the page's part for that head, so there is nothing to lock; a segment's heads run side by side, since their
 // values are neighbours in memory.  A page is at most 128 x 128 values: the CTA holds its 16-bit values in registers between the maximum and the
@@ -43,6 +44,18 @@ AE_DEVICE void ae_from_e4m3x2(u32 w, float& lo, float& hi) {
   hi = unpack_hi<0>(h);
 }
 
+// A quotient or product rounded towards 0, its last bit set where something was left (`rest`): rounded again to fewer bits it gives what the exact
+// value gives.
+AE_DEVICE float ae_sticky(float x, float rest) { return rest != 0.f ? __uint_as_float(__float_as_uint(x) | 1u) : x; }
+AE_DEVICE float ae_div_odd(float x, float y) {
+  const float q = __fdiv_rz(x, y);
+  return ae_sticky(q, fmaf(-q, y, x));
+}
+AE_DEVICE float ae_mul_odd(float x, float y) {
+  const float p = __fmul_rz(x, y);
+  return ae_sticky(p, fmaf(x, y, -p));
+}
+
 AE_DEVICE u32 ae_max2(u32 a, u32 b) {  // of two unsigned halves each
   u32 r;
   asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -57,6 +70,24 @@ AE_DEVICE u32 ae_block_max(u32 x, u32* red) {
 #pragma unroll
   for (int i = 0; i < AE_W_THREADS / 32; ++i) x = x > red[i] ? x : red[i];
   return x;
+}
+
+// The values of a segment by a scale that is not a power of two: a page that goes on may have come with one, which it keeps while it is the coarser
+// one.  Rare, so in a loop of its own over values read once more; unrolled into the loop below the divisions made the writes of a step 2 us slower.
+template <int BF16, int D>
+__device__ __noinline__ void ae_write_divided(const AeCache8WriteArgs& a, const AePageSegment seg, int h, int which, float s) {
+  const u16* const x = (const u16*)a.x[which] + (i64)h * a.x_sh[which];
+  u8* const codes = a.codes[which] + (i64)seg.page * a.c_sp[which] + (i64)h * a.c_sh[which];
+#pragma unroll 1
+  for (int c = (int)threadIdx.x; c < seg.tokens * (D / 2); c += AE_W_THREADS) {
+    const int row = c / (D / 2), col = c % (D / 2) * 2;
+    const u32 u = *(const u32*)(x + (i64)(seg.token + row) * a.x_st[which] + col);
+    const float v[2] = {unpack_lo<BF16>(u), unpack_hi<BF16>(u)};
+    u32 r = ae_e4m3x2(ae_div_odd(v[0], s), ae_div_odd(v[1], s));
+    if (fabsf(v[0]) == __int_as_float(0x7f800000)) r |= 0x7fu;  // the conversion saturates; an infinity is to be NaN
+    if (fabsf(v[1]) == __int_as_float(0x7f800000)) r |= 0x7f00u;
+    *(u16*)(codes + (i64)(seg.slot + row) * a.c_st[which] + col) = (u16)r;
+  }
 }
 
 template <int BF16, int D>
@@ -117,10 +148,13 @@ AE_DEVICE void ae_write_part(const AeCache8WriteArgs& a, const AePageSegment seg
           float e0, e1, e2, e3;
           ae_from_e4m3x2(v & 0xffffu, e0, e1);
           ae_from_e4m3x2(v >> 16, e2, e3);
-          r[k] = ae_e4m3x2(e0 * f, e1 * f) | ae_e4m3x2(e2 * f, e3 * f) << 16;
+          r[k] = ae_e4m3x2(ae_mul_odd(e0, f), ae_mul_odd(e1, f)) | ae_e4m3x2(ae_mul_odd(e2, f), ae_mul_odd(e3, f)) << 16;
         }
         *at = make_uint2(r[0], r[1]);
       }
+    } else if (__float_as_uint(s) & 0x7fffffu) {
+      ae_write_divided<BF16, D>(a, seg, h, which, s);
+      return;  // *scale stays
     }
   }
   const float inv = 1.f / s;  // a power of two
