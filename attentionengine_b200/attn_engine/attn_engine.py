@@ -124,7 +124,6 @@ class _AttnKernels:
             smem += 4 * MAX_PACKED  # the blocks of query rows of every sequence
             cfg = rt.KernelConfig(kind=rt.KIND_ATTN_PACKED, dtype=dtype_tag, head_dim=D, head_dim_v=DV, threads=384, smem_bytes=smem,
                                   stages=stages, mask_mode=mask_mode)
-            cfg.reserved[1] = len(low.final_names)
             self.fwd_src = rt.kernel_source("attn_packed.cuh", prelude=low.prelude_fwd)
             self.fwd = rt.compile_module(self.fwd_src, "ae_attn_packed", cfg)
         elif self.fwd_pair:

@@ -400,9 +400,6 @@ py::object attn_packed(const std::shared_ptr<AttnPlan>& plan, const Tensor& q, c
   if (custom_args(P.custom, C, P.dtype, T, T, true, p.custom, p.custom_stride)) {
     o = at::empty({T, Hq, P.DV}, q.options());
     if (T > 0) {
-      Tensor finals;
-      if (P.n_final) finals = at::empty({P.n_final, Hq, T}, q.options().dtype(at::kFloat));
-      for (int i = 0; i < P.n_final; ++i) p.final_rowscales[i] = (float*)finals.data_ptr() + i * Hq * T;
       p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr(); p.o = o.data_ptr();
       p.cu_seqlens = (const int32_t*)cu.data_ptr();
       for (int i = 0; i < 2; ++i) {

@@ -539,8 +539,6 @@ int ae_launch_attn_packed(void* module, const AeAttnPackedParams* p, void* strea
     set_error("at most 4096 packed sequences");
     return AE_ERR_INVALID;
   }
-  for (int i = 0; i < m->cfg.reserved[1] && i < AE_MAX_FINAL; ++i)
-    if (!p->final_rowscales[i]) return AE_ERR_INVALID;
   rc = ensure_loaded(m);
   if (rc) return rc;
   AeAttnFwdArgs args;
@@ -561,7 +559,6 @@ int ae_launch_attn_packed(void* module, const AeAttnPackedParams* p, void* strea
     set_error("output must be 16-byte aligned with strides that are multiples of 8 elements");
     return AE_ERR_INVALID;
   }
-  for (int i = 0; i < AE_MAX_FINAL; ++i) args.final_rs[i] = p->final_rowscales[i];
   for (int i = 0; i < AE_MAX_CUSTOM; ++i) {
     args.custom[i] = p->custom[i];
     for (int k = 0; k < 4; ++k) args.custom_st[i][k] = p->custom_stride[i][k];

@@ -15,7 +15,7 @@
 //
 // Bound by the tensor cores at 128 dims (2048 clk of products a step; what is left are the hand-overs), and by the exponentials, as many clk, at 64.
 //
-// Expects the forward prelude (AE_D, AE_DV, AE_BF16, AE_STAGES, AE_MASK_MODE 0, 1 or 3, AE_NFINAL, AE_O_SCALE_ONE, AE_PACK_SCORES, AeRow and its functions).
+// Expects the forward prelude (AE_D, AE_DV, AE_BF16, AE_STAGES, AE_MASK_MODE 0, 1 or 3, AE_O_SCALE_ONE, AE_PACK_SCORES, AeRow and its functions).
 
 #define AE_BM 128
 #define AE_BN 128
@@ -461,14 +461,6 @@ ae_attn_packed(const __grid_constant__ AeAttnFwdArgs args) {
             }
           }
         }
-#if AE_NFINAL > 0
-        if (store) {
-          float fr[AE_NFINAL];
-          ae_final_rowscales(st, fr);
-#pragma unroll
-          for (int i = 0; i < AE_NFINAL; ++i) args.final_rs[i][(i64)h_row * args.Sq + w.seq0 + q_idx] = fr[i];
-        }
-#endif
         tc_fence_before_sync();  // before this group's next hand-over of P, behind which the next item's P V overwrites O
       }
       mbar_arrive_warp(&bars->item_empty[k & 1]);

@@ -138,8 +138,7 @@ class LinearBwdParams(C.Structure):
 class AttnPackedParams(C.Structure):
     _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("o", C.c_void_p), ("cu_seqlens", C.c_void_p),
                 ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2), ("o_stride", C.c_int64 * 2),
-                ("final_rowscales", C.c_void_p * AE_MAX_FINAL), ("custom", C.c_void_p * AE_MAX_CUSTOM),
-                ("custom_stride", (C.c_int64 * 4) * AE_MAX_CUSTOM),
+                ("custom", C.c_void_p * AE_MAX_CUSTOM), ("custom_stride", (C.c_int64 * 4) * AE_MAX_CUSTOM),
                 ("n_seq", C.c_int32), ("T", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("status", C.c_void_p),
                 ("counters", C.c_void_p)]
 

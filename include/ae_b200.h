@@ -151,7 +151,6 @@ typedef struct AeAttnPackedParams {
   void* o;                   /* [T, Hq, DV]  */
   const int32_t* cu_seqlens; /* [n_seq + 1] device */
   int64_t q_stride[2], k_stride[2], v_stride[2], o_stride[2]; /* (position, head) */
-  float* final_rowscales[AE_MAX_FINAL_ROWSCALES];             /* each [Hq, T] fp32 */
   const void* custom[AE_MAX_CUSTOM_INPUTS];
   int64_t custom_stride[AE_MAX_CUSTOM_INPUTS][4]; /* over (sequence, h, q, kv); the last two 0 */
   int32_t n_seq, T, Hq, Hkv;                      /* n_seq: at most 4096 */

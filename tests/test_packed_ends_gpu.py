@@ -168,3 +168,13 @@ def test_sequences_do_not_meet(which, value):
         t[130:190] = value
     b = eng.prefill_packed(q, k, v, offsets(lens))
     assert torch.equal(a[:130], b[:130]) and torch.equal(a[190:], b[190:]) and a.isfinite().all()
+
+
+def test_a_call_allocates_its_output_alone():
+    eng = engine(lambda s, c, b, h, q, kv: s * 0.125, examples.OnlineSoftmax(), examples.causal_mask)
+    q, k, v = inputs(LENS, 4, 2, 64, 64, torch.float16)
+    cu = offsets(LENS)
+    eng.prefill_packed(q, k, v, cu)  # the status word and the counters are the engine's
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    o = eng.prefill_packed(q, k, v, cu)
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] - before == 1 and o.shape == q.shape
