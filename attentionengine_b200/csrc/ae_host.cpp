@@ -373,6 +373,9 @@ bool row_customs(const std::vector<Custom>& specs, const std::vector<Tensor>& ts
   return true;
 }
 
+// A stride, or for a dimension of one, whose stride says nothing, one that every check of alignment takes.
+int64_t step_of(const Tensor& t, int i) { return t.size(i) > 1 ? t.stride(i) : t.size(t.dim() - 1); }
+
 bool good_ints(const Tensor& t, int64_t dim, const Tensor& like) {
   return t.is_cuda() && t.scalar_type() == at::kInt && t.dim() == dim && t.device() == like.device() &&
          (dim == 0 || t.size(dim - 1) < 2 || t.stride(dim - 1) == 1);
@@ -403,7 +406,7 @@ py::object attn_packed(const std::shared_ptr<AttnPlan>& plan, const Tensor& q, c
       p.q = q.data_ptr(); p.k = k.data_ptr(); p.v = v.data_ptr(); p.o = o.data_ptr();
       p.cu_seqlens = (const int32_t*)cu.data_ptr();
       for (int i = 0; i < 2; ++i) {
-        p.q_stride[i] = q.stride(i); p.k_stride[i] = k.stride(i); p.v_stride[i] = v.stride(i); p.o_stride[i] = o.stride(i);
+        p.q_stride[i] = step_of(q, i); p.k_stride[i] = step_of(k, i); p.v_stride[i] = step_of(v, i); p.o_stride[i] = o.stride(i);
       }
       p.n_seq = (int)cu.size(0) - 1; p.T = (int)T; p.Hq = (int)Hq; p.Hkv = (int)Hkv;
       p.status = word(plan->status_for(q));
@@ -470,8 +473,7 @@ struct Cache8 {
 };
 
 void strides_of(const Cache8& c, int64_t (&kst)[3], int64_t (&vst)[3], int64_t& ks, int64_t& vs) {
-  strides3(c.k, kst);
-  strides3(c.v, vst);
+  for (int i = 0; i < 3; ++i) kst[i] = step_of(c.k, i), vst[i] = step_of(c.v, i);
   ks = c.ks.stride(0);
   vs = c.vs.stride(0);
 }
@@ -494,7 +496,7 @@ bool cache8_write(uint64_t kernel, const std::shared_ptr<Cache8>& cache, const T
   p.k_codes = (uint8_t*)c.k.data_ptr(); p.v_codes = (uint8_t*)c.v.data_ptr();
   p.k_scale = (float*)c.ks.data_ptr(); p.v_scale = (float*)c.vs.data_ptr();
   p.segments = (const int32_t*)segments.data_ptr();
-  for (int i = 0; i < 2; ++i) p.k_stride[i] = k.stride(i), p.v_stride[i] = v.stride(i);
+  for (int i = 0; i < 2; ++i) p.k_stride[i] = step_of(k, i), p.v_stride[i] = step_of(v, i);
   strides_of(c, p.k_codes_stride, p.v_codes_stride, p.k_scale_stride, p.v_scale_stride);
   p.n_tokens = (int)k.size(0); p.n_segments = (int)segments.size(0); p.num_pages = (int)c.k.size(0); p.H = (int)c.k.size(2);
   p.dtype = k.scalar_type() == at::kBFloat16 ? AE_DTYPE_BF16 : AE_DTYPE_F16;
@@ -536,7 +538,7 @@ py::object decode8(const std::shared_ptr<Decode8Plan>& plan, const std::shared_p
       p.k_codes = (const uint8_t*)c.k.data_ptr(); p.v_codes = (const uint8_t*)c.v.data_ptr();
       p.k_scale = (const float*)c.ks.data_ptr(); p.v_scale = (const float*)c.vs.data_ptr();
       p.block_table = (const int32_t*)table.data_ptr(); p.seq_lens = (const int32_t*)lens.data_ptr();
-      strides3(q, p.q_stride);
+      for (int i = 0; i < 3; ++i) p.q_stride[i] = step_of(q, i);
       strides_of(c, p.k_codes_stride, p.v_codes_stride, p.k_scale_stride, p.v_scale_stride);
       p.table_stride = table.stride(0);
       p.B = (int)B; p.Hq = P.Hq; p.Hkv = P.Hkv; p.Sq = P.Sq; p.max_pages = (int)table.size(1); p.num_pages = (int)c.k.size(0);
