@@ -502,7 +502,11 @@ class AttentionEngine:
     def prefill_packed(self, q, k, v, cu_seqlens, *custom):
         """Engines built with ``packed``: ``q`` [T, Hq, D], ``k`` [T, Hkv, D], ``v`` [T, Hkv, DV] hold sequences behind each other,
         sequence i at positions ``cu_seqlens[i]`` ... ``cu_seqlens[i + 1] - 1`` (int32 on the GPU, from 0 to T; up to 4096 sequences).  Each
-        attends to itself: masks and score_mod see positions in the sequence, ``b`` is its number.  Forward only."""
+        attends to itself: masks and score_mod see positions in the sequence, ``b`` is its number.  Keys that a mask drops and keys behind a
+        sequence's end have no weight under a softmax, whatever ``score_mod`` makes of them; other online functions get ``score_mod(-inf)`` for the
+        former, as in a padded batch.  A row whose mask leaves nothing gets what the epilogue makes of it (0 / 0 under a softmax), as there.
+        Causal bounds are used where ``mask_mod`` is the comparison q_idx >= kv_idx; any other mask visits every tile of its sequence.
+        Forward only."""
         if not self.packed:
             raise NotImplementedError("prefill_packed belongs to engines built with packed=True")
         if self.DV_total != self.DV and v.dim() == 3:

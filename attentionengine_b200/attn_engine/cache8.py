@@ -250,9 +250,12 @@ class CacheDecode8:
 
     def _build(self):
         # 32 keys a tile at 128 dims, 64 at 64: 8 KB; eight warps with three tiles under way each (two where the partials of 16 query rows need
-        # the room) fill an SM's shared memory.  Measured with 64 ragged rows of up to 16384 keys, 128 dims: 6 warps of four tiles 182 us,
-        # 8 of three 158, 12 of two 165, 4 of three 64-key tiles 185 (cp.async by each warp;
-        # 8 of three take 121 now that four warps only fetch).  A team takes two tiles at least; a unit of up to four tiles a warp is a CTA's (`single`).
+        # the room) fill an SM's shared memory, and four warps fetch.  In a graph: 64 ragged rows of up to 16384 keys, 8 heads of 128 dims: 125 us, with
+        # two tiles under way 135; 16 rows of 4096 keys 34.8 and 36.0.  A team takes two tiles at least: one row of 2000 keys 12.0, one at least
+        # 10.0, four 15.9; 24 rows of up to 1500 keys, 16 heads of 64 dims 15.9, 15.9 and 17.1; the others within 1 %.  A unit of up to four tiles a
+        # warp is a CTA's (`single`): one row of 700 keys 8.2 instead of 11.2, 16 rows of 1000 keys 13.0 instead of 18.0; up to eight tiles a warp, 16 rows of 2000 keys take
+        # 19.1 instead of 21.7, one row of them 15.7 instead of 12.0.  Other numbers of warps were compared on an earlier form alone, in which each warp copied its own
+        # tiles.
         tile, warps, fetch, slots, least, single = 4096 // max(self.D, self.DV), 8, 4, 3 if self.rt == 8 else 2, 2, 4
         smem = warps * slots * (tile * (self.D + self.DV) + tile // 8 * 4 + 16) + warps * (self.rt * (self.DV + 2) * 4 + 64) + 208 + 1024
         cfg = rt.KernelConfig(kind=rt.KIND_CACHE8_DECODE, dtype=rt.DTYPE_BF16 if self.dtype == torch.bfloat16 else rt.DTYPE_F16,

@@ -6,14 +6,16 @@
 // * A CTA's two q tiles are one 128-row tile of two heads where a kv head's query heads are even in number: both walk the same kv tiles, so a sequence with
 //   an odd number of tiles leaves none alone and no tile idles in the last step of a causal pair.  Otherwise they are two neighbouring tiles of a head;
 //   and where every tile finds an SM of its own, there is one (args.pair_mode).  Four prompts up to 8192 tokens, 32 heads of 128 dims: 848 us
-//   with two tiles of a head, 706 with two heads.
+//   with two tiles of a head, 706 with two heads (single calls in a burst, as first built: 680 now, 800 where calls follow each other under the power cap).
 // * The grid is persistent: a CTA takes the next item (a block of query rows, its heads) near the end of one, longest first.  Barriers
 //   and TMEM are set up once; a warp of its own finds the item from cu_seqlens, and its first copies and products run under this item's last row
 //   work and epilogue.  One item a CTA spent 8000 clk around 4 to 5 steps of 3000 with twelve prompts up to 1500 tokens.
-// * The rows behind a sequence's end are another sequence's: their scores are masked, and their values are overwritten with zeros in
-//   shared memory before P V (a P of 0 times an infinity is NaN).
+// * The rows behind a sequence's end are another sequence's: their scores do not count (AE_PACK_SCORES says how they are left out), and their values
+//   are overwritten with zeros in shared memory before P V (a P of 0 times an infinity is NaN).
 //
-// Bound by the tensor cores at 128 dims (2048 clk of products a step; what is left are the hand-overs), and by the exponentials, as many clk, at 64.
+// Long prompts are bound by the tensor cores at 128 dims (2048 clk of products a step; what is left are the hand-overs), and by the exponentials, as many
+// clk, at 64.  Short ones are not: twelve of up to 1500 tokens, 16 heads of 64 dims, take 39 us, of which the 14 steps of the longest CTA are 22; the rest
+// lies around the ends of its three or four items, where both row groups write their outputs and the next scores are yet to come.
 //
 // Expects the forward prelude (AE_D, AE_DV, AE_BF16, AE_STAGES, AE_MASK_MODE 0, 1 or 3, AE_O_SCALE_ONE, AE_PACK_SCORES, AeRow and its functions).
 
@@ -391,7 +393,7 @@ ae_attn_packed(const __grid_constant__ AeAttnFwdArgs args) {
           for (int c = 0; c < AE_BN; ++c) s[c] = c < lim ? s[c] : -__int_as_float(0x7f800000);
         }
 #endif
-#if AE_MASK_MODE != 0 && AE_MASK_NEG_INF  // (additive mask value 0: scores stay as they are)
+#if AE_MASK_MODE != 0  // (the mask value is -inf: the engine takes no other)
         if (w.partial(j, t)) {
 #pragma unroll
           for (int c = 0; c < AE_BN; ++c) s[c] = ae_mask(w.b, h_row, q_idx, kv0 + c) ? s[c] : -__int_as_float(0x7f800000);

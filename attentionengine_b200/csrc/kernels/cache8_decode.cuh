@@ -9,7 +9,7 @@
 // conversion straight into operand registers, and no accumulator takes a trip through TMEM for 8 used rows in 128.
 //
 // Precision: e4m3 is exact in fp16, so K and V enter the products as they are.  Each query row enters as fp16 times a power of two that
-// brings its largest value to [1, 2): exact for fp16 input, and for bf16 down to 2^-24 of that value.  P is fp16 in [0, 1].  Sums, maxima and the
+// brings its largest value to [1, 2): exact down to 2^-14 of that power for fp16 input and 2^-17 for bf16, below it within 2^-25 of it.  P is fp16 in [0, 1].  Sums, maxima and the
 // scales are fp32.  The value scale goes into the exponent, p' = 2^(x + log2(vs) - m) with m the maximum of x + log2(vs): no page's values are
 // scaled after the product, and the row sum takes p' / vs.
 //
