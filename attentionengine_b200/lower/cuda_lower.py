@@ -798,7 +798,7 @@ def lower_attention(score_mod, mask_mod, online_func, custom_fwd_inputs: CustomI
     if state_names:
         row_struct += "  float " + ", ".join(f"st_{k}" for k in state_names) + ";\n"
     if packed:
-        row_struct += "  int lim;  // columns of this tile that are there (AE_PACK_SCORES 2)\n"
+        row_struct += "#if AE_PACK_SCORES == 2\n  int lim;  // columns of this tile that are there\n#endif\n"
     row_struct += ("#if AE_RSPLIT > 1\n  volatile float* xch; u32 xme, xother, xbar, xn, xphase;\n#endif\n")
     row_struct += "  AE_DEVICE void init() {" + " ".join(
         f"st_{k} = {_flit(state_init[k])};" for k in state_names) + " }\n};\n"
