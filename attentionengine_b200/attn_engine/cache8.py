@@ -60,7 +60,9 @@ def plan_pages(old_lens, new_lens, block_table, free_pages, free_head, page_size
     All int32 tensors on one GPU: ``old_lens``, ``new_lens`` [B]; ``block_table`` [B, max_pages], whose new entries are written in place;
     ``free_pages`` [n] of which the first ``free_head[0]`` are taken.  Pages are handed out in the order of the rows.  ``n_tokens`` is the
     length of the packed axis, at least the sum of ``new_lens``.  Lengths are not read on the host: what does not fit is left out and
-    reported in ``status``.  ``old_lens`` and ``free_head`` are not changed; the next step's are ``plan.seq_lens`` and ``plan.free_head``."""
+    reported in ``status``.  ``old_lens`` and ``free_head`` are not changed; the next step's are ``plan.seq_lens`` and ``plan.free_head``.
+    Pages come back by the caller's hand: a row that has ended gets a length of 0, and the next step a ``free_pages`` with its pages behind those not yet
+    taken, and a head of 0."""
     if isinstance(page_size, bool) or not isinstance(page_size, int) or isinstance(n_tokens, bool) or not isinstance(n_tokens, int):
         raise TypeError("page_size and n_tokens are ints")
     r = rt.host().plan_pages(_plan_kernel().handle.value, old_lens, new_lens, block_table, free_pages, free_head, page_size, n_tokens)
