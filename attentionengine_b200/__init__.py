@@ -7,7 +7,8 @@ compiled with NVRTC and launched through the C ABI in ``include/ae_b200.h``.
 import sys as _sys
 
 from . import attn_engine, core
-from .attn_engine import AttentionEngine, LinearAttentionEngine, OnlineFunc, PagedCache8, PagePlan, plan_pages
+from .attn_engine import (AttentionEngine, CompactionPlan, ForkPlan, LinearAttentionEngine, OnlineFunc, PagedCache8, PagePlan, QKNormRope, copy_pages,
+                          plan_compaction, plan_forks, plan_pages)
 from .core import (CustomIO, SymbolicArray, SymbolicTensor, SymbolScalar, Var, create_block_mask, meta_tensor)
 
 
@@ -22,4 +23,4 @@ def install_reference_aliases():
 
 __all__ = ["AttentionEngine", "OnlineFunc", "LinearAttentionEngine", "CustomIO", "SymbolicArray", "SymbolicTensor",
            "SymbolScalar", "Var", "create_block_mask", "meta_tensor", "install_reference_aliases", "PagedCache8", "PagePlan",
-           "plan_pages"]
+           "plan_pages", "QKNormRope", "ForkPlan", "plan_forks", "CompactionPlan", "plan_compaction", "copy_pages"]

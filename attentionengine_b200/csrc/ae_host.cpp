@@ -14,6 +14,7 @@
 #include <cuda_runtime_api.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
@@ -553,6 +554,335 @@ py::object decode8(const std::shared_ptr<Decode8Plan>& plan, const std::shared_p
   }
   py::gil_scoped_acquire gil;
   return o.defined() ? py::cast(o) : py::none();
+}
+
+// ---------------------------------------------------------------------------------------------------- pages that rows share and give back
+// 32-bit tensors over the parts of one allocation, without the dispatcher.  Parts of four words and more in a row come first, for their alignment.
+struct Parts {
+  Tensor all;
+  int64_t used = 0;
+  Parts(int64_t words, const at::TensorOptions& ints) : all(at::empty({words}, ints)) {}
+  Tensor take(at::IntArrayRef sizes) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), caffe2::TypeMeta::Make<int32_t>());
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    t.unsafeGetTensorImpl()->set_storage_offset(used);
+    int64_t n = 1;
+    for (int64_t s : sizes) n *= s;
+    used += n;
+    return t;
+  }
+};
+
+bool good_page_size(int64_t n) { return n >= 1 && n <= (1 << 30) && !(n & (n - 1)); }
+bool good_table(const Tensor& table, const Tensor& like, int64_t B) {
+  return good_ints(table, 2, like) && table.size(0) == B && table.size(1) >= 1 && B * table.size(1) <= 0x7fffffff;
+}
+
+// (block_table, seq_lens, free_pages, free_head, copies, status), or None.
+py::object plan_forks(uint64_t kernel, const Tensor& parents, const Tensor& lens, const Tensor& table, const Tensor& free_pages,
+                      const Tensor& free_head, int64_t page_size, int64_t num_pages, const std::optional<Tensor>& keep) {
+  const int64_t B = lens.dim() == 1 ? lens.size(0) : 0;
+  if (B < 1 || B > 4096 || !good_ints(lens, 1, lens) || !good_ints(parents, 1, lens) || parents.size(0) != B || !good_table(table, lens, B) ||
+      !good_ints(free_pages, 1, lens) || !good_ints(free_head, 1, lens) || free_head.size(0) != 1 || (keep && (!good_ints(*keep, 1, lens) || keep->size(0) != B)) ||
+      !good_page_size(page_size) || num_pages < 1 || num_pages > 0x7ffffff0 || free_pages.size(0) > 0x7fffffff)
+    return py::none();
+  py::gil_scoped_release nogil;
+  c10::cuda::CUDAGuard guard(lens.device());
+  at::AutoGradMode no_grad(false);
+  const int64_t W = table.size(1), n_free = free_pages.size(0);
+  Parts parts(4 * B + B * W + B + n_free + 2, lens.options());
+  Tensor copies = parts.take({B, 4}), table_out = parts.take({B, W}), lens_out = parts.take({B}), free_out = parts.take({n_free}), head = parts.take({1}),
+         status = parts.take({1});
+  const Tensor workspace = at::empty({ae_plan_lists_workspace((int)num_pages)}, lens.options().dtype(at::kByte));
+  AePlanForksParams p;
+  memset(&p, 0, sizeof p);
+  p.parents = (const int32_t*)parents.data_ptr(); p.seq_lens = (const int32_t*)lens.data_ptr();
+  p.keep_lens = keep ? (const int32_t*)keep->data_ptr() : nullptr;
+  p.block_table = (const int32_t*)table.data_ptr(); p.free_pages = (const int32_t*)free_pages.data_ptr();
+  p.free_head = (const int32_t*)free_head.data_ptr();
+  p.table_out = (int32_t*)table_out.data_ptr(); p.lens_out = (int32_t*)lens_out.data_ptr(); p.free_out = (int32_t*)free_out.data_ptr();
+  p.head_out = (int32_t*)head.data_ptr(); p.copies = (int32_t*)copies.data_ptr(); p.status = word(status); p.workspace = workspace.data_ptr();
+  p.table_stride = table.stride(0);
+  p.B = (int)B; p.max_pages = (int)W; p.n_free = (int)n_free; p.page_size = (int)page_size; p.num_pages = (int)num_pages;
+  check(ae_launch_plan_forks(handle(kernel), &p, stream_of(lens)), "ae_launch_plan_forks");
+  py::gil_scoped_acquire gil;
+  return py::make_tuple(table_out, lens_out, free_out, head, copies, status);
+}
+
+// (block_table, free_pages, free_head, copies, status), or None.
+py::object plan_compaction(uint64_t kernel, const Tensor& lens, const Tensor& table, int64_t page_size, int64_t num_pages) {
+  const int64_t B = lens.dim() == 1 ? lens.size(0) : 0;
+  if (B < 1 || !good_ints(lens, 1, lens) || !good_table(table, lens, B) || !good_page_size(page_size) || num_pages < 1 || num_pages > 0x7ffffff0)
+    return py::none();
+  py::gil_scoped_release nogil;
+  c10::cuda::CUDAGuard guard(lens.device());
+  at::AutoGradMode no_grad(false);
+  const int64_t W = table.size(1), n = num_pages / 2;
+  Parts parts(4 * n + B * W + num_pages + 2, lens.options());
+  Tensor copies = parts.take({n, 4}), table_out = parts.take({B, W}), free_out = parts.take({num_pages}), head = parts.take({1}), status = parts.take({1});
+  const Tensor workspace = at::empty({ae_plan_lists_workspace((int)num_pages)}, lens.options().dtype(at::kByte));
+  AePlanCompactionParams p;
+  memset(&p, 0, sizeof p);
+  p.seq_lens = (const int32_t*)lens.data_ptr(); p.block_table = (const int32_t*)table.data_ptr();
+  p.table_out = (int32_t*)table_out.data_ptr(); p.free_out = (int32_t*)free_out.data_ptr(); p.head_out = (int32_t*)head.data_ptr();
+  p.copies = (int32_t*)copies.data_ptr(); p.status = word(status); p.workspace = workspace.data_ptr();
+  p.table_stride = table.stride(0);
+  p.B = (int)B; p.max_pages = (int)W; p.page_size = (int)page_size; p.num_pages = (int)num_pages; p.n_copies = (int)n;
+  check(ae_launch_plan_compaction(handle(kernel), &p, stream_of(lens)), "ae_launch_plan_compaction");
+  py::gil_scoped_acquire gil;
+  return py::make_tuple(table_out, free_out, head, copies, status);
+}
+
+// A pool [pages, slots, (rows,) (run)] as bytes; false when its layout is not one of those.
+bool pool_of(const Tensor& t, AePagePool& d) {
+  const int64_t es = t.element_size(), n = t.dim();
+  if (n < 2 || n > 4) return false;
+  for (int64_t i = 0; i < n; ++i)
+    if (t.size(i) > 1 && t.stride(i) < 1) return false;
+  memset(&d, 0, sizeof d);
+  d.base = t.data_ptr();
+  auto st = [&](int64_t i, int64_t whole) { return t.size(i) > 1 ? t.stride(i) * es : whole; };
+  int64_t run = es, rows = 1;
+  if (n >= 3) {
+    if (t.size(n - 1) > 1 && t.stride(n - 1) != 1) return false;
+    run *= t.size(n - 1);
+  }
+  d.row_stride = run;
+  if (n == 4) {
+    rows = t.size(2);
+    d.row_stride = st(2, run);
+    if (d.row_stride == run) run *= rows, rows = 1, d.row_stride = run;
+  }
+  if (run > 0x7fffffff || rows > 0x7fffffff || run * rows * t.size(1) > 0x7fffffff) return false;
+  d.slot_stride = st(1, run * rows);
+  d.page_stride = st(0, d.slot_stride * t.size(1));
+  d.rows = (int)rows; d.run_bytes = (int)run;
+  return true;
+}
+
+// `pools`: caches (their native side) and tensors.  False when they or the list do not fit.
+bool copy_pages(uint64_t kernel, const py::list& pools, const Tensor& copies) {
+  if (!good_ints(copies, 2, copies) || copies.size(1) != 4 || (copies.size(0) > 1 && copies.stride(0) != 4) || copies.size(0) > 0x7fffffff ||
+      reinterpret_cast<uintptr_t>(copies.data_ptr()) % 16)
+    return false;
+  std::vector<std::pair<Tensor, Tensor>> all;  // slots, and the scales of a page
+  for (py::handle h : pools) {
+    if (py::isinstance<Cache8>(h)) {
+      const Cache8& c = *h.cast<std::shared_ptr<Cache8>>();
+      all.emplace_back(c.k, c.ks);
+      all.emplace_back(c.v, c.vs);
+    } else {
+      all.emplace_back(h.cast<Tensor>(), Tensor());
+    }
+  }
+  std::vector<AePagePool> d(all.size());
+  size_t n = 0;
+  for (size_t i = 0; i < all.size(); ++i) {
+    const Tensor &t = all[i].first, &extra = all[i].second;
+    if (!t.is_cuda() || t.device() != copies.device() || t.dim() < 2 || t.size(0) != all[0].first.size(0) || t.size(1) != all[0].first.size(1) ||
+        t.size(0) > 0x7fffffff || (t.requires_grad() && at::GradMode::is_enabled()) || needs_function({&t}))
+      return false;
+    if (t.numel() == 0) continue;
+    if (!pool_of(t, d[n])) return false;
+    if (extra.defined()) {
+      d[n].extra = extra.data_ptr();
+      d[n].extra_stride = extra.stride(0) * 4;
+      d[n].extra_bytes = (int)extra.size(1) * 4;
+    }
+    ++n;
+  }
+  if (n == 0) return true;
+  py::gil_scoped_release nogil;
+  c10::cuda::CUDAGuard guard(copies.device());
+  AeCopyPagesParams p;
+  memset(&p, 0, sizeof p);
+  p.copies = (const int32_t*)copies.data_ptr();
+  p.n_copies = (int)copies.size(0);
+  p.num_pages = (int)all[0].first.size(0); p.page_size = (int)all[0].first.size(1);
+  for (size_t i = 0; i < n; i += AE_MAX_COPY_POOLS) {
+    p.n_pools = (int)std::min<size_t>(n - i, AE_MAX_COPY_POOLS);
+    std::copy(d.begin() + i, d.begin() + i + p.n_pools, p.pools);
+    check(ae_launch_copy_pages(handle(kernel), &p, stream_of(copies)), "ae_launch_copy_pages");
+  }
+  for (auto& t : all)  // what autograd has saved of a pool has changed
+    if (!t.first.is_inference()) t.first.unsafeGetTensorImpl()->bump_version();
+  return true;
+}
+
+// ---------------------------------------------------------------------------------------------------- norm and rotation of heads
+struct RopePlan {
+  void *fwd = nullptr, *bwd = nullptr, *dw = nullptr;
+  int D = 0;
+  bool norm = true;
+  float eps = 0, scale = 1;
+  std::vector<uint64_t> turns;
+};
+
+bool aligned16(const Tensor& t) {
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) % 8) return false;
+  return true;
+}
+
+// (batch, position, head) strides of [B, S, H, D] or [T, H, D]
+void head_strides(const Tensor& t, int64_t (&st)[3]) {
+  const int n = (int)t.dim() - 1;
+  auto at = [&](int i) { return t.size(i) > 1 ? t.stride(i) : 0; };
+  st[0] = n == 3 ? at(0) : 0;
+  st[1] = at(n - 2);
+  st[2] = at(n - 1);
+}
+
+void rope_params(const RopePlan& plan, const Tensor* const (&x)[2], const Tensor* const (&w)[2], const Tensor& pos, AeQkRopeParams& p) {
+  memset(&p, 0, sizeof p);
+  const Tensor& q = *x[0];
+  const bool batch = q.dim() == 4;
+  p.B = batch ? (int)q.size(0) : 1;
+  p.S = (int)q.size(batch ? 1 : 0);
+  p.dtype = q.scalar_type() == at::kBFloat16 ? AE_DTYPE_BF16 : AE_DTYPE_F16;
+  for (int i = 0; i < 2; ++i) {
+    if (!x[i]->defined()) continue;
+    p.x[i] = x[i]->data_ptr();
+    p.H[i] = (int)x[i]->size(-2);
+    head_strides(*x[i], p.x_stride[i]);
+    if (w[i]->defined()) {
+      p.w[i] = w[i]->data_ptr();
+      p.w_fp32 = w[i]->scalar_type() == at::kFloat;
+    }
+  }
+  p.positions = pos.data_ptr();
+  p.pos_int64 = pos.scalar_type() == at::kLong;
+  p.pos_stride[0] = pos.dim() == 2 && pos.size(0) > 1 ? pos.stride(0) : 0;
+  p.pos_stride[1] = pos.size(-1) > 1 ? pos.stride(-1) : 0;
+  p.eps = plan.eps;
+  p.rotary_scale = plan.scale;
+  std::copy(plan.turns.begin(), plan.turns.end(), p.turns);
+}
+
+struct RopeNode : Node {
+  std::shared_ptr<RopePlan> plan;
+  SavedVariable q, k, wq, wk, pos;
+
+  variable_list apply(variable_list&& grads) override {
+    const bool second = at::GradMode::is_enabled();
+    const int n = (int)num_inputs();
+    variable_list out(4);
+    Tensor X[2], W[2], G[2], P;
+    {
+      std::lock_guard<std::mutex> lock(mutex_);
+      X[0] = q.unpack(), X[1] = k.unpack(), W[0] = wq.unpack(), W[1] = wk.unpack(), P = pos.unpack();
+    }
+    {
+      at::AutoGradMode no_grad(false);
+      c10::cuda::CUDAGuard guard(P.device());
+      for (int i = 0; i < n; ++i) {
+        G[i] = grads[i].defined() ? grads[i] : input_metadata(i).zeros_like();  // as torch.autograd.Function does
+        if (G[i].stride(-1) != 1 || !aligned16(G[i])) G[i] = G[i].clone(at::MemoryFormat::Contiguous);
+        if (!plan->norm) X[i] = G[i];  // not read: sizes and type alone
+      }
+      AeQkRopeParams p;
+      rope_params(*plan, {&X[0], &X[1]}, {&W[0], &W[1]}, P, p);
+      for (int i = 0; i < n; ++i) {
+        p.g[i] = G[i].data_ptr();
+        head_strides(G[i], p.g_stride[i]);
+        out[i] = at::empty(G[i].sizes(), G[i].options(), at::MemoryFormat::Contiguous);
+        p.y[i] = out[i].data_ptr();
+      }
+      const bool sums = (W[0].defined() && task_should_compute_output(2)) || (W[1].defined() && task_should_compute_output(3));
+      Tensor workspace, dw[2];
+      if (sums) {
+        workspace = at::empty({ae_qk_rope_workspace(plan->bwd)}, X[0].options().dtype(at::kByte));
+        p.workspace = (float*)workspace.data_ptr();
+        const auto like = (W[0].defined() ? W[0] : W[1]).options();
+        for (int i = 0; i < n; ++i) {
+          dw[i] = at::empty({plan->D}, like);
+          p.dw[i] = dw[i].data_ptr();
+        }
+      }
+      void* st = stream_of(X[0]);
+      check(ae_launch_qk_rope(plan->bwd, &p, st), "ae_launch_qk_rope");
+      if (sums) {
+        check(ae_launch_qk_rope(plan->dw, &p, st), "ae_launch_qk_rope");
+        for (int i = 0; i < 2; ++i)
+          if (W[i].defined()) out[2 + i] = dw[i];
+      }
+    }
+    for (int i = 0; i < 4; ++i)
+      if (!task_should_compute_output(i)) out[i] = Tensor();
+    if (second)  // differentiated again, they say that they cannot be
+      for (Tensor& t : out)
+        if (t.defined()) {
+          t.set_requires_grad(true);
+          t = torch::autograd::DelayedError("QKNormRope has no second derivative", 1)({t})[0];
+        }
+    return out;
+  }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* s : {&q, &k, &wq, &wk, &pos}) s->reset_data();
+  }
+  std::string name() const override { return "QKNormRopeBackward"; }
+};
+
+// (q, k) normed and rotated, k None where there is none; None when the tensors do not fit.
+py::object qk_rope(const std::shared_ptr<RopePlan>& plan, const Tensor& q, const std::optional<Tensor>& k_, const Tensor& pos,
+                   const std::optional<Tensor>& wq_, const std::optional<Tensor>& wk_) {
+  const Tensor k = k_ ? *k_ : Tensor(), wq = wq_ ? *wq_ : Tensor(), wk = wk_ ? *wk_ : Tensor();
+  const int64_t n = q.dim();
+  if (!q.is_cuda() || (n != 3 && n != 4) || (q.scalar_type() != at::kHalf && q.scalar_type() != at::kBFloat16) || (wk.defined() && !k.defined()))
+    return py::none();
+  for (const Tensor* x : {&q, &k}) {
+    if (!x->defined()) continue;
+    if (!x->is_cuda() || x->device() != q.device() || x->scalar_type() != q.scalar_type() || x->dim() != n || x->size(n - 1) != plan->D || x->stride(n - 1) != 1 ||
+        x->size(n - 2) < 1 || x->size(n - 2) > 65535 || x->sizes().slice(0, n - 2) != q.sizes().slice(0, n - 2) || (x->numel() && !aligned16(*x)))
+      return py::none();
+  }
+  const int64_t B = n == 4 ? q.size(0) : 1, S = q.size(n == 4 ? 1 : 0);
+  if (B > 0x7fffffff || S > 0x7fffffff || B * S > 0x7fffffff) return py::none();
+  if (!pos.is_cuda() || pos.device() != q.device() || (pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong) || pos.dim() < 1 || pos.dim() > n - 2 ||
+      pos.size(-1) != S || (pos.dim() == 2 && pos.size(0) != B && pos.size(0) != 1))
+    return py::none();
+  for (const Tensor* w : {&wq, &wk}) {
+    if (!w->defined()) continue;
+    const Tensor& other = w == &wq ? wk : wq;
+    if (!plan->norm || !w->is_cuda() || w->device() != q.device() || w->dim() != 1 || w->size(0) != plan->D || w->stride(0) != 1 ||
+        (w->scalar_type() != at::kFloat && w->scalar_type() != q.scalar_type()) || (other.defined() && other.scalar_type() != w->scalar_type()) ||
+        reinterpret_cast<uintptr_t>(w->data_ptr()) % 16)
+      return py::none();
+  }
+  for (const Tensor* t : {&q, &k, &wq, &wk})
+    if (t->defined() && needs_function({t})) return py::none();
+  Tensor y[2];
+  {
+    py::gil_scoped_release nogil;
+    c10::cuda::CUDAGuard guard(q.device());
+    at::AutoGradMode no_grad(false);
+    AeQkRopeParams p;
+    rope_params(*plan, {&q, &k}, {&wq, &wk}, pos, p);
+    for (int i = 0; i < 2; ++i) {
+      const Tensor& x = i ? k : q;
+      if (!x.defined()) continue;
+      y[i] = at::empty(x.sizes(), x.options(), at::MemoryFormat::Contiguous);
+      p.y[i] = y[i].data_ptr();
+    }
+    check(ae_launch_qk_rope(plan->fwd, &p, stream_of(q)), "ae_launch_qk_rope");
+  }
+  if (wants_grad({&q, &k, &wq, &wk})) {
+    auto node = std::shared_ptr<RopeNode>(new RopeNode(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(q, k, wq, wk));
+    node->plan = plan;
+    if (plan->norm) {
+      node->q = SavedVariable(q, false);
+      if (k.defined()) node->k = SavedVariable(k, false);
+    }
+    if (wq.defined()) node->wq = SavedVariable(wq, false);
+    if (wk.defined()) node->wk = SavedVariable(wk, false);
+    node->pos = SavedVariable(pos, false);
+    for (Tensor& t : y)
+      if (t.defined()) torch::autograd::set_history(t, node);
+  }
+  return py::make_tuple(y[0], k.defined() ? py::cast(y[1]) : py::none());
 }
 
 // ---------------------------------------------------------------------------------------------------- split-KV decode
@@ -1228,6 +1558,19 @@ PYBIND11_MODULE(_ae_host, m) {
   m.def("plan_pages", torch::wrap_pybind_function(&plan_pages));
   m.def("cache8_write", torch::wrap_pybind_function(&cache8_write));
   m.def("decode8", torch::wrap_pybind_function(&decode8));
+  m.def("plan_forks", torch::wrap_pybind_function(&plan_forks));
+  m.def("plan_compaction", torch::wrap_pybind_function(&plan_compaction));
+  m.def("copy_pages", torch::wrap_pybind_function(&copy_pages));
+  py::class_<RopePlan, std::shared_ptr<RopePlan>>(m, "RopePlan")
+      .def(py::init([](uint64_t fwd, uint64_t bwd, uint64_t dw, int D, bool norm, double eps, double scale, const std::vector<uint64_t>& turns) {
+        auto p = std::make_shared<RopePlan>();
+        p->fwd = handle(fwd); p->bwd = handle(bwd); p->dw = handle(dw);
+        p->D = D; p->norm = norm; p->eps = (float)eps; p->scale = (float)scale;
+        if (turns.size() > sizeof(AeQkRopeParams::turns) / sizeof(uint64_t)) throw py::value_error("too many frequencies");
+        p->turns = turns;
+        return p;
+      }));
+  m.def("qk_rope", torch::wrap_pybind_function(&qk_rope));
   m.def("decode", torch::wrap_pybind_function(&decode));
   m.def("mla", torch::wrap_pybind_function(&mla));
   m.def("mla_paged", torch::wrap_pybind_function(&mla_paged));

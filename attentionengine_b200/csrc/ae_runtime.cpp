@@ -1283,6 +1283,181 @@ int ae_launch_decode_combine(void* module, const AeDecodeParams* p, void* stream
   return launch_after(m, combine_blocks(a.H, a.DV), (unsigned)p->B, 1, &a, stream);
 }
 
+// The planners of a pool's pages run as one cluster (page_lists.cuh); behind a word for each page the workspace has one for each of its CTAs.
+static const int kListCtas = 8;
+static int64_t list_words(int32_t num_pages) { return ((int64_t)num_pages + 3) / 4 * 4; }
+int64_t ae_plan_lists_workspace(int32_t num_pages) { return (list_words(std::max(num_pages, 0)) + 16) * 4; }
+
+static bool list_args_ok(int B, int max_pages, int page_log2, int num_pages, const void* copies, const void* workspace) {
+  return page_log2 >= 0 && B >= 1 && max_pages >= 1 && num_pages >= 1 && num_pages <= 0x7ffffff0 && (int64_t)B * max_pages <= 0x7fffffff &&
+         !((reinterpret_cast<uintptr_t>(copies) | reinterpret_cast<uintptr_t>(workspace)) & 15);
+}
+
+int ae_launch_plan_forks(void* module, const AePlanForksParams* p, void* stream) {
+  if (!module || !p || !p->parents || !p->seq_lens || !p->block_table || !p->free_head || !p->table_out || !p->lens_out || !p->head_out ||
+      !p->copies || !p->status || !p->workspace || (p->n_free > 0 && (!p->free_pages || !p->free_out)))
+    return AE_ERR_INVALID;
+  Module* m = (Module*)module;
+  if (m->cfg.kind != AE_KIND_PLAN_FORKS) {
+    set_error("module kind does not match the entry point");
+    return AE_ERR_UNSUPPORTED;
+  }
+  const int log2 = page_log2_of(p->page_size);
+  if (!list_args_ok(p->B, p->max_pages, log2, p->num_pages, p->copies, p->workspace) || p->B > 4096 || p->n_free < 0 ||
+      (const int32_t*)p->table_out == p->block_table || (const int32_t*)p->free_out == p->free_pages || (const int32_t*)p->lens_out == p->seq_lens) {
+    set_error("plan_forks: 1 to 4096 rows, a page size that is a power of two, a pool, outputs that are no inputs");
+    return AE_ERR_INVALID;
+  }
+  int rc = ensure_loaded(m);
+  if (rc) return rc;
+  AePlanForksArgs a;
+  memset(&a, 0, sizeof a);
+  a.parents = p->parents; a.lens = p->seq_lens; a.keep = p->keep_lens; a.table = p->block_table; a.free_pages = p->free_pages;
+  a.free_head = p->free_head; a.table_out = p->table_out; a.lens_out = p->lens_out; a.free_out = p->free_out; a.head_out = p->head_out;
+  a.copies = (AePageCopy*)p->copies; a.status = p->status; a.state = (u32*)p->workspace; a.counts = (int*)a.state + list_words(p->num_pages);
+  a.table_stride = p->table_stride; a.B = p->B; a.max_pages = p->max_pages; a.n_free = p->n_free; a.page_log2 = log2; a.num_pages = p->num_pages;
+  return launch_cluster(m, kListCtas, 1, 1, kListCtas, &a, stream);
+}
+
+int ae_launch_plan_compaction(void* module, const AePlanCompactionParams* p, void* stream) {
+  if (!module || !p || !p->seq_lens || !p->block_table || !p->table_out || !p->free_out || !p->head_out || !p->status || !p->workspace ||
+      (p->n_copies > 0 && !p->copies))
+    return AE_ERR_INVALID;
+  Module* m = (Module*)module;
+  if (m->cfg.kind != AE_KIND_PLAN_COMPACTION) {
+    set_error("module kind does not match the entry point");
+    return AE_ERR_UNSUPPORTED;
+  }
+  const int log2 = page_log2_of(p->page_size);
+  if (!list_args_ok(p->B, p->max_pages, log2, p->num_pages, p->copies, p->workspace) || p->n_copies < p->num_pages / 2 ||
+      (const int32_t*)p->table_out == p->block_table) {
+    set_error("plan_compaction: rows, a page size that is a power of two, a pool, room for num_pages / 2 copies");
+    return AE_ERR_INVALID;
+  }
+  int rc = ensure_loaded(m);
+  if (rc) return rc;
+  AePlanCompactionArgs a;
+  memset(&a, 0, sizeof a);
+  a.lens = p->seq_lens; a.table = p->block_table; a.table_out = p->table_out; a.free_out = p->free_out; a.head_out = p->head_out;
+  a.copies = (AePageCopy*)p->copies; a.status = p->status; a.state = (u32*)p->workspace; a.counts = (int*)a.state + list_words(p->num_pages);
+  a.table_stride = p->table_stride; a.B = p->B; a.max_pages = p->max_pages; a.page_log2 = log2; a.num_pages = p->num_pages;
+  a.n_copies = p->n_copies;
+  return launch_cluster(m, kListCtas, 1, 1, kListCtas, &a, stream);
+}
+
+int ae_launch_copy_pages(void* module, const AeCopyPagesParams* p, void* stream) {
+  if (!module || !p) return AE_ERR_INVALID;
+  Module* m = (Module*)module;
+  if (m->cfg.kind != AE_KIND_COPY_PAGES) {
+    set_error("module kind does not match the entry point");
+    return AE_ERR_UNSUPPORTED;
+  }
+  if (p->n_copies < 0 || p->n_pools < 0 || p->n_pools > AE_MAX_COPY_POOLS || p->num_pages < 0 || p->page_size < 1) return AE_ERR_INVALID;
+  if (p->n_copies == 0 || p->n_pools == 0) return AE_OK;
+  if (!p->copies || (reinterpret_cast<uintptr_t>(p->copies) & 15)) return AE_ERR_INVALID;
+  AeCopyPagesArgs a;
+  memset(&a, 0, sizeof a);
+  a.copies = (const AePageCopy*)p->copies; a.n_copies = p->n_copies; a.n_pools = p->n_pools; a.num_pages = p->num_pages; a.page_size = p->page_size;
+  const int part_bytes = m->cfg.reserved[0];
+  for (int i = 0; i < p->n_pools; ++i) {
+    const AePagePool& s = p->pools[i];
+    AeCopyPool& d = a.pools[i];
+    const int64_t slot = (int64_t)s.rows * s.run_bytes;
+    if (!s.base || s.rows < 1 || s.run_bytes < 1 || slot * p->page_size > 0x7fffffff || (s.extra && (s.extra_bytes < 0 || s.extra_bytes % 4 || s.extra_stride % 4 ||
+        (reinterpret_cast<uintptr_t>(s.extra) & 3)))) {
+      set_error("copy_pages: a pool with rows of at least a byte, pages below 2 GB, extra words of 4 bytes");
+      return AE_ERR_INVALID;
+    }
+    d.base = (u8*)s.base; d.extra = (u8*)s.extra;
+    d.page_st = s.page_stride; d.slot_st = s.slot_stride; d.row_st = s.row_stride; d.extra_st = s.extra_stride;
+    d.rows = s.rows; d.run = s.run_bytes; d.extra_bytes = s.extra_bytes;
+    const uint64_t all = (uint64_t)(uintptr_t)s.base | (uint64_t)s.page_stride | (uint64_t)s.run_bytes | (p->page_size > 1 ? (uint64_t)s.slot_stride : 0) |
+                         (s.rows > 1 ? (uint64_t)s.row_stride : 0);
+    d.vec = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
+    d.slots_part = (int)std::max<int64_t>(1, part_bytes / slot);
+    d.first = a.parts;
+    a.parts += (p->page_size + d.slots_part - 1) / d.slots_part;
+  }
+  const int64_t items = (int64_t)p->n_copies * a.parts;
+  int rc = ensure_loaded(m);
+  if (rc) return rc;
+  return launch_after(m, (unsigned)std::min<int64_t>(items, 148 * (int64_t)m->cfg.reserved[1]), 1, 1, &a, stream);
+}
+
+static const int kRopeSms = 148;
+int64_t ae_qk_rope_workspace(void* module) {
+  const Module* m = (const Module*)module;
+  return m && m->cfg.kind == AE_KIND_QK_ROPE ? (int64_t)kRopeSms * m->cfg.reserved[2] * m->cfg.head_dim * 4 + 2 * m->cfg.head_dim * 4 : 0;
+}
+
+int ae_launch_qk_rope(void* module, const AeQkRopeParams* p, void* stream) {
+  if (!module || !p) return AE_ERR_INVALID;
+  Module* m = (Module*)module;
+  if (m->cfg.kind != AE_KIND_QK_ROPE) {
+    set_error("module kind does not match the entry point");
+    return AE_ERR_UNSUPPORTED;
+  }
+  const bool bwd = m->kernel == "ae_qk_rope_bwd", sums = m->kernel == "ae_qk_rope_dw";
+  const int64_t T = (int64_t)p->B * p->S;
+  const int D = m->cfg.head_dim, warps = m->cfg.threads / 32, teams = 512 / D;
+  if (p->B < 0 || p->S < 0 || p->H[0] < 1 || p->H[1] < 0 || T > 0x7fffffff || (int64_t)p->H[0] * D > 0x7fffffff || (int64_t)p->H[1] * D > 0x7fffffff) {
+    set_error("norm and rotation: bad shape");
+    return AE_ERR_INVALID;
+  }
+  if (T == 0 && !sums) return AE_OK;
+  if (!p->positions && T) return AE_ERR_INVALID;
+  AeQkRopeArgs a;
+  memset(&a, 0, sizeof a);
+  uint64_t all = 0;
+  for (int i = 0; i < 2; ++i) {
+    if (p->H[i] == 0) continue;
+    if (!sums && (!p->x[i] || !p->y[i] || (bwd && !p->g[i]))) return AE_ERR_INVALID;
+    a.x[i] = p->x[i]; a.g[i] = p->g[i]; a.y[i] = p->y[i]; a.w[i] = p->w[i]; a.dw[i] = p->dw[i]; a.H[i] = p->H[i];
+    all |= (uint64_t)(uintptr_t)p->x[i] | (uint64_t)(uintptr_t)p->y[i] | (uint64_t)(uintptr_t)p->w[i] | (bwd ? (uint64_t)(uintptr_t)p->g[i] : 0);
+    for (int j = 0; j < 3; ++j) {
+      a.x_st[i][j] = p->x_stride[i][j]; a.g_st[i][j] = p->g_stride[i][j];
+      all |= (uint64_t)p->x_stride[i][j] * 2 | (bwd ? (uint64_t)p->g_stride[i][j] * 2 : 0);
+    }
+  }
+  if (all & 15) {
+    set_error("norm and rotation: tensors and their strides must be multiples of 16 bytes");
+    return AE_ERR_INVALID;
+  }
+  a.pos = p->positions; a.pos_st[0] = p->pos_stride[0]; a.pos_st[1] = p->pos_stride[1];
+  a.S = std::max(p->S, 1); a.T = (int)T;
+  a.bf16 = p->dtype == AE_DTYPE_BF16; a.w32 = p->w_fp32; a.pos64 = p->pos_int64; a.eps = p->eps; a.scale = p->rotary_scale;
+  a.dw_part = p->workspace;
+  memcpy(a.turns, p->turns, sizeof a.turns);
+  // heads of a warp: eight for each team, fewer while the tokens do not give every SM 16 warps
+  auto slices = [&](int per) {
+    for (int i = 0; i < 2; ++i) a.slices[i] = (a.H[i] + per - 1) / per;
+    return (int64_t)a.slices[0] + a.slices[1];
+  };
+  a.per = teams * 8;
+  while (a.per > teams && T * slices(a.per) < kRopeSms * 16) a.per /= 2;
+  const int64_t items = T * slices(a.per);
+  if (bwd || sums) {
+    // queries' and keys' CTAs in proportion to their heads
+    const int64_t most = (int64_t)kRopeSms * m->cfg.reserved[2];
+    for (int i = 0; i < 2; ++i) {
+      const int64_t need = (T * a.slices[i] + warps - 1) / warps, share = most * a.H[i] / (a.H[0] + a.H[1]);
+      a.ctas[i] = a.H[i] == 0 ? 0 : (int)std::min(need, std::max<int64_t>(share, 1));
+    }
+  }
+  int rc = ensure_loaded(m);
+  if (rc) return rc;
+  if (sums) {
+    if (!p->workspace || !p->dw[0] || (p->H[1] > 0 && !p->dw[1])) return AE_ERR_INVALID;
+    return launch_after(m, (unsigned)(D / 32), p->H[1] > 0 ? 2 : 1, 1, &a, stream);
+  }
+  if (bwd) return launch_after(m, (unsigned)(a.ctas[0] + a.ctas[1]), 1, 1, &a, stream);
+  if ((items + warps - 1) / warps > 0x7fffffff / warps) {
+    set_error("norm and rotation: too many heads for one launch");
+    return AE_ERR_INVALID;
+  }
+  return launch_after(m, (unsigned)((items + warps - 1) / warps), 1, 1, &a, stream);
+}
+
 int ae_launch_rowscale(void* module, const AeRowScaleParams* p, void* stream) {
   if (!module || !p || !p->x || p->n_rows < 0) return AE_ERR_INVALID;
   Module* m = (Module*)module;

@@ -324,6 +324,87 @@ struct AeCache8MergeArgs {  // kernel ae_cache8_merge
   int Hq, gq, rows;
 };
 
+// ---- pages of rows that go on from others, are cut or end (kernel ae_plan_forks) ----------------
+struct alignas(16) AePageCopy {
+  int src, dst;  // pages
+  int slots;     // the first slots of src that are copied; 0: the list has ended
+  int zero;
+};
+struct AePlanForksArgs {
+  const int* parents;     // [B] row that each row goes on from; -1: none
+  const int* lens;        // [B] tokens of each row
+  const int* keep;        // [B] tokens of the parent that it keeps, or null: all
+  const int* table;       // [B, max_pages], row stride table_stride
+  const int* free_pages;  // [n_free]
+  const int* free_head;   // [1]
+  int* table_out;         // [B, max_pages] contiguous
+  int* lens_out;          // [B]
+  int* free_out;          // [n_free]
+  int* head_out;          // [1]
+  AePageCopy* copies;     // [B]
+  u32* status;            // [1] written
+  u32* state;             // [num_pages rounded up to 4] scratch
+  int* counts;            // [clusters' CTAs] scratch
+  i64 table_stride;
+  int B, max_pages, n_free, page_log2, num_pages;
+};
+
+// ---- pages moved to the front of the pool (kernel ae_plan_compaction) ----------------------------
+struct AePlanCompactionArgs {
+  const int* lens;     // [B]
+  const int* table;    // [B, max_pages], row stride table_stride
+  int* table_out;      // [B, max_pages] contiguous
+  int* free_out;       // [num_pages]
+  int* head_out;       // [1]
+  AePageCopy* copies;  // [n_copies], num_pages / 2
+  u32* status;         // [1] written
+  u32* state;          // [num_pages rounded up to 4] scratch
+  int* counts;         // [clusters' CTAs] scratch
+  i64 table_stride;
+  int B, max_pages, page_log2, num_pages, n_copies;
+};
+
+// ---- copies of pages (kernel ae_copy_pages) --------------------------------------------------------
+#define AE_COPY_POOLS 48  // of a launch
+struct AeCopyPool {
+  u8* base;          // [pages, slots, rows, run]
+  u8* extra;         // bytes that each page has beside its slots (scales), or null
+  i64 page_st, slot_st, row_st, extra_st;  // bytes
+  int rows, run;     // of a slot; run: contiguous bytes
+  int extra_bytes;
+  int vec;           // bytes of an access: 16, 4 or 1
+  int first;         // its first part of a copy's
+  int slots_part;    // slots of a part
+};
+struct AeCopyPagesArgs {
+  const AePageCopy* copies;  // [n_copies]
+  int n_copies, n_pools;
+  int parts;                 // of a copy, over all pools
+  int num_pages, page_size;
+  AeCopyPool pools[AE_COPY_POOLS];
+};
+
+// ---- norm and rotation of query and key heads (kernels ae_qk_rope_fwd, _bwd, _dw) --------------
+#define AE_ROPE_MAX_PAIRS 128
+struct AeQkRopeArgs {
+  const void* x[2];       // queries, keys [B, S, H, D], 16 bits
+  const void* g[2];       // backward: gradients of the outputs
+  void* y[2];             // [T, H, D] contiguous: outputs, or gradients of x
+  const void* w[2];       // [D] or null: fp32 with w32, else the type of x
+  void* dw[2];            // [D], the type of w
+  float* dw_part;         // [ctas[0] + ctas[1]][D], or null: no gradients of the weights
+  const void* pos;        // [B, S] int32, int64 with pos64; negative: no token
+  i64 x_st[2][3], g_st[2][3];  // element strides: batch, position, head
+  i64 pos_st[2];
+  int H[2];
+  int S, T;               // positions of a batch row; T = B S
+  int per, slices[2];     // heads of a warp, and how many warps they make of a token's
+  int ctas[2];            // backward
+  int bf16, w32, pos64;
+  float eps, scale;
+  u64 turns[AE_ROPE_MAX_PAIRS];  // of each pair, a position's fraction of a turn in units of 2^-64
+};
+
 // ---- UMMA / TMA probe kernels (bring-up checks, kernel ae_probe) -------------------
 struct AeProbeArgs {
   AeTmaDesc tm_a;  // [128 rows, KD] 16-bit, box {64, 128}

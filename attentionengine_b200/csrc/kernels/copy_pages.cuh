@@ -1,0 +1,82 @@
+// Copies the first slots of pages into other pages, in every pool of a launch: keys, values and scales of all layers at once.
+//
+// A copy's bytes are cut into parts of about AE_COPY_PART, and a CTA takes parts in turn: one load of the list's entry, then all of its part's loads in
+// front of the stores.  HBM-bound once a few hundred parts are under way.  Which page goes where and how many slots stands on the device; a list ends at
+// its first entry without slots, which every CTA looks for itself (its length is next to nothing beside the pages that it names).  Entries that name a
+// page outside the pool, or more slots than a page has, are passed over.
+// Expects AE_COPY_THREADS, AE_COPY_PART.
+#define AE_COPY_UNROLL (AE_COPY_PART / 16 / AE_COPY_THREADS)
+
+// n units of V, from the unit `from` on of a page's part.  A pool's slots are runs of `per` units, row_st bytes apart, `rows` of them in slot_st bytes.
+template <typename V>
+AE_DEVICE void ae_copy_part(const AeCopyPool& p, const u8* src, u8* dst, int from, int n) {
+  const int per = p.run / (int)sizeof(V);
+  if (p.rows == 1 && p.slot_st == p.run) {  // slots behind each other
+    src += (i64)from * sizeof(V);
+    dst += (i64)from * sizeof(V);
+    for (int i = threadIdx.x; i < n; i += AE_COPY_THREADS * AE_COPY_UNROLL) {
+      V v[AE_COPY_UNROLL];
+#pragma unroll
+      for (int u = 0; u < AE_COPY_UNROLL; ++u)
+        if (i + u * AE_COPY_THREADS < n) v[u] = ((const V*)src)[i + u * AE_COPY_THREADS];
+#pragma unroll
+      for (int u = 0; u < AE_COPY_UNROLL; ++u)
+        if (i + u * AE_COPY_THREADS < n) ((V*)dst)[i + u * AE_COPY_THREADS] = v[u];
+    }
+  } else {
+    for (int i = from + threadIdx.x; i < from + n; i += AE_COPY_THREADS) {
+      const int row = i / per, slot = row / p.rows;
+      const i64 at = slot * p.slot_st + (row - slot * p.rows) * p.row_st + (i64)(i - row * per) * sizeof(V);
+      *(V*)(dst + at) = *(const V*)(src + at);
+    }
+  }
+}
+
+// Entries in front of the first without slots.
+AE_DEVICE int ae_list_length(const AePageCopy* copies, int most) {
+  __shared__ int red[AE_COPY_THREADS / 32];
+  for (int base = 0; base < most; base += 4 * AE_COPY_THREADS) {
+    int end = most;
+#pragma unroll
+    for (int j = 3; j >= 0; --j) {
+      const int i = base + j * AE_COPY_THREADS + (int)threadIdx.x;
+      if (i < most && copies[i].slots <= 0) end = i;
+    }
+    end = __reduce_min_sync(0xffffffffu, end);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = end;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < AE_COPY_THREADS / 32; ++w) end = min(end, red[w]);
+    if (end < most) return end;
+    __syncthreads();  // `red` has been read
+  }
+  return most;
+}
+
+extern "C" __global__ void __launch_bounds__(AE_COPY_THREADS) ae_copy_pages(const __grid_constant__ AeCopyPagesArgs a) {
+  ae_grid_wait();
+  ae_grid_trigger();
+  const i64 items = (i64)ae_list_length(a.copies, a.n_copies) * a.parts;
+  for (i64 item = blockIdx.x; item < items; item += gridDim.x) {
+    const int c = (int)(item / a.parts), part = (int)(item - (i64)c * a.parts);
+    const AePageCopy e = a.copies[c];
+    if (e.src < 0 || e.src >= a.num_pages || e.dst < 0 || e.dst >= a.num_pages || e.slots > a.page_size) continue;
+    int i = 0;
+    while (i + 1 < a.n_pools && part >= a.pools[i + 1].first) ++i;
+    const AeCopyPool& p = a.pools[i];
+    const int s0 = (part - p.first) * p.slots_part, s1 = min(s0 + p.slots_part, e.slots);
+    if (s0 == 0 && p.extra)
+      for (int k = threadIdx.x * 4; k < p.extra_bytes; k += AE_COPY_THREADS * 4)
+        *(u32*)(p.extra + (i64)e.dst * p.extra_st + k) = *(const u32*)(p.extra + (i64)e.src * p.extra_st + k);
+    if (s0 >= s1) continue;
+    const u8* const src = p.base + (i64)e.src * p.page_st;
+    u8* const dst = p.base + (i64)e.dst * p.page_st;
+    const int slot = p.rows * (p.run / p.vec);  // units of a slot
+    if (p.vec == 16)
+      ae_copy_part<uint4>(p, src, dst, s0 * slot, (s1 - s0) * slot);
+    else if (p.vec == 4)
+      ae_copy_part<u32>(p, src, dst, s0 * slot, (s1 - s0) * slot);
+    else
+      ae_copy_part<u8>(p, src, dst, s0 * slot, (s1 - s0) * slot);
+  }
+}

@@ -6,7 +6,8 @@ import math
 
 import torch
 
-from .attn_engine import AttentionEngine, LinearAttentionEngine, OnlineFunc, PagedCache8, plan_pages
+from .attn_engine import (AttentionEngine, LinearAttentionEngine, OnlineFunc, PagedCache8, copy_pages, plan_compaction, plan_forks,
+                          plan_pages)
 from .core import CustomIO, SymbolScalar, Var, meta_tensor
 
 
@@ -226,10 +227,15 @@ def retention_engine(B, H, S, D, DV, dtype):
 class PagedLayers:
     """The attention of a server's layers over paged 8-bit caches: ``prompts`` admits a batch of requests of different lengths, ``tokens``
     takes one more token for each.  The layers share the pages' numbers, so one plan serves a step; nothing is read back.  A prompt attends to itself
-    alone, so ``prompts`` is the first step: rows that hold tokens cannot get another one (a later turn, a part of a long prompt)."""
+    alone, so ``prompts`` is the first step: rows that hold tokens cannot get another one (a later turn, a part of a long prompt).
 
-    def __init__(self, n_layers, Hq, Hkv, D, dtype, rows, num_pages, page_size, max_len, device="cuda"):
-        self.page_size, self.rows = page_size, rows
+    ``rope``: a ``QKNormRope`` that norms and rotates the queries and keys of every step by the plan's positions, with ``weights`` (q_weight, k_weight) of
+    every layer.  ``fork`` lets rows go on from others (samples of one prompt, beams), cuts and ends them; ``compact`` brings the pages in use to the
+    front of the pools."""
+
+    def __init__(self, n_layers, Hq, Hkv, D, dtype, rows, num_pages, page_size, max_len, device="cuda", rope=None, weights=None):
+        self.page_size, self.rows, self.num_pages = page_size, rows, num_pages
+        self.rope, self.weights = rope, weights if weights is not None else [(None, None)] * n_layers
         self.caches = [PagedCache8(num_pages, page_size, Hkv, D, device=device) for _ in range(n_layers)]
         self.prompt = softmax_engine("B", Hq, Hkv, "S", D, D, dtype, True, packed=True)
         self.token = decode_engine("B", Hq, Hkv, 1, "S", D, dtype, cache_dtype=torch.float8_e4m3fn)
@@ -237,7 +243,7 @@ class PagedLayers:
         self.free, self.head = torch.arange(num_pages, **ints), torch.zeros(1, **ints)
         self.table, self.lens = torch.zeros(rows, -(-max_len // page_size), **ints), torch.zeros(rows, **ints)
         self.one = torch.ones(rows, **ints)
-        self.status = torch.zeros(1, **ints)
+        self.status, self.moved = torch.zeros(1, **ints), torch.zeros(1, **ints)
         self.begun = False
 
     def _plan(self, new_lens, n_tokens):
@@ -247,13 +253,17 @@ class PagedLayers:
         self.status |= plan.status
         return plan
 
+    def _rotated(self, layers, plan):
+        for (q, k, v), w in zip(layers, self.weights):
+            yield (q, k, v) if self.rope is None else (*self.rope(q, k, plan.positions, *w), v)
+
     def prompts(self, layers, new_lens):
         """``layers``: (q, k, v) of every layer, [T, heads, D] with the requests' tokens behind each other; returns the layers' outputs."""
         if self.begun:
             raise NotImplementedError("rows hold tokens already: new prompts would attend to themselves alone, without what is cached")
         plan = self._plan(new_lens, layers[0][0].shape[0])
         out = []
-        for cache, (q, k, v) in zip(self.caches, layers):
+        for cache, (q, k, v) in zip(self.caches, self._rotated(layers, plan)):
             cache.write(k, v, plan.segments)
             out.append(self.prompt.prefill_packed(q, k, v, plan.cu_seqlens))
         return out
@@ -262,14 +272,32 @@ class PagedLayers:
         """``layers``: (q, k, v) of every layer, [rows, heads, D]."""
         plan = self._plan(self.one, self.rows)
         out = []
-        for cache, (q, k, v) in zip(self.caches, layers):
+        for cache, (q, k, v) in zip(self.caches, self._rotated(layers, plan)):
             cache.write(k, v, plan.segments)
             out.append(self.token.decode_cache8(q.unsqueeze(1), cache, plan.block_table, plan.seq_lens).squeeze(1))
         return out
+
+    def fork(self, parents, keep_lens=None):
+        """Row b goes on from the first ``keep_lens[b]`` tokens (None: all) of row ``parents[b]``; -1: it ends, and its pages are free again.  A row that has
+        ended takes part in ``tokens`` from position 0."""
+        plan = plan_forks(parents, self.lens, self.table, self.free, self.head, self.page_size, self.num_pages, keep_lens)
+        self._moved(plan)
+        self.lens = plan.seq_lens
+
+    def compact(self):
+        """The pages in use to the front of every layer's pool; the number of them stays on the GPU, in ``head``."""
+        self._moved(plan_compaction(self.lens, self.table, self.page_size, self.num_pages))
+
+    def _moved(self, plan):
+        copy_pages(self.caches, plan.copies)
+        self.table, self.free, self.head = plan.block_table, plan.free_pages, plan.free_head
+        self.moved |= plan.status
 
     def check(self):
         """Raise if a step did not fit the pages or a kernel reported something (waits for the GPU)."""
         if int(self.status.item()):
             raise ValueError(f"plan_pages reported 0x{int(self.status.item()):x}")
+        if int(self.moved.item()):
+            raise ValueError(f"plan_forks or plan_compaction reported 0x{int(self.moved.item()):x}")
         self.prompt.check_status()
         self.token.check_status()

@@ -29,6 +29,7 @@ KIND_ATTN_FWD_PAIR = 14
 KIND_LINEAR_SEGMENTS = 15
 KIND_ATTN_PACKED, KIND_PLAN_PAGES, KIND_CACHE8_WRITE, KIND_CACHE8_DECODE = 16, 17, 18, 19
 KIND_CACHE8_MERGE = 20
+KIND_QK_ROPE, KIND_PLAN_FORKS, KIND_PLAN_COMPACTION, KIND_COPY_PAGES = 21, 22, 23, 24
 DTYPE_F16, DTYPE_BF16 = 0, 1
 
 
@@ -165,6 +166,34 @@ class Cache8DecodeParams(C.Structure):
                [(n, C.c_int32) for n in ("B", "Hq", "Hkv", "Sq", "max_pages", "num_pages", "page_size")] + [("status", C.c_void_p), ("workspace", C.c_void_p)]
 
 
+class PlanForksParams(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("parents", "seq_lens", "keep_lens", "block_table", "free_pages", "free_head", "table_out", "lens_out",
+                                          "free_out", "head_out", "copies", "status", "workspace")] + \
+               [("table_stride", C.c_int64)] + [(n, C.c_int32) for n in ("B", "max_pages", "n_free", "page_size", "num_pages")]
+
+
+class PlanCompactionParams(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("seq_lens", "block_table", "table_out", "free_out", "head_out", "copies", "status", "workspace")] + \
+               [("table_stride", C.c_int64)] + [(n, C.c_int32) for n in ("B", "max_pages", "page_size", "num_pages", "n_copies")]
+
+
+class PagePool(C.Structure):
+    _fields_ = [("base", C.c_void_p), ("extra", C.c_void_p)] + \
+               [(n, C.c_int64) for n in ("page_stride", "slot_stride", "row_stride", "extra_stride")] + \
+               [(n, C.c_int32) for n in ("rows", "run_bytes", "extra_bytes")]
+
+
+class CopyPagesParams(C.Structure):
+    _fields_ = [("copies", C.c_void_p)] + [(n, C.c_int32) for n in ("n_copies", "n_pools", "num_pages", "page_size")] + [("pools", PagePool * 48)]
+
+
+class QkRopeParams(C.Structure):
+    _fields_ = [(n, C.c_void_p * 2) for n in ("x", "g", "y", "w", "dw")] + [("positions", C.c_void_p), ("workspace", C.c_void_p),
+                ("x_stride", _S3 * 2), ("g_stride", _S3 * 2), ("pos_stride", C.c_int64 * 2), ("H", C.c_int32 * 2)] + \
+               [(n, C.c_int32) for n in ("B", "S", "dtype", "w_fp32", "pos_int64")] + [("eps", C.c_float), ("rotary_scale", C.c_float),
+                ("turns", C.c_uint64 * 128)]
+
+
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -173,7 +202,8 @@ EXPORTS = ["ae_compile", "ae_module_from_cubin", "ae_module_cubin", "ae_query", 
            "ae_launch_attn_bwd_dkv", "ae_launch_attn_bwd_fused", "ae_launch_attn_bwd_dq_cast", "ae_launch_probe", "ae_launch_attn_bwd_static_scratch", "ae_launch_mla_decode", "ae_launch_mla_combine", "ae_launch_mla_decode_paged", "ae_launch_attn_decode", "ae_launch_decode_combine", "ae_launch_rowscale", "ae_launch_linear_fwd", "ae_launch_linear_states", "ae_launch_linear_bwd",
            "ae_launch_linear_segments", "ae_launch_attn_packed", "ae_launch_plan_pages", "ae_launch_cache8_write",
            "ae_launch_cache8_decode", "ae_cache8_decode_workspace",
-           "ae_cache8_decode_merges", "ae_launch_cache8_merge"]
+           "ae_cache8_decode_merges", "ae_launch_cache8_merge", "ae_launch_plan_forks", "ae_launch_plan_compaction", "ae_launch_copy_pages",
+           "ae_plan_lists_workspace", "ae_launch_qk_rope", "ae_qk_rope_workspace"]
 
 
 def lib() -> C.CDLL:
@@ -218,6 +248,12 @@ def lib() -> C.CDLL:
             L.ae_cache8_decode_workspace.restype = C.c_int64
             L.ae_cache8_decode_merges.argtypes = [C.c_void_p, C.POINTER(Cache8DecodeParams)]
             L.ae_launch_cache8_merge.argtypes = [C.c_void_p, C.POINTER(Cache8DecodeParams), C.c_void_p]
+            L.ae_launch_plan_forks.argtypes = [C.c_void_p, C.POINTER(PlanForksParams), C.c_void_p]
+            L.ae_launch_plan_compaction.argtypes = [C.c_void_p, C.POINTER(PlanCompactionParams), C.c_void_p]
+            L.ae_launch_copy_pages.argtypes = [C.c_void_p, C.POINTER(CopyPagesParams), C.c_void_p]
+            L.ae_plan_lists_workspace.argtypes, L.ae_plan_lists_workspace.restype = [C.c_int32], C.c_int64
+            L.ae_launch_qk_rope.argtypes = [C.c_void_p, C.POINTER(QkRopeParams), C.c_void_p]
+            L.ae_qk_rope_workspace.argtypes, L.ae_qk_rope_workspace.restype = [C.c_void_p], C.c_int64
             L.ae_launch_probe.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
                                           C.c_void_p, C.c_void_p]
             _lib = L

@@ -65,6 +65,10 @@ enum {
   AE_KIND_CACHE8_WRITE = 18,
   AE_KIND_CACHE8_DECODE = 19,
   AE_KIND_CACHE8_MERGE = 20,
+  AE_KIND_QK_ROPE = 21,
+  AE_KIND_PLAN_FORKS = 22,
+  AE_KIND_PLAN_COMPACTION = 23,
+  AE_KIND_COPY_PAGES = 24,
 };
 
 #define AE_MAX_CUSTOM_INPUTS 4
@@ -229,6 +233,88 @@ int64_t ae_cache8_decode_workspace(void* module);
 int ae_cache8_decode_merges(void* module, const AeCache8DecodeParams* p);
 int ae_launch_cache8_merge(void* module, const AeCache8DecodeParams* p, void* stream);
 int ae_launch_cache8_decode(void* module, const AeCache8DecodeParams* p, void* stream);
+
+/* Pages of a step in which row i of B goes on from the first keep_lens[i] tokens of row parents[i] (all of them without keep_lens; -1: the row
+ * ends).  Whole pages are shared; a begun page that another row holds too is copied: the row takes the next of free_pages behind *free_head, in
+ * the order of the rows, and `copies` gets {page, new page, slots, 0} (unused entries at the end all 0).  Pages that no row holds any more go on
+ * top of the free list, in ascending order.  Nothing that is read is changed.  *status receives 0 or bits: 1 the free pages ran out (such
+ * a row ends with its whole pages), 2 a length beyond the table, 4 more pages came back than had been taken (the rest is left out), 8 a parent that is no row, a negative
+ * length or more tokens kept than there are, 16 a page outside the pool. */
+typedef struct AePlanForksParams {
+  const int32_t* parents;     /* [B] */
+  const int32_t* seq_lens;    /* [B] */
+  const int32_t* keep_lens;   /* [B] or null */
+  const int32_t* block_table; /* [B, max_pages] */
+  const int32_t* free_pages;  /* [n_free] */
+  const int32_t* free_head;   /* [1] */
+  int32_t* table_out;         /* [B, max_pages] contiguous; 0 where a row has no page.  No output is an input. */
+  int32_t* lens_out;          /* [B] */
+  int32_t* free_out;          /* [n_free] */
+  int32_t* head_out;          /* [1] */
+  int32_t* copies;            /* [B][4], 16-byte aligned */
+  uint32_t* status;           /* [1] */
+  void* workspace;            /* ae_plan_lists_workspace(num_pages) bytes with any contents, 16-byte aligned */
+  int64_t table_stride;
+  int32_t B, max_pages, n_free, page_size, num_pages; /* B: at most 4096; page_size: a power of two; B * max_pages below 2^31 */
+} AePlanForksParams;
+int64_t ae_plan_lists_workspace(int32_t num_pages);
+int ae_launch_plan_forks(void* module, const AePlanForksParams* p, void* stream);
+
+/* Moves the pages in use to the front of a pool: with U of them, those from U on go into the unused ones below U, both in ascending order.
+ * table_out has the new numbers, copies {page, new page, slots in use, 0} for each move (n_copies >= num_pages / 2; unused entries all 0), free_out
+ * all pages in order, and *head_out is U.  Status bits 2, 8, 16 as above. */
+typedef struct AePlanCompactionParams {
+  const int32_t* seq_lens;    /* [B] */
+  const int32_t* block_table; /* [B, max_pages] */
+  int32_t* table_out;         /* [B, max_pages] contiguous */
+  int32_t* free_out;          /* [num_pages] */
+  int32_t* head_out;          /* [1] */
+  int32_t* copies;            /* [n_copies][4], 16-byte aligned; may be null if n_copies is 0 */
+  uint32_t* status;           /* [1] */
+  void* workspace;
+  int64_t table_stride;
+  int32_t B, max_pages, page_size, num_pages, n_copies;
+} AePlanCompactionParams;
+int ae_launch_plan_compaction(void* module, const AePlanCompactionParams* p, void* stream);
+
+/* The first slots of pages into other pages, in up to AE_MAX_COPY_POOLS pools.  `copies` ends at its first entry without slots; entries that name pages
+ * outside the pools, or more slots than a page has, are passed over.  Destinations are distinct and no entry's source. */
+#define AE_MAX_COPY_POOLS 48
+typedef struct AePagePool {
+  void* base;            /* [num_pages, page_size, rows, run_bytes], strides in bytes */
+  void* extra;           /* 4-byte words that a page has beside its slots, or null */
+  int64_t page_stride, slot_stride, row_stride, extra_stride;
+  int32_t rows, run_bytes, extra_bytes;
+} AePagePool;
+typedef struct AeCopyPagesParams {
+  const int32_t* copies; /* [n_copies][4], 16-byte aligned */
+  int32_t n_copies, n_pools, num_pages, page_size;
+  AePagePool pools[AE_MAX_COPY_POOLS];
+} AeCopyPagesParams;
+int ae_launch_copy_pages(void* module, const AeCopyPagesParams* p, void* stream);
+
+/* ---- norm and rotation of query and key heads ------------------------------------------------
+ * The module's kernel name selects what is launched: "ae_qk_rope_fwd" writes y from x; "ae_qk_rope_bwd" the gradients of x from those of y
+ * (g), and with `workspace` (ae_qk_rope_workspace(module) bytes) the sums that "ae_qk_rope_dw", launched behind it with the same
+ * parameters, turns into the weights' gradients.  Config: head_dim, reserved[0] rotary dims, [1] heads of a thread team on their way, [2] CTAs of an SM
+ * (backward).  Index 0: queries, 1: keys (H 0: none). */
+typedef struct AeQkRopeParams {
+  const void* x[2];       /* [B, S, H, D] 16-bit, rows 16-byte aligned */
+  const void* g[2];
+  void* y[2];             /* contiguous */
+  const void* w[2];       /* [D], 16-byte aligned, or null */
+  void* dw[2];            /* [D] in the type of w */
+  const void* positions;  /* [B, S]; negative: no token, zeros */
+  float* workspace;       /* or null: no gradients of weights */
+  int64_t x_stride[2][3], g_stride[2][3]; /* (batch, position, head) */
+  int64_t pos_stride[2];
+  int32_t H[2], B, S;
+  int32_t dtype, w_fp32, pos_int64;
+  float eps, rotary_scale;
+  uint64_t turns[128];    /* of pair i: fraction of a turn that one position makes, in units of 2^-64 */
+} AeQkRopeParams;
+int64_t ae_qk_rope_workspace(void* module);
+int ae_launch_qk_rope(void* module, const AeQkRopeParams* p, void* stream);
 
 /* ---- attention backward -----------------------------------------------------------
  * Stands in for `_attention.backward` (attn_tl.py:582-601): `mod_prep(o, dO)` (K2,
