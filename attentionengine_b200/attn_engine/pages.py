@@ -21,10 +21,9 @@ from .cache8 import MAX_ROWS, PagedCache8, _ints
 
 STATUS_TEXT = {1: "the free pages ran out", 2: "a length is beyond block_table's columns", 4: "more pages came back than free_head says are taken",
                8: "a parent is no row, a length is negative, or more tokens are kept than there are", 16: "a page is outside the pool"}
-LIST_THREADS, LIST_CTAS, LIST_BATCH = 512, 8, 4
-LIST_DEFINES = {"AE_LIST_THREADS": LIST_THREADS, "AE_LIST_CTAS": LIST_CTAS, "AE_LIST_BATCH": LIST_BATCH}
-FORKS_DEFINES = {"AE_LIST_ROWS": MAX_ROWS, **LIST_DEFINES}
-COPY_THREADS, COPY_PART, COPY_CTAS = 256, 16384, 8
+LIST_THREADS, LIST_BATCH = (1024, 512), 4  # threads of the kernel of all phases, and of those of one
+LIST_SMEM = 16 * 1024 + 12 * 512 + 6 * 16384 + 16  # 1024 rows, 16384 pages
+COPY_THREADS, COPY_PART, COPY_CTAS = 128, 32768, 16
 COPY_DEFINES = {"AE_COPY_THREADS": COPY_THREADS, "AE_COPY_PART": COPY_PART}
 
 
@@ -61,17 +60,28 @@ class CompactionPlan(NamedTuple):
         _check("plan_compaction", self.status)
 
 
-@functools.lru_cache(maxsize=None)
-def _forks_kernel():
-    smem = 4 * MAX_ROWS * 4 + 3 * (LIST_THREADS // 32) * 4 + 4
-    cfg = rt.KernelConfig(kind=rt.KIND_PLAN_FORKS, threads=LIST_THREADS, smem_bytes=smem)
-    return rt.compile_module(rt.kernel_source("page_lists.cuh", "plan_forks.cuh", defines=FORKS_DEFINES), "ae_plan_forks", cfg)
+def _list_source(file: str, phase: int) -> str:
+    return rt.kernel_source("page_lists.cuh", file, defines={"AE_LIST_THREADS": LIST_THREADS[phase > 0], "AE_LIST_BATCH": LIST_BATCH, "AE_PHASE": phase})
+
+
+def _list_kernels(kind: int, file: str, name: str, phases: int):
+    """The kernel that runs all phases in one CTA, then one for each phase."""
+    out = []
+    for phase in range(phases + 1):
+        cfg = rt.KernelConfig(kind=kind, threads=LIST_THREADS[phase > 0], smem_bytes=0 if phase else LIST_SMEM)
+        cfg.reserved[1] = phase
+        out.append(rt.compile_module(_list_source(file, phase), name, cfg))
+    return tuple(out), [m.handle.value for m in out]
 
 
 @functools.lru_cache(maxsize=None)
-def _compaction_kernel():
-    cfg = rt.KernelConfig(kind=rt.KIND_PLAN_COMPACTION, threads=LIST_THREADS)
-    return rt.compile_module(rt.kernel_source("page_lists.cuh", "plan_compaction.cuh", defines=LIST_DEFINES), "ae_plan_compaction", cfg)
+def _forks_kernels():
+    return _list_kernels(rt.KIND_PLAN_FORKS, "plan_forks.cuh", "ae_plan_forks", 3)
+
+
+@functools.lru_cache(maxsize=None)
+def _compaction_kernels():
+    return _list_kernels(rt.KIND_PLAN_COMPACTION, "plan_compaction.cuh", "ae_plan_compaction", 4)
 
 
 @functools.lru_cache(maxsize=None)
@@ -100,7 +110,7 @@ def plan_forks(parents, seq_lens, block_table, free_pages, free_head, page_size:
     Pages that something beside the table's rows is to keep (a prefix for later requests) need a row of their own in it.  What does not fit is left
     out and reported in ``status``."""
     _sizes(page_size, num_pages)
-    r = rt.host().plan_forks(_forks_kernel().handle.value, parents, seq_lens, block_table, free_pages, free_head, page_size, num_pages, keep_lens)
+    r = rt.host().plan_forks(_forks_kernels()[1], parents, seq_lens, block_table, free_pages, free_head, page_size, num_pages, keep_lens)
     if r is None:
         named = [("parents", parents, 1), ("seq_lens", seq_lens, 1), ("block_table", block_table, 2), ("free_pages", free_pages, 1),
                  ("free_head", free_head, 1)] + ([("keep_lens", keep_lens, 1)] if keep_lens is not None else [])
@@ -119,7 +129,7 @@ def plan_compaction(seq_lens, block_table, page_size: int, num_pages: int) -> Co
     Every page that no row holds counts as unused, so all of a pool's rows have to be in the table.  ``copy_pages(caches, plan.copies)`` has to
     follow before the new table is used."""
     _sizes(page_size, num_pages)
-    r = rt.host().plan_compaction(_compaction_kernel().handle.value, seq_lens, block_table, page_size, num_pages)
+    r = rt.host().plan_compaction(_compaction_kernels()[1], seq_lens, block_table, page_size, num_pages)
     if r is None:
         _refuse([("seq_lens", seq_lens, 1), ("block_table", block_table, 2)], seq_lens, block_table, page_size, num_pages)
         raise ValueError("seq_lens [B] and block_table [B, max_pages] of a row at least")
@@ -131,8 +141,8 @@ def _refuse(named, seq_lens, block_table, page_size, num_pages):
         _ints(name, t, dim, seq_lens.device)
     if page_size < 1 or page_size > 2 ** 30 or page_size & (page_size - 1):
         raise ValueError(f"page_size {page_size}: a power of two")
-    if not 1 <= num_pages <= 0x7ffffff0:
-        raise ValueError(f"num_pages {num_pages}: at least 1")
+    if not 1 <= num_pages <= 0x3fffffff:
+        raise ValueError(f"num_pages {num_pages}: 1 to 2^30 - 1")
     if block_table.shape[0] != seq_lens.shape[0] or block_table.shape[1] < 1 or block_table.numel() > 0x7fffffff:
         raise ValueError(f"block_table must be [{seq_lens.shape[0]}, max_pages] with a column at least and fewer than 2^31 entries, got {tuple(block_table.shape)}")
 

@@ -27,7 +27,8 @@ def turns_of(frequency: float) -> int:
     return round((t - math.floor(t)) * 2 ** 64) % 2 ** 64
 
 
-SHAPES = ((4, 4, 0), (8, 2, 2), (8, 1, 2))  # warps of a CTA, heads of a team on their way, CTAs of an SM (backward), of each kernel
+# of each kernel: warps of a CTA, heads of a team on their way together (the forward takes four, two or one itself), CTAs of an SM
+SHAPES = ((4, 4, 4), (8, 1, 3), (8, 1, 1))
 
 
 def _defines(D: int, R: int, norm: bool, interleaved: bool, which: int) -> dict:
@@ -41,7 +42,9 @@ def _kernels(D: int, R: int, norm: bool, interleaved: bool):
     out = []
     for i, name in enumerate(("ae_qk_rope_fwd", "ae_qk_rope_bwd", "ae_qk_rope_dw")):
         cfg = rt.KernelConfig(kind=rt.KIND_QK_ROPE, head_dim=D, threads=32 * SHAPES[i][0])
-        cfg.reserved[0], cfg.reserved[1], cfg.reserved[2] = R, SHAPES[i][1], SHAPES[i][2]
+        cfg.reserved[0] = R
+        for j in range(3):
+            cfg.reserved[1 + j] = SHAPES[min(i, 1)][j]  # the sums: the backward's
         out.append(rt.compile_module(rt.kernel_source("qk_norm_rope.cuh", defines=_defines(D, R, norm, interleaved, i)), name, cfg))
     return tuple(out)
 

@@ -578,13 +578,20 @@ bool good_table(const Tensor& table, const Tensor& like, int64_t B) {
   return good_ints(table, 2, like) && table.size(0) == B && table.size(1) >= 1 && B * table.size(1) <= 0x7fffffff;
 }
 
+// One launch with the first kernel, or one for each of the others.
+template <class P, class F>
+void list_phases(const std::vector<uint64_t>& kernels, const P& p, F&& launch) {
+  if (ae_plan_lists_phases(p.B, p.max_pages, p.num_pages) == 0) return launch(handle(kernels.at(0)));
+  for (size_t i = 1; i < kernels.size(); ++i) launch(handle(kernels[i]));
+}
+
 // (block_table, seq_lens, free_pages, free_head, copies, status), or None.
-py::object plan_forks(uint64_t kernel, const Tensor& parents, const Tensor& lens, const Tensor& table, const Tensor& free_pages,
+py::object plan_forks(const std::vector<uint64_t>& kernels, const Tensor& parents, const Tensor& lens, const Tensor& table, const Tensor& free_pages,
                       const Tensor& free_head, int64_t page_size, int64_t num_pages, const std::optional<Tensor>& keep) {
   const int64_t B = lens.dim() == 1 ? lens.size(0) : 0;
   if (B < 1 || B > 4096 || !good_ints(lens, 1, lens) || !good_ints(parents, 1, lens) || parents.size(0) != B || !good_table(table, lens, B) ||
       !good_ints(free_pages, 1, lens) || !good_ints(free_head, 1, lens) || free_head.size(0) != 1 || (keep && (!good_ints(*keep, 1, lens) || keep->size(0) != B)) ||
-      !good_page_size(page_size) || num_pages < 1 || num_pages > 0x7ffffff0 || free_pages.size(0) > 0x7fffffff)
+      !good_page_size(page_size) || num_pages < 1 || num_pages > 0x3fffffff || free_pages.size(0) > 0x7fffffff)
     return py::none();
   py::gil_scoped_release nogil;
   c10::cuda::CUDAGuard guard(lens.device());
@@ -593,7 +600,7 @@ py::object plan_forks(uint64_t kernel, const Tensor& parents, const Tensor& lens
   Parts parts(4 * B + B * W + B + n_free + 2, lens.options());
   Tensor copies = parts.take({B, 4}), table_out = parts.take({B, W}), lens_out = parts.take({B}), free_out = parts.take({n_free}), head = parts.take({1}),
          status = parts.take({1});
-  const Tensor workspace = at::empty({ae_plan_lists_workspace((int)num_pages)}, lens.options().dtype(at::kByte));
+  const Tensor workspace = at::empty({ae_plan_lists_workspace((int)B, (int)num_pages)}, lens.options().dtype(at::kByte));
   AePlanForksParams p;
   memset(&p, 0, sizeof p);
   p.parents = (const int32_t*)parents.data_ptr(); p.seq_lens = (const int32_t*)lens.data_ptr();
@@ -604,15 +611,15 @@ py::object plan_forks(uint64_t kernel, const Tensor& parents, const Tensor& lens
   p.head_out = (int32_t*)head.data_ptr(); p.copies = (int32_t*)copies.data_ptr(); p.status = word(status); p.workspace = workspace.data_ptr();
   p.table_stride = table.stride(0);
   p.B = (int)B; p.max_pages = (int)W; p.n_free = (int)n_free; p.page_size = (int)page_size; p.num_pages = (int)num_pages;
-  check(ae_launch_plan_forks(handle(kernel), &p, stream_of(lens)), "ae_launch_plan_forks");
+  list_phases(kernels, p, [&](void* k) { check(ae_launch_plan_forks(k, &p, stream_of(lens)), "ae_launch_plan_forks"); });
   py::gil_scoped_acquire gil;
   return py::make_tuple(table_out, lens_out, free_out, head, copies, status);
 }
 
 // (block_table, free_pages, free_head, copies, status), or None.
-py::object plan_compaction(uint64_t kernel, const Tensor& lens, const Tensor& table, int64_t page_size, int64_t num_pages) {
+py::object plan_compaction(const std::vector<uint64_t>& kernels, const Tensor& lens, const Tensor& table, int64_t page_size, int64_t num_pages) {
   const int64_t B = lens.dim() == 1 ? lens.size(0) : 0;
-  if (B < 1 || !good_ints(lens, 1, lens) || !good_table(table, lens, B) || !good_page_size(page_size) || num_pages < 1 || num_pages > 0x7ffffff0)
+  if (B < 1 || !good_ints(lens, 1, lens) || !good_table(table, lens, B) || !good_page_size(page_size) || num_pages < 1 || num_pages > 0x3fffffff)
     return py::none();
   py::gil_scoped_release nogil;
   c10::cuda::CUDAGuard guard(lens.device());
@@ -620,7 +627,7 @@ py::object plan_compaction(uint64_t kernel, const Tensor& lens, const Tensor& ta
   const int64_t W = table.size(1), n = num_pages / 2;
   Parts parts(4 * n + B * W + num_pages + 2, lens.options());
   Tensor copies = parts.take({n, 4}), table_out = parts.take({B, W}), free_out = parts.take({num_pages}), head = parts.take({1}), status = parts.take({1});
-  const Tensor workspace = at::empty({ae_plan_lists_workspace((int)num_pages)}, lens.options().dtype(at::kByte));
+  const Tensor workspace = at::empty({ae_plan_lists_workspace((int)B, (int)num_pages)}, lens.options().dtype(at::kByte));
   AePlanCompactionParams p;
   memset(&p, 0, sizeof p);
   p.seq_lens = (const int32_t*)lens.data_ptr(); p.block_table = (const int32_t*)table.data_ptr();
@@ -628,7 +635,7 @@ py::object plan_compaction(uint64_t kernel, const Tensor& lens, const Tensor& ta
   p.copies = (int32_t*)copies.data_ptr(); p.status = word(status); p.workspace = workspace.data_ptr();
   p.table_stride = table.stride(0);
   p.B = (int)B; p.max_pages = (int)W; p.page_size = (int)page_size; p.num_pages = (int)num_pages; p.n_copies = (int)n;
-  check(ae_launch_plan_compaction(handle(kernel), &p, stream_of(lens)), "ae_launch_plan_compaction");
+  list_phases(kernels, p, [&](void* k) { check(ae_launch_plan_compaction(k, &p, stream_of(lens)), "ae_launch_plan_compaction"); });
   py::gil_scoped_acquire gil;
   return py::make_tuple(table_out, free_out, head, copies, status);
 }

@@ -1283,14 +1283,31 @@ int ae_launch_decode_combine(void* module, const AeDecodeParams* p, void* stream
   return launch_after(m, combine_blocks(a.H, a.DV), (unsigned)p->B, 1, &a, stream);
 }
 
-// The planners of a pool's pages run as one cluster (page_lists.cuh); behind a word for each page the workspace has one for each of its CTAs.
-static const int kListCtas = 8;
-static int64_t list_words(int32_t num_pages) { return ((int64_t)num_pages + 3) / 4 * 4; }
-int64_t ae_plan_lists_workspace(int32_t num_pages) { return (list_words(std::max(num_pages, 0)) + 16) * 4; }
+// The planners of a pool's pages (page_lists.cuh): one CTA for small tables and pools, a launch for each phase for others.  Microseconds in a graph, one CTA /
+// launches: forks of 16 x 101 table entries 5.9 / 7.9, 64 x 65 7.3 / 8.4, 64 x 129 9.3 / 8.5, 128 x 129 13.2 / 9.4; compactions 5.8 / 8.7, 7.6 / 10.1,
+// 11.1 / 10.2, 18.0 / 10.8; on the host 10 / 15.
+static int64_t list_words(int32_t num_pages) { return ((int64_t)num_pages + 127) / 128 * 4; }
+int64_t ae_plan_lists_workspace(int32_t B, int32_t num_pages) { return 16 * (int64_t)B + 12 * list_words(num_pages) + 4 * (int64_t)num_pages; }
+static const int kListRows = 1024, kListPages = 16384;  // of the one CTA: its shared memory
+int ae_plan_lists_phases(int32_t B, int32_t max_pages, int32_t num_pages) {
+  return B > kListRows || num_pages > kListPages || (int64_t)B * max_pages > 8192;
+}
 
 static bool list_args_ok(int B, int max_pages, int page_log2, int num_pages, const void* copies, const void* workspace) {
-  return page_log2 >= 0 && B >= 1 && max_pages >= 1 && num_pages >= 1 && num_pages <= 0x7ffffff0 && (int64_t)B * max_pages <= 0x7fffffff &&
+  return page_log2 >= 0 && B >= 1 && max_pages >= 1 && num_pages >= 1 && num_pages <= 0x3fffffff && (int64_t)B * max_pages <= 0x7fffffff &&
          !((reinterpret_cast<uintptr_t>(copies) | reinterpret_cast<uintptr_t>(workspace)) & 15);
+}
+
+// items: what the phase works through, in fours a thread, and the most CTAs that it takes
+static int launch_lists(Module* m, int64_t items, int most, void* args, void* stream) {
+  const int64_t per = 4 * (int64_t)m->cfg.threads;
+  const int64_t ctas = m->cfg.reserved[1] == 0 ? 1 : std::min<int64_t>(std::max<int64_t>((items + per - 1) / per, 1), most);
+  return launch_after(m, (unsigned)ctas, 1, 1, args, stream);
+}
+
+// Whether the module with all phases has the shared memory for these rows and pages.
+static bool lists_fit(const Module* m, int64_t B, int64_t num_pages) {
+  return m->cfg.reserved[1] != 0 || 16 * B + 12 * list_words((int32_t)num_pages) + 6 * num_pages + 16 <= m->cfg.smem_bytes;
 }
 
 int ae_launch_plan_forks(void* module, const AePlanForksParams* p, void* stream) {
@@ -1303,8 +1320,9 @@ int ae_launch_plan_forks(void* module, const AePlanForksParams* p, void* stream)
     return AE_ERR_UNSUPPORTED;
   }
   const int log2 = page_log2_of(p->page_size);
-  if (!list_args_ok(p->B, p->max_pages, log2, p->num_pages, p->copies, p->workspace) || p->B > 4096 || p->n_free < 0 ||
-      (const int32_t*)p->table_out == p->block_table || (const int32_t*)p->free_out == p->free_pages || (const int32_t*)p->lens_out == p->seq_lens) {
+  if (!list_args_ok(p->B, p->max_pages, log2, p->num_pages, p->copies, p->workspace) || p->B > 4096 || p->n_free < 0 || !lists_fit(m, p->B, p->num_pages) ||
+      (const int32_t*)p->table_out == p->block_table || (p->n_free > 0 && (const int32_t*)p->free_out == p->free_pages) ||
+      (const int32_t*)p->lens_out == p->seq_lens) {
     set_error("plan_forks: 1 to 4096 rows, a page size that is a power of two, a pool, outputs that are no inputs");
     return AE_ERR_INVALID;
   }
@@ -1314,9 +1332,12 @@ int ae_launch_plan_forks(void* module, const AePlanForksParams* p, void* stream)
   memset(&a, 0, sizeof a);
   a.parents = p->parents; a.lens = p->seq_lens; a.keep = p->keep_lens; a.table = p->block_table; a.free_pages = p->free_pages;
   a.free_head = p->free_head; a.table_out = p->table_out; a.lens_out = p->lens_out; a.free_out = p->free_out; a.head_out = p->head_out;
-  a.copies = (AePageCopy*)p->copies; a.status = p->status; a.state = (u32*)p->workspace; a.counts = (int*)a.state + list_words(p->num_pages);
+  a.copies = (AePageCopy*)p->copies; a.status = p->status;
+  a.rows = (AeInt4*)p->workspace; a.held = (u32*)(a.rows + p->B); a.words = (int)list_words(p->num_pages);
   a.table_stride = p->table_stride; a.B = p->B; a.max_pages = p->max_pages; a.n_free = p->n_free; a.page_log2 = log2; a.num_pages = p->num_pages;
-  return launch_cluster(m, kListCtas, 1, 1, kListCtas, &a, stream);
+  const int phase = m->cfg.reserved[1];
+  const int64_t items = phase == 1 ? std::max(p->B, a.words) : phase == 2 ? (int64_t)p->B * p->max_pages : std::max<int64_t>(p->n_free, 64 * (int64_t)a.words);
+  return launch_lists(m, items, phase == 2 ? 296 : 148, &a, stream);
 }
 
 int ae_launch_plan_compaction(void* module, const AePlanCompactionParams* p, void* stream) {
@@ -1329,7 +1350,7 @@ int ae_launch_plan_compaction(void* module, const AePlanCompactionParams* p, voi
     return AE_ERR_UNSUPPORTED;
   }
   const int log2 = page_log2_of(p->page_size);
-  if (!list_args_ok(p->B, p->max_pages, log2, p->num_pages, p->copies, p->workspace) || p->n_copies < p->num_pages / 2 ||
+  if (!list_args_ok(p->B, p->max_pages, log2, p->num_pages, p->copies, p->workspace) || p->n_copies < p->num_pages / 2 || !lists_fit(m, 0, p->num_pages) ||
       (const int32_t*)p->table_out == p->block_table) {
     set_error("plan_compaction: rows, a page size that is a power of two, a pool, room for num_pages / 2 copies");
     return AE_ERR_INVALID;
@@ -1339,10 +1360,12 @@ int ae_launch_plan_compaction(void* module, const AePlanCompactionParams* p, voi
   AePlanCompactionArgs a;
   memset(&a, 0, sizeof a);
   a.lens = p->seq_lens; a.table = p->block_table; a.table_out = p->table_out; a.free_out = p->free_out; a.head_out = p->head_out;
-  a.copies = (AePageCopy*)p->copies; a.status = p->status; a.state = (u32*)p->workspace; a.counts = (int*)a.state + list_words(p->num_pages);
+  a.copies = (AePageCopy*)p->copies; a.status = p->status; a.held = (u32*)p->workspace; a.words = (int)list_words(p->num_pages);
   a.table_stride = p->table_stride; a.B = p->B; a.max_pages = p->max_pages; a.page_log2 = log2; a.num_pages = p->num_pages;
   a.n_copies = p->n_copies;
-  return launch_cluster(m, kListCtas, 1, 1, kListCtas, &a, stream);
+  const int phase = m->cfg.reserved[1];
+  const int64_t items = phase == 1 ? std::max<int64_t>(std::max(p->B, p->num_pages), p->n_copies) : phase == 3 ? 64 * (int64_t)a.words : (int64_t)p->B * p->max_pages;
+  return launch_lists(m, items, phase == 3 ? 148 : 296, &a, stream);
 }
 
 int ae_launch_copy_pages(void* module, const AeCopyPagesParams* p, void* stream) {
@@ -1387,7 +1410,7 @@ int ae_launch_copy_pages(void* module, const AeCopyPagesParams* p, void* stream)
 static const int kRopeSms = 148;
 int64_t ae_qk_rope_workspace(void* module) {
   const Module* m = (const Module*)module;
-  return m && m->cfg.kind == AE_KIND_QK_ROPE ? (int64_t)kRopeSms * m->cfg.reserved[2] * m->cfg.head_dim * 4 + 2 * m->cfg.head_dim * 4 : 0;
+  return m && m->cfg.kind == AE_KIND_QK_ROPE ? ((int64_t)kRopeSms * m->cfg.reserved[3] + 2) * m->cfg.head_dim * 4 : 0;
 }
 
 int ae_launch_qk_rope(void* module, const AeQkRopeParams* p, void* stream) {
@@ -1399,7 +1422,7 @@ int ae_launch_qk_rope(void* module, const AeQkRopeParams* p, void* stream) {
   }
   const bool bwd = m->kernel == "ae_qk_rope_bwd", sums = m->kernel == "ae_qk_rope_dw";
   const int64_t T = (int64_t)p->B * p->S;
-  const int D = m->cfg.head_dim, warps = m->cfg.threads / 32, teams = 512 / D;
+  const int D = m->cfg.head_dim, teams = 512 / D, warps = m->cfg.reserved[1];
   if (p->B < 0 || p->S < 0 || p->H[0] < 1 || p->H[1] < 0 || T > 0x7fffffff || (int64_t)p->H[0] * D > 0x7fffffff || (int64_t)p->H[1] * D > 0x7fffffff) {
     set_error("norm and rotation: bad shape");
     return AE_ERR_INVALID;
@@ -1428,17 +1451,25 @@ int ae_launch_qk_rope(void* module, const AeQkRopeParams* p, void* stream) {
   a.bf16 = p->dtype == AE_DTYPE_BF16; a.w32 = p->w_fp32; a.pos64 = p->pos_int64; a.eps = p->eps; a.scale = p->rotary_scale;
   a.dw_part = p->workspace;
   memcpy(a.turns, p->turns, sizeof a.turns);
-  // heads of a warp: eight for each team, fewer while the tokens do not give every SM 16 warps
+  // heads of a warp: all of a token's (backward: of its queries or keys), fewer while the tokens do not give every SM 16 warps
+  const bool both = !bwd && !sums;
   auto slices = [&](int per) {
-    for (int i = 0; i < 2; ++i) a.slices[i] = (a.H[i] + per - 1) / per;
+    a.slices[0] = ((both ? a.H[0] + a.H[1] : a.H[0]) + per - 1) / per;
+    a.slices[1] = both ? 0 : (a.H[1] + per - 1) / per;
     return (int64_t)a.slices[0] + a.slices[1];
   };
-  a.per = teams * 8;
-  while (a.per > teams && T * slices(a.per) < kRopeSms * 16) a.per /= 2;
+  a.per = ((both ? a.H[0] + a.H[1] : std::max(a.H[0], a.H[1])) + teams - 1) / teams * teams;
+  while (a.per > teams && T * slices(a.per) < kRopeSms * 16) a.per = (a.per / 2 + teams - 1) / teams * teams;
   const int64_t items = T * slices(a.per);
-  if (bwd || sums) {
-    // queries' and keys' CTAs in proportion to their heads
-    const int64_t most = (int64_t)kRopeSms * m->cfg.reserved[2];
+  if (items > 0x7fffffff - kRopeSms * 64) {
+    set_error("norm and rotation: too many heads for one launch");
+    return AE_ERR_INVALID;
+  }
+  // Inputs that L2 does not hold are asked for early: 16029 tokens of 40 heads of 128 dims (118 MB) 42.9 -> 39.3 us; 3333 of 32 heads of 64 dims, 14 MB
+  // in L2 from the call before, 7.0 -> 7.4.
+  a.prefetch = both && a.slices[0] == 1 && T * (a.H[0] + a.H[1]) * D * 2 > (48 << 20);
+  if (!both) {  // queries' and keys' CTAs in proportion to their heads
+    const int64_t most = (int64_t)kRopeSms * m->cfg.reserved[3];
     for (int i = 0; i < 2; ++i) {
       const int64_t need = (T * a.slices[i] + warps - 1) / warps, share = most * a.H[i] / (a.H[0] + a.H[1]);
       a.ctas[i] = a.H[i] == 0 ? 0 : (int)std::min(need, std::max<int64_t>(share, 1));
@@ -1451,10 +1482,6 @@ int ae_launch_qk_rope(void* module, const AeQkRopeParams* p, void* stream) {
     return launch_after(m, (unsigned)(D / 32), p->H[1] > 0 ? 2 : 1, 1, &a, stream);
   }
   if (bwd) return launch_after(m, (unsigned)(a.ctas[0] + a.ctas[1]), 1, 1, &a, stream);
-  if ((items + warps - 1) / warps > 0x7fffffff / warps) {
-    set_error("norm and rotation: too many heads for one launch");
-    return AE_ERR_INVALID;
-  }
   return launch_after(m, (unsigned)((items + warps - 1) / warps), 1, 1, &a, stream);
 }
 

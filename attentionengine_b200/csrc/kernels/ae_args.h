@@ -324,6 +324,15 @@ struct AeCache8MergeArgs {  // kernel ae_cache8_merge
   int Hq, gq, rows;
 };
 
+// int4 where a kernel is compiled; the host knows its size alone
+#ifdef __CUDACC__
+typedef int4 AeInt4;
+#else
+struct alignas(16) AeInt4 {
+  int x, y, z, w;
+};
+#endif
+
 // ---- pages of rows that go on from others, are cut or end (kernel ae_plan_forks) ----------------
 struct alignas(16) AePageCopy {
   int src, dst;  // pages
@@ -343,10 +352,11 @@ struct AePlanForksArgs {
   int* head_out;          // [1]
   AePageCopy* copies;     // [B]
   u32* status;            // [1] written
-  u32* state;             // [num_pages rounded up to 4] scratch
-  int* counts;            // [clusters' CTAs] scratch
+  // scratch of the launches for single phases
+  AeInt4* rows;           // [B] what a row takes over: parent or -1, tokens, begun page or -1, pages held before
+  u32* held;              // 3 [words] pages held before, now whole, now begun; [num_pages] of begun pages: the least key of the rows
   i64 table_stride;
-  int B, max_pages, n_free, page_log2, num_pages;
+  int B, max_pages, n_free, page_log2, num_pages, words;
 };
 
 // ---- pages moved to the front of the pool (kernel ae_plan_compaction) ----------------------------
@@ -358,10 +368,9 @@ struct AePlanCompactionArgs {
   int* head_out;       // [1]
   AePageCopy* copies;  // [n_copies], num_pages / 2
   u32* status;         // [1] written
-  u32* state;          // [num_pages rounded up to 4] scratch
-  int* counts;         // [clusters' CTAs] scratch
+  u32* held;           // scratch of the launches for single phases: 2 [words] pages that are whole, begun; [num_pages] a begun page's slots, a moving one's place
   i64 table_stride;
-  int B, max_pages, page_log2, num_pages, n_copies;
+  int B, max_pages, page_log2, num_pages, words, n_copies;
 };
 
 // ---- copies of pages (kernel ae_copy_pages) --------------------------------------------------------
@@ -398,9 +407,10 @@ struct AeQkRopeArgs {
   i64 pos_st[2];
   int H[2];
   int S, T;               // positions of a batch row; T = B S
-  int per, slices[2];     // heads of a warp, and how many warps they make of a token's
+  int per, slices[2];     // heads of a warp, and how many warps they make of a token's queries and keys (forward: of both as one line, slices[0])
   int ctas[2];            // backward
   int bf16, w32, pos64;
+  int prefetch;           // forward: a token's heads into L2 first
   float eps, scale;
   u64 turns[AE_ROPE_MAX_PAIRS];  // of each pair, a position's fraction of a turn in units of 2^-64
 };

@@ -18,10 +18,10 @@ AE_DEVICE void ae_copy_part(const AeCopyPool& p, const u8* src, u8* dst, int fro
       V v[AE_COPY_UNROLL];
 #pragma unroll
       for (int u = 0; u < AE_COPY_UNROLL; ++u)
-        if (i + u * AE_COPY_THREADS < n) v[u] = ((const V*)src)[i + u * AE_COPY_THREADS];
+        if (i + u * AE_COPY_THREADS < n) v[u] = __ldcs((const V*)src + i + u * AE_COPY_THREADS);
 #pragma unroll
       for (int u = 0; u < AE_COPY_UNROLL; ++u)
-        if (i + u * AE_COPY_THREADS < n) ((V*)dst)[i + u * AE_COPY_THREADS] = v[u];
+        if (i + u * AE_COPY_THREADS < n) __stcs((V*)dst + i + u * AE_COPY_THREADS, v[u]);
     }
   } else {
     for (int i = from + threadIdx.x; i < from + n; i += AE_COPY_THREADS) {

@@ -1,131 +1,137 @@
 // Moves every page in use to the front of its pool: with U pages in use, those from U on go into the unused ones below it, both in ascending order.
 // Written are the block tables with the new numbers, the list of copies {page, new page, slots in use} and the free list (all pages, U of them taken).
 //
-// One word a page holds how many of its slots the rows use (a maximum, so the order of the atomics does not show), then for a page that moves its place in
-// the list.  One running sum over the pages serves both sides: x is hole number x - (in use below x), or mover number (in use below x) - (in use
-// below U).  Holes write the list's second number, moving pages the others.
-// Expects AE_LIST_THREADS, AE_LIST_CTAS, AE_LIST_BATCH (table entries of a thread on their way together).
-extern "C" __global__ void __launch_bounds__(AE_LIST_THREADS) ae_plan_compaction(const __grid_constant__ AePlanCompactionArgs a) {
-  __shared__ int warp_sum[2][AE_LIST_THREADS / 32];
-  __shared__ u32 sm_bad;
-  ae_grid_wait();
-  ae_grid_trigger();
-  const int cta = (int)cluster_ctarank(), tid = (int)threadIdx.x, lane = tid & 31;
-  const int gtid = cta * AE_LIST_THREADS + tid, gstep = AE_LIST_CTAS * AE_LIST_THREADS;
-  const int P = 1 << a.page_log2, B = a.B, W = a.max_pages, groups = (a.num_pages + 3) / 4;
-  const i64 most = (i64)W << a.page_log2;
-  u32 bad = 0;
-  if (tid == 0) sm_bad = 0;
-  if (gtid == 0) *a.status = 0;
-  for (int i = gtid; i < groups; i += gstep) ((uint4*)a.state)[i] = make_uint4(0, 0, 0, 0);
-  for (int i = gtid; i < a.n_copies; i += gstep) ((uint4*)a.copies)[i] = make_uint4(0, 0, 0, 0);
-  for (int i = gtid; i < a.num_pages; i += gstep) a.free_out[i] = i;
-  ae_phase_end();
+// Phase 1 clears the bitmaps and the slots of begun pages; phase 2 sets the pages' bits (held whole, begun) and takes the maximum of a begun page's slots; in
+// phase 3 one running sum over the pages serves both sides: page x is hole number x - (in use below x), or mover number (in use below x) - (in use below
+// U), and holes write the list's second number, moving pages the others; phase 4 writes the tables.
 
-  // how many slots of each page are in use
-  const int warps = gstep / 32, chunks = (W + 31) / 32, gwarp = cta * (AE_LIST_THREADS / 32) + (tid >> 5);
-  auto tokens_of = [&](int len) { return min((i64)max(len, 0), most); };
-  for (int i0 = gwarp; i0 < B * chunks; i0 += warps * AE_LIST_BATCH) {
+AE_DEVICE int ae_len(const AePlanCompactionArgs& a, int r) {  // in the table
+  return (int)min((i64)max(a.lens[r], 0), (i64)a.max_pages << a.page_log2);
+}
+
+AE_DEVICE void ae_pack_rows(const AePlanCompactionArgs& a, const AeListState& st, const AeListShare sh) {
+  if (sh.first() == 0) *a.status = 0;
+  for (u32 i = sh.first(); i < 2u * (u32)a.words / 4; i += sh.step()) ((uint4*)st.whole)[i] = make_uint4(0, 0, 0, 0);
+  for (u32 r = sh.first(); r < (u32)a.B; r += sh.step()) {
+    const int n = ae_len(a, (int)r);
+    if (n & ((1 << a.page_log2) - 1)) {
+      const int page = a.table[(i64)r * a.table_stride + (n >> a.page_log2)];
+      if (ae_in_pool(page, a.num_pages)) st.owner[page] = 0;
+    }
+  }
+  for (u32 i = sh.first(); i < (u32)a.n_copies; i += sh.step()) ((uint4*)a.copies)[i] = make_uint4(0, 0, 0, 0);
+  for (u32 i = sh.first(); i < (u32)a.num_pages; i += sh.step()) a.free_out[i] = (int)i;
+}
+
+AE_DEVICE void ae_pack_marks(const AePlanCompactionArgs& a, const AeListState& st, const AeListShare sh) {
+  const int P = 1 << a.page_log2;
+  u32 bad = 0;
+  for (AeEntries e(sh, a.B, a.max_pages); e.more();) {
     int page[AE_LIST_BATCH], slots[AE_LIST_BATCH];
 #pragma unroll
     for (int j = 0; j < AE_LIST_BATCH; ++j) {  // the reads in front of the atomics, which the compiler moves no read across
       page[j] = slots[j] = 0;
-      const int i = i0 + j * warps;
-      if (i >= B * chunks) continue;
-      const int r = i / chunks, c = (i - r * chunks) * 32 + lane, len = a.lens[r];
-      if (c == 0) bad |= len < 0 ? 8u : len > most ? 2u : 0u;
-      slots[j] = c < W ? (int)min(max(tokens_of(len) - ((i64)c << a.page_log2), (i64)0), (i64)P) : 0;
-      if (slots[j]) page[j] = a.table[(i64)r * a.table_stride + c];
+      if (e.more()) {
+        const int n = ae_len(a, e.r);
+        if (e.c == 0) bad |= a.lens[e.r] < 0 ? 8u : a.lens[e.r] > n ? 2u : 0u;
+        if (e.c < (int)(((i64)n + P - 1) >> a.page_log2)) {
+          slots[j] = min(n - (e.c << a.page_log2), P);
+          page[j] = a.table[(i64)e.r * a.table_stride + e.c];
+        }
+      }
+      e.next(sh.step());
     }
 #pragma unroll
     for (int j = 0; j < AE_LIST_BATCH; ++j) {
       if (!slots[j]) continue;
-      if (page[j] >= 0 && page[j] < a.num_pages)
-        atomicMax(a.state + page[j], (u32)slots[j]);
-      else
+      if (!ae_in_pool(page[j], a.num_pages)) {
         bad |= 16u;
-    }
-  }
-  ae_phase_end();
-
-  // pages in use in front of a thread's share
-  int first, end, mine = 0;
-  ae_page_share(a.num_pages, cta, first, end);
-  const int share = (end - first) / 4, tper = (share + AE_LIST_THREADS - 1) / AE_LIST_THREADS;
-  const int g0 = first / 4 + min(tid * tper, share), g1 = min(g0 + tper, end / 4);
-#pragma unroll 4
-  for (int g = g0; g < g1; ++g) {
-    const uint4 u = __ldcg((const uint4*)a.state + g);
-    mine += (u.x != 0) + (u.y != 0) + (u.z != 0) + (u.w != 0);
-  }
-  int cta_used, used = 0;
-  int before = ae_cta_scan(mine, warp_sum[0], cta_used);
-  if (tid == 0) a.counts[cta] = cta_used;
-  if (bad) atomicOr(&sm_bad, bad);
-  ae_phase_end();
-#pragma unroll
-  for (int i = 0; i < AE_LIST_CTAS; ++i) {
-    const int n = __ldcg(a.counts + i);
-    if (i < cta) before += n;
-    used += n;
-  }
-  // those below page `used`: whole shares, and a part of the one that it lies in, counted by every CTA for itself
-  int below = 0, part = 0;
-  for (int i = 0; i < AE_LIST_CTAS; ++i) {
-    int f, e;
-    ae_page_share(a.num_pages, i, f, e);
-    if (e <= used)
-      below += __ldcg(a.counts + i);
-    else if (f < used)
-      for (int x = f + tid; x < used; x += AE_LIST_THREADS) part += __ldcg(a.state + x) != 0;
-  }
-  ae_cta_scan(part, warp_sum[1], part);
-  below += part;
-  for (int g = g0; g < g1; ++g) {
-    const uint4 u = __ldcg((const uint4*)a.state + g);
-    const u32 w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int page = g * 4 + k;
-      if (page >= a.num_pages) break;
-      if (w[k]) {
-        const int place = before++ - below;
-        if (page >= used) {
-          a.copies[place].src = page;
-          a.copies[place].slots = (int)w[k];
-          a.state[page] = (u32)place;
-        }
-      } else if (page < used) {
-        a.copies[page - before].dst = page;
+      } else if (slots[j] == P) {
+        ae_set_bit(st.whole, page[j]);
+      } else {
+        ae_set_bit(st.begun, page[j]);
+        atomicMax(st.owner + page[j], (u32)slots[j]);
       }
     }
   }
-  if (gtid == 0) *a.head_out = used;
-  if (tid == 0 && sm_bad) atomicOr(a.status, sm_bad);
-  ae_phase_end();
+  if (bad) atomicOr(a.status, bad);
+}
 
-  // the tables with the new numbers
-  for (int i0 = gwarp; i0 < B * chunks; i0 += warps * AE_LIST_BATCH) {
+AE_DEVICE int ae_pack_lists(const AePlanCompactionArgs& a, const AeListState& st, const AeListShare sh) {
+  auto in_use = [&](int w) { return ae_word(st.whole + w) | ae_word(st.begun + w); };
+  const int share = (a.words + sh.ctas - 1) / sh.ctas, w0 = min(sh.cta * share, a.words), w1 = min(w0 + share, a.words);
+  int before, used, below, all;
+  ae_count_bits(a.words, w0, in_use, before, used);
+  auto low = [&](int w) { return w * 32 + 32 <= used ? 0xffffffffu : w * 32 >= used ? 0u : (1u << (used & 31)) - 1; };  // pages below `used`
+  ae_count_bits(a.words, a.words, [&](int w) { return in_use(w) & low(w); }, below, all);
+  ae_each_page(w0, w1, before, in_use, [&](int page, bool is, int j) {
+    if (page < used && !is) {
+      a.copies[page - j].dst = page;
+      if (st.holes) st.holes[page - j] = page;
+    } else if (page >= used && is) {
+      const int place = j - below;
+      const bool whole = ae_word(st.whole + (page >> 5)) >> (page & 31) & 1;
+      a.copies[place].src = page;
+      a.copies[place].slots = whole ? 1 << a.page_log2 : (int)ae_word(st.owner + page);
+      st.owner[page] = (u32)place;
+    }
+  });
+  if (sh.first() == 0) *a.head_out = used;
+  return used;
+}
+
+AE_DEVICE void ae_pack_tables(const AePlanCompactionArgs& a, const AeListState& st, const AeListShare sh, int used) {
+  for (AeEntries e(sh, a.B, a.max_pages); e.more();) {
     int page[AE_LIST_BATCH], place[AE_LIST_BATCH];
+    const u32 i0 = e.i;
 #pragma unroll
     for (int j = 0; j < AE_LIST_BATCH; ++j) {
       page[j] = 0;
-      const int i = i0 + j * warps;
-      if (i >= B * chunks) continue;
-      const int r = i / chunks, c = (i - r * chunks) * 32 + lane;
-      if (c < W && ((i64)c << a.page_log2) < tokens_of(a.lens[r])) page[j] = a.table[(i64)r * a.table_stride + c];
+      if (e.more() && (i64)e.c << a.page_log2 < ae_len(a, e.r)) page[j] = a.table[(i64)e.r * a.table_stride + e.c];
+      e.next(sh.step());
     }
 #pragma unroll
-    for (int j = 0; j < AE_LIST_BATCH; ++j) place[j] = page[j] >= used && page[j] < a.num_pages ? (int)__ldcg(a.state + page[j]) : -1;
+    for (int j = 0; j < AE_LIST_BATCH; ++j) place[j] = page[j] >= used && page[j] < a.num_pages ? (int)ae_word(st.owner + page[j]) : -1;
 #pragma unroll
     for (int j = 0; j < AE_LIST_BATCH; ++j)
-      if (place[j] >= 0) page[j] = __ldcg(&a.copies[place[j]].dst);
+      if (place[j] >= 0) page[j] = st.holes ? st.holes[place[j]] : __ldcg(&a.copies[place[j]].dst);
 #pragma unroll
-    for (int j = 0; j < AE_LIST_BATCH; ++j) {
-      const int i = i0 + j * warps;
-      if (i >= B * chunks) break;
-      const int r = i / chunks, c = (i - r * chunks) * 32 + lane;
-      if (c < W) a.table_out[(i64)r * W + c] = page[j];
-    }
+    for (int j = 0; j < AE_LIST_BATCH; ++j)
+      if (i0 + j * sh.step() < e.total) a.table_out[i0 + j * sh.step()] = page[j];
   }
+}
+
+extern "C" __global__ void __launch_bounds__(AE_LIST_THREADS) ae_plan_compaction(const __grid_constant__ AePlanCompactionArgs a) {
+  const AeListShare sh = {(int)blockIdx.x, (int)gridDim.x};
+  AeListState st;
+  st.rows = nullptr;
+#if AE_PHASE == 0
+  extern __shared__ uint4 smem_raw[];
+  st.held = (u32*)smem_raw;
+#else
+  st.held = a.held;
+#endif
+  st.whole = st.held;
+  st.begun = st.whole + a.words;
+  st.owner = st.begun + a.words;
+  st.holes = AE_PHASE == 0 ? (int*)(st.owner + a.num_pages) : nullptr;
+  ae_grid_wait();  // brought up under the kernel in front
+  ae_grid_trigger();
+#if AE_PHASE == 0
+  ae_pack_rows(a, st, sh);
+  __syncthreads();
+  ae_pack_marks(a, st, sh);
+  __syncthreads();
+  const int used = ae_pack_lists(a, st, sh);
+  __syncthreads();
+  ae_pack_tables(a, st, sh, used);
+#elif AE_PHASE == 1
+  ae_pack_rows(a, st, sh);
+#elif AE_PHASE == 2
+  ae_pack_marks(a, st, sh);
+#elif AE_PHASE == 3
+  ae_pack_lists(a, st, sh);
+#else
+  ae_pack_tables(a, st, sh, __ldcg(a.head_out));
+#endif
 }

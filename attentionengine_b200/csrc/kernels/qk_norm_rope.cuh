@@ -9,15 +9,21 @@
 // position, where an fp32 angle is off by 0.03 at position 500000.
 //
 // A team of D / 16 threads has a head, each thread 16 values that hold both halves of its 8 pairs, so that the rotation needs no exchange and the norm
-// log2(D / 16) shuffles.  A warp has a token and a share of its heads: cosines and sines are made once for them (two pairs a lane, through shared
-// memory) and folded with the weights into four factors a pair.  Bound by HBM for long calls: everything is read and written once.
-// Expects AE_D (32, 64, 128 or 256), AE_R (rotary dims, a multiple of 16), AE_NORM, AE_NEXT (pairs of neighbours), AE_ROPE_WARPS, AE_ROPE_U (heads
-// of a team on their way together), AE_ROPE_KERNEL (0 forward, 1 backward, 2 the weights' sums).
+// log2(D / 16) shuffles.  A warp has a token, or where tokens are few a share of its heads: its lanes make the token's cosines and sines once and fold
+// them (forward: with the weights) into two factors a value, which pass through shared memory.  Arithmetic on two fp32 values an instruction.
+//
+// Bound by HBM for long calls: everything is read and written once.  What that takes is bytes on their way, and a warp has four chains of reads in a row
+// (position, two batches of queries, keys): the forward asks L2 for a token's heads before anything else.  In a graph, 40 heads of 128 dims, bf16: 16029 tokens (236 MB) 39.3 us,
+// 6.0 TB/s (42.9 without that request; 44 to 45 with the factors made by every team for itself; 79 with factors at 64-byte steps, four-fold bank conflicts;
+// 84 with whole CTAs a token, whose barriers leave nothing on its way); forward and backward of 16384 tokens (839 MB) 154 us.  64 tokens, one a request: 2.6.
+// The backward is joined work of 24 warps an SM with one head a team on its way (80 registers): 97 us, 5.2 TB/s; a ring of copies through shared memory, two heads on their
+// way, or requests to L2 ahead took 1 to 30 % more.
+// Expects AE_D (32, 64, 128 or 256), AE_R (rotary dims, a multiple of 16), AE_NORM, AE_NEXT (pairs of neighbours), AE_ROPE_WARPS, AE_ROPE_U (backward: heads
+// of a team on their way together), AE_ROPE_CTAS (of an SM), AE_ROPE_KERNEL (0 forward, 1 backward, 2 the weights' sums).
+#define AE_ROPE_THREADS (32 * AE_ROPE_WARPS)
 #define AE_TPR (AE_D / 16)      // threads of a team
 #define AE_TEAMS (32 / AE_TPR)  // teams of a warp
-#define AE_ROPE_THREADS (32 * AE_ROPE_WARPS)
 #define AE_PAIRS (AE_R / 2)
-#define AE_PAIRS1 (AE_PAIRS > 0 ? AE_PAIRS : 1)
 
 // cos and sin of the turns that position p makes.
 AE_DEVICE float2 ae_turn(u64 per_position, i64 p) {
@@ -35,191 +41,231 @@ AE_DEVICE int ae_chunk(int t, int second) {
   return t < AE_R / 16 ? 8 * t + second * (AE_R / 2) : AE_R + 16 * (t - AE_R / 16) + 8 * second;
 #endif
 }
-// Where of a thread's 16 values pair e has its first and second.
-AE_DEVICE constexpr int ae_first(int e) { return AE_NEXT ? 2 * e : e; }
-AE_DEVICE constexpr int ae_second(int e) { return AE_NEXT ? 2 * e + 1 : e + 8; }
+// Two fp32 values in a register pair.
+AE_DEVICE u64 ae_mul2(u64 a, u64 b) {
+  u64 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+AE_DEVICE u64 ae_fma22(u64 a, u64 b, u64 c) {
+  u64 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+AE_DEVICE float ae_sum2(u64 a) {
+  float lo, hi;
+  ae_unpack2f(a, lo, hi);
+  return lo + hi;
+}
 
+// A thread's 16 values as 8 pairs of neighbours.
 template <int BF16>
-AE_DEVICE void ae_unpack16(const uint4 (&v)[2], float (&x)[16]) {
+AE_DEVICE void ae_unpack16(const uint4& lo, const uint4& hi, u64 (&x)[8]) {
+  const u32 u[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const u32 u[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+  for (int k = 0; k < 8; ++k) x[k] = ae_pack2f(unpack_lo<BF16>(u[k]), unpack_hi<BF16>(u[k]));
+}
+template <int BF16>
+AE_DEVICE uint4 ae_pack8(const u64* x) {
+  u32 r[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      x[8 * c + 2 * k] = unpack_lo<BF16>(u[k]);
-      x[8 * c + 2 * k + 1] = unpack_hi<BF16>(u[k]);
-    }
+  for (int k = 0; k < 4; ++k) {
+    float lo, hi;
+    ae_unpack2f(x[k], lo, hi);
+    r[k] = pack2<BF16>(lo, hi);
   }
+  return make_uint4(r[0], r[1], r[2], r[3]);
 }
-template <int BF16>
-AE_DEVICE uint4 ae_pack8(const float* x) {
-  return make_uint4(pack2<BF16>(x[0], x[1]), pack2<BF16>(x[2], x[3]), pack2<BF16>(x[4], x[5]), pack2<BF16>(x[6], x[7]));
+// What the rotation mixes with pair k: the values of the other half, or the same two the other way round.
+AE_DEVICE u64 ae_partner(const u64 (&x)[8], int k) {
+#if AE_NEXT
+  float lo, hi;
+  ae_unpack2f(x[k], lo, hi);
+  return ae_pack2f(hi, lo);
+#else
+  return x[k ^ 4];
+#endif
 }
-
 AE_DEVICE float ae_team_sum(float x) {
 #pragma unroll
   for (int o = 1; o < AE_TPR; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
   return x;
 }
 
-// The weights of a thread's 16 values.
-AE_DEVICE void ae_load_weights(const AeQkRopeArgs& a, int kind, int t, float (&w)[16]) {
-#pragma unroll
-  for (int j = 0; j < 16; ++j) w[j] = 1.f;
-  if (!a.w[kind]) return;
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int at = ae_chunk(t, c);
-    if (a.w32) {
-      const float4* const p = (const float4*)((const float*)a.w[kind] + at);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float4 u = p[j];
-        w[8 * c + 4 * j] = u.x;
-        w[8 * c + 4 * j + 1] = u.y;
-        w[8 * c + 4 * j + 2] = u.z;
-        w[8 * c + 4 * j + 3] = u.w;
-      }
-    } else {
-      const uint4 v = *(const uint4*)((const u16*)a.w[kind] + at);
-      const u32 u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        w[8 * c + 2 * j] = a.bf16 ? unpack_lo<1>(u[j]) : unpack_lo<0>(u[j]);
-        w[8 * c + 2 * j + 1] = a.bf16 ? unpack_hi<1>(u[j]) : unpack_hi<0>(u[j]);
-      }
-    }
-  }
-}
+#if AE_ROPE_KERNEL < 2
 
+#define AE_KINDS (AE_ROPE_KERNEL == 0 ? 2 : 1)
+// Factors of each value and of its partner, as the threads read them (ae_place).
 struct AeRopeSmem {
-  u64 turns[AE_PAIRS1];
-  float2 cs[AE_ROPE_WARPS][AE_PAIRS1];
+  float f[AE_ROPE_WARPS][AE_KINDS][2][AE_D];
+  float w[AE_KINDS][AE_D];  // weights, in that order too
+  u64 turns[AE_PAIRS];
 #if AE_ROPE_KERNEL == 1 && AE_NORM
   float dw[AE_ROPE_WARPS][AE_D];
 #endif
 };
 
-AE_DEVICE i64 ae_position(const AeQkRopeArgs& a, int b, int s) {
-  const i64 at = b * a.pos_st[0] + s * a.pos_st[1];
-  return a.pos64 ? ((const i64*)a.pos)[at] : (i64)((const int*)a.pos)[at];
+// Place of dim d among the threads' values (ae_chunk the other way round): four values of every thread behind each other, so that a warp's wide loads
+// meet every bank once.
+AE_DEVICE int ae_place(int d) {
+#if AE_NEXT
+  const int t = d >> 4, j = d & 15;
+#else
+  const int second = d >= AE_R / 2, i = d - second * (AE_R / 2);
+  const int t = d < AE_R ? i >> 3 : d >> 4, j = d < AE_R ? 8 * second + (i & 7) : d & 15;
+#endif
+  return ((j >> 2) * AE_TPR + t) * 4 + (j & 3);
 }
 
-// cos and sin times m of a thread's pairs, made by the warp together.
-AE_DEVICE void ae_cos_sin(const AeQkRopeArgs& a, AeRopeSmem& sm, i64 p, int t, float (&c)[8], float (&s)[8]) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __syncwarp();  // the pairs of the item in front have been read
-#pragma unroll
-  for (int i = 0; i < (AE_PAIRS + 31) / 32; ++i)
-    if (i * 32 + lane < AE_PAIRS) {
-      const float2 r = ae_turn(sm.turns[i * 32 + lane], p);
-      sm.cs[warp][i * 32 + lane] = make_float2(r.x * a.scale, r.y * a.scale);
-    }
-  __syncwarp();
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float2 r = make_float2(1.f, 0.f);
-    if (t < AE_R / 16) r = sm.cs[warp][8 * t + e];
-    c[e] = r.x;
-    s[e] = r.y;
+AE_DEVICE float ae_weight(const AeQkRopeArgs& a, int kind, int d) {
+  if (!a.w[kind]) return 1.f;
+  if (a.w32) return ((const float*)a.w[kind])[d];
+  const u32 u = ((const u16*)a.w[kind])[d];
+  return a.bf16 ? unpack_lo<1>(u) : unpack_lo<0>(u);
+}
+
+struct AeRopeToken {
+  int b, s;
+  AE_DEVICE AeRopeToken(const AeQkRopeArgs& a, int token) : b(0), s(token) {
+    if (a.S < a.T) b = token / a.S, s = token - b * a.S;
   }
+  AE_DEVICE i64 position(const AeQkRopeArgs& a) const {
+    const i64 at = b * a.pos_st[0] + s * a.pos_st[1];
+    return a.pos64 ? ((const i64*)a.pos)[at] : (i64)((const int*)a.pos)[at];
+  }
+  AE_DEVICE const u16* heads(const void* x, const i64 (&st)[3]) const { return (const u16*)x + b * st[0] + s * st[1]; }
+};
+
+// Thread t's 16 values.
+AE_DEVICE void ae_read8(const float* f, int t, u64 (&x)[8]) {
+  const u32 at = smem_u32(f) + 16 * t;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(x[2 * i]), "=l"(x[2 * i + 1]) : "r"(at + 16 * AE_TPR * i) : "memory");
 }
 
-AE_DEVICE void ae_load_turns(const AeQkRopeArgs& a, AeRopeSmem& sm) {
-  for (int i = threadIdx.x; i < AE_PAIRS; i += AE_ROPE_THREADS) sm.turns[i] = a.turns[i];
-  __syncthreads();
-}
-
+#endif
 #if AE_ROPE_KERNEL == 0
 
-// Heads h0 ... h1 - 1 of a token, by a warp.
-template <int BF16>
-AE_DEVICE void ae_rope_heads(const AeQkRopeArgs& a, AeRopeSmem& sm, int kind, int token, int h0, int h1) {
-  const int lane = threadIdx.x & 31, t = lane % AE_TPR, team = lane / AE_TPR;
-  const int b = token / a.S, s = token - b * a.S;
-  const u16* const x = (const u16*)a.x[kind] + b * a.x_st[kind][0] + s * a.x_st[kind][1];
-  u16* const y = (u16*)a.y[kind] + (i64)token * a.H[kind] * AE_D;
-  const int at[2] = {ae_chunk(t, 0), ae_chunk(t, 1)};
-  const i64 p = ae_position(a, b, s);
-  if (p < 0) {  // no token
-    for (int h = h0 + team; h < h1; h += AE_TEAMS)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) *(uint4*)(y + h * AE_D + at[c]) = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  uint4 v[AE_ROPE_U][2];
-  auto load = [&](int base) {
-#pragma unroll
-    for (int u = 0; u < AE_ROPE_U; ++u) {
-      const int h = base + u * AE_TEAMS + team;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        v[u][c] = make_uint4(0, 0, 0, 0);
-        if (h < h1) v[u][c] = *(const uint4*)(x + h * a.x_st[kind][2] + at[c]);
-      }
-    }
-  };
-  load(h0);
-  // y_a = rstd (x_a fa[0] - x_b fb[0]), y_b = rstd (x_b fb[1] + x_a fa[1])
-  float fa[2][8], fb[2][8];
-  {
-    float c[8], sn[8], w[16];
-    ae_cos_sin(a, sm, p, t, c, sn);
-    ae_load_weights(a, kind, t, w);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      fa[0][e] = c[e] * w[ae_first(e)];
-      fa[1][e] = sn[e] * w[ae_first(e)];
-      fb[0][e] = sn[e] * w[ae_second(e)];
-      fb[1][e] = c[e] * w[ae_second(e)];
-    }
-  }
-  for (int base = h0;;) {
-#pragma unroll
-    for (int u = 0; u < AE_ROPE_U; ++u) {
-      float f[16], o[16];
-      ae_unpack16<BF16>(v[u], f);
-      float r = 1.f;
-#if AE_NORM
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) sum = fmaf(f[j], f[j], sum);
-      r = rsqrtf(fmaf(ae_team_sum(sum), 1.f / AE_D, a.eps));
-#endif
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float xa = f[ae_first(e)], xb = f[ae_second(e)];
-        o[ae_first(e)] = r * fmaf(xa, fa[0][e], -(xb * fb[0][e]));
-        o[ae_second(e)] = r * fmaf(xb, fb[1][e], xa * fa[1][e]);
-      }
-      const int h = base + u * AE_TEAMS + team;
-      if (h < h1)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) *(uint4*)(y + h * AE_D + at[c]) = ae_pack8<BF16>(o + 8 * c);
-    }
-    base += AE_ROPE_U * AE_TEAMS;
-    if (base >= h1) break;
-    load(base);
+// n heads on their way into L2, by a warp: what registers have no room for yet.
+AE_DEVICE void ae_prefetch_heads(const u16* x, i64 st, int n) {
+  const int lane = threadIdx.x & 31;
+  if (st == AE_D) {
+    if (lane == 0 && n > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(x), "r"(n * AE_D * 2) : "memory");
+  } else {
+    for (int h = lane; h < n; h += 32) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(x + h * st), "r"(AE_D * 2) : "memory");
   }
 }
 
-extern "C" __global__ void __launch_bounds__(AE_ROPE_THREADS) ae_qk_rope_fwd(const __grid_constant__ AeQkRopeArgs a) {
-  __shared__ AeRopeSmem sm;
-  ae_load_turns(a, sm);
+// U heads of each team from h on: y = x f0 + partner(x) f1 times the norm's factor; f1 holds the partner's weight.
+template <int BF16, int U>
+AE_DEVICE void ae_rope_batch(const AeQkRopeArgs& a, const u64 (&f)[2][8], const u16* x, u16* y, i64 st, const int (&at)[2], int h, int end) {
+  uint4 v[U][2];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    v[u][0] = v[u][1] = make_uint4(0, 0, 0, 0);
+    if (h + u * AE_TEAMS < end)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) v[u][c] = *(const uint4*)(x + (h + u * AE_TEAMS) * st + at[c]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    u64 z[8], o[8];
+    ae_unpack16<BF16>(v[u][0], v[u][1], z);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] = ae_fma22(z[k], f[0][k], ae_mul2(ae_partner(z, k), f[1][k]));
+#if AE_NORM
+    u64 sum = ae_mul2(z[0], z[0]);
+#pragma unroll
+    for (int k = 1; k < 8; ++k) sum = ae_fma22(z[k], z[k], sum);
+    const float r = rsqrtf(fmaf(ae_team_sum(ae_sum2(sum)), 1.f / AE_D, a.eps));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] = ae_mul2(o[k], ae_pack2f(r, r));
+#endif
+    if (h + u * AE_TEAMS < end)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) __stcs((uint4*)(y + (h + u * AE_TEAMS) * AE_D + at[c]), ae_pack8<BF16>(o + 4 * c));
+  }
+}
+
+// Heads h0 ... h1 - 1 of a token, queries or keys, by a warp.
+template <int BF16>
+AE_DEVICE void ae_rope_heads(const AeQkRopeArgs& a, const AeRopeSmem& sm, bool none, int kind, int token, const AeRopeToken& at_token, int h0, int h1) {
+  const int lane = threadIdx.x & 31, t = lane % AE_TPR, team = lane / AE_TPR;
+  u16* const y = (u16*)a.y[kind] + (i64)token * a.H[kind] * AE_D;
+  if (none) {
+    for (int i = h0 * (AE_D / 8) + lane; i < h1 * (AE_D / 8); i += 32) ((uint4*)y)[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const u16* const x = at_token.heads(a.x[kind], a.x_st[kind]);
+  const i64 st = a.x_st[kind][2];
+  const int at[2] = {ae_chunk(t, 0), ae_chunk(t, 1)};
+  u64 f[2][8];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) ae_read8(sm.f[threadIdx.x >> 5][kind][i], t, f[i]);
+#pragma unroll 1
+  for (; h0 + 2 * AE_TEAMS < h1; h0 += 4 * AE_TEAMS) ae_rope_batch<BF16, 4>(a, f, x, y, st, at, h0 + team, h1);
+  if (h0 + AE_TEAMS < h1)
+    ae_rope_batch<BF16, 2>(a, f, x, y, st, at, h0 + team, h1);
+  else if (h0 < h1)
+    ae_rope_batch<BF16, 1>(a, f, x, y, st, at, h0 + team, h1);
+}
+
+template <int BF16>
+AE_DEVICE void ae_rope_fwd(const AeQkRopeArgs& a, AeRopeSmem& sm) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int item = blockIdx.x * AE_ROPE_WARPS + warp, token = a.slices[0] == 1 ? item : item / a.slices[0];
+  // heads of queries, then keys, as one line
+  const int c0 = (item - token * a.slices[0]) * a.per, c1 = min(c0 + a.per, a.H[0] + a.H[1]);
+  const int q1 = min(c1, a.H[0]), k0 = max(c0 - a.H[0], 0), k1 = c1 - a.H[0];
+  const AeRopeToken at(a, token);
+  i64 p = -1;
+  if (token < a.T) {
+    p = at.position(a);
+    if (a.prefetch) {
+      ae_prefetch_heads(at.heads(a.x[0], a.x_st[0]) + c0 * a.x_st[0][2], a.x_st[0][2], q1 - c0);
+      if (k1 > 0) ae_prefetch_heads(at.heads(a.x[1], a.x_st[1]) + k0 * a.x_st[1][2], a.x_st[1][2], k1 - k0);
+    }
+  }
+  for (int i = threadIdx.x; i < 2 * AE_D; i += AE_ROPE_THREADS) {
+    const int kind = i / AE_D, d = i % AE_D, place = ae_place(d);
+    const float w = ae_weight(a, kind, d);
+    sm.w[kind][place] = w;
+    if (d >= AE_R)
+#pragma unroll
+      for (int k = 0; k < AE_ROPE_WARPS; ++k) sm.f[k][kind][0][place] = w, sm.f[k][kind][1][place] = 0.f;
+  }
+  __syncthreads();
+  if (token >= a.T) return;
+#pragma unroll
+  for (int e = lane; e < AE_PAIRS; e += 32) {
+    const float2 r = ae_turn(sm.turns[e], p);
+    const float c = r.x * a.scale, s = r.y * a.scale;
+    const int pa = ae_place(AE_NEXT ? 2 * e : e), pb = ae_place(AE_NEXT ? 2 * e + 1 : e + AE_R / 2);
+#pragma unroll
+    for (int kind = 0; kind < 2; ++kind) {
+      const float wa = sm.w[kind][pa], wb = sm.w[kind][pb];
+      float(&f)[2][AE_D] = sm.f[warp][kind];
+      f[0][pa] = c * wa;
+      f[1][pa] = -s * wb;
+      f[0][pb] = c * wb;
+      f[1][pb] = s * wa;
+    }
+  }
+  __syncwarp();
+  if (c0 < q1) ae_rope_heads<BF16>(a, sm, p < 0, 0, token, at, c0, q1);
+  if (k0 < k1) ae_rope_heads<BF16>(a, sm, p < 0, 1, token, at, k0, k1);
+}
+
+extern "C" __global__ void __launch_bounds__(AE_ROPE_THREADS, AE_ROPE_CTAS) ae_qk_rope_fwd(const __grid_constant__ AeQkRopeArgs a) {
+  __shared__ __align__(16) AeRopeSmem sm;
+  for (int i = threadIdx.x; i < AE_PAIRS; i += AE_ROPE_THREADS) sm.turns[i] = a.turns[i];
   ae_grid_wait();  // brought up under the kernel in front
   ae_grid_trigger();
-  const int slices = a.slices[0] + a.slices[1];
-  const int item = blockIdx.x * AE_ROPE_WARPS + (threadIdx.x >> 5);
-  const int token = item / slices;
-  if (token >= a.T) return;
-  int slice = item - token * slices;
-  const int kind = slice >= a.slices[0];
-  if (kind) slice -= a.slices[0];
-  const int h0 = slice * a.per, h1 = min(h0 + a.per, a.H[kind]);
   if (a.bf16)
-    ae_rope_heads<1>(a, sm, kind, token, h0, h1);
+    ae_rope_fwd<1>(a, sm);
   else
-    ae_rope_heads<0>(a, sm, kind, token, h0, h1);
+    ae_rope_fwd<0>(a, sm);
 }
 
 #elif AE_ROPE_KERNEL == 1
@@ -227,95 +273,110 @@ extern "C" __global__ void __launch_bounds__(AE_ROPE_THREADS) ae_qk_rope_fwd(con
 // A CTA works on queries alone or keys alone, so that its threads keep one set of weight sums.  They are joined in a fixed order: teams, warps,
 // and by ae_qk_rope_dw CTAs; results do not vary.
 template <int BF16>
-AE_DEVICE void ae_rope_bwd_heads(const AeQkRopeArgs& a, AeRopeSmem& sm, int kind, const float (&w)[16], float (&dw)[16], int token, int h0, int h1) {
-  const int lane = threadIdx.x & 31, t = lane % AE_TPR, team = lane / AE_TPR;
-  const int b = token / a.S, s = token - b * a.S;
-  const u16* const x = (const u16*)a.x[kind] + b * a.x_st[kind][0] + s * a.x_st[kind][1];
-  const u16* const g = (const u16*)a.g[kind] + b * a.g_st[kind][0] + s * a.g_st[kind][1];
-  u16* const y = (u16*)a.y[kind] + (i64)token * a.H[kind] * AE_D;
+AE_DEVICE void ae_rope_bwd(const AeQkRopeArgs& a, AeRopeSmem& sm) {
+  const int kind = (int)blockIdx.x >= a.ctas[0], cta = (int)blockIdx.x - kind * a.ctas[0], H = a.H[kind], slices = a.slices[kind], per = a.per;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = lane % AE_TPR, team = lane / AE_TPR;
   const int at[2] = {ae_chunk(t, 0), ae_chunk(t, 1)};
-  const i64 p = ae_position(a, b, s);
-  if (p < 0) {
-    for (int h = h0 + team; h < h1; h += AE_TEAMS)
+  const i64 x_st = a.x_st[kind][2], g_st = a.g_st[kind][2];
+  for (int d = threadIdx.x; d < AE_D; d += AE_ROPE_THREADS) {
+    const int place = ae_place(d);
+    sm.w[0][place] = ae_weight(a, kind, d);
+    if (d >= AE_R)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) *(uint4*)(y + h * AE_D + at[c]) = make_uint4(0, 0, 0, 0);
-    return;
+      for (int k = 0; k < AE_ROPE_WARPS; ++k) sm.f[k][0][0][place] = 1.f, sm.f[k][0][1][place] = 0.f;
   }
-  uint4 v[AE_ROPE_U][2], gv[AE_ROPE_U][2];
-  auto load = [&](int base) {
+  __syncthreads();
+  u64 dw2[8];
 #pragma unroll
-    for (int u = 0; u < AE_ROPE_U; ++u) {
-      const int h = base + u * AE_TEAMS + team;
+  for (int j = 0; j < 8; ++j) dw2[j] = 0;
+  float(&f)[2][AE_D] = sm.f[warp][0];
+  const int items = a.T * slices, step = a.ctas[kind] * AE_ROPE_WARPS;
+#pragma unroll 1
+  for (int item = cta * AE_ROPE_WARPS + warp; item < items; item += step) {
+    const int token = slices == 1 ? item : item / slices, h0 = (item - token * slices) * per, h1 = min(h0 + per, H);
+    const AeRopeToken here(a, token);
+    const i64 p = here.position(a);
+    const u16* const g = here.heads(a.g[kind], a.g_st[kind]);
+    const u16* const x = AE_NORM ? here.heads(a.x[kind], a.x_st[kind]) : g;
+    u16* const y = (u16*)a.y[kind] + (i64)token * H * AE_D;
+    uint4 v[AE_ROPE_U][2], gv[AE_ROPE_U][2];
+    auto load = [&](int h) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        v[u][c] = gv[u][c] = make_uint4(0, 0, 0, 0);
-        if (h < h1) {
-#if AE_NORM
-          v[u][c] = *(const uint4*)(x + h * a.x_st[kind][2] + at[c]);
-#endif
-          gv[u][c] = *(const uint4*)(g + h * a.g_st[kind][2] + at[c]);
+      for (int u = 0; u < AE_ROPE_U; ++u) {
+        v[u][0] = v[u][1] = gv[u][0] = gv[u][1] = make_uint4(0, 0, 0, 0);
+        if (h + u * AE_TEAMS < h1) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            gv[u][c] = *(const uint4*)(g + (h + u * AE_TEAMS) * g_st + at[c]);
+            if (AE_NORM) v[u][c] = *(const uint4*)(x + (h + u * AE_TEAMS) * x_st + at[c]);
+          }
         }
       }
+    };
+    load(h0 + team);
+    if (p < 0) {  // no token
+      for (int i = h0 * (AE_D / 8) + lane; i < h1 * (AE_D / 8); i += 32) ((uint4*)y)[i] = make_uint4(0, 0, 0, 0);
+      continue;
     }
-  };
-  load(h0);
-  float c[8], sn[8];
-  ae_cos_sin(a, sm, p, t, c, sn);
-  for (int base = h0;;) {
+    __syncwarp();  // the factors of the token in front have been read
 #pragma unroll
-    for (int u = 0; u < AE_ROPE_U; ++u) {
-      float gf[16], dz[16];
-      ae_unpack16<BF16>(gv[u], gf);
+    for (int i = lane; i < AE_PAIRS; i += 32) {  // dz = g f0 + partner(g) f1
+      const float2 r = ae_turn(sm.turns[i], p);
+      const float c = r.x * a.scale, s = r.y * a.scale;
+      const int pa = ae_place(AE_NEXT ? 2 * i : i), pb = ae_place(AE_NEXT ? 2 * i + 1 : i + AE_R / 2);
+      f[0][pa] = f[0][pb] = c;
+      f[1][pa] = s;
+      f[1][pb] = -s;
+    }
+    __syncwarp();
+#pragma unroll 1
+    for (int base = h0;;) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float ga = gf[ae_first(e)], gb = gf[ae_second(e)];
-        dz[ae_first(e)] = fmaf(ga, c[e], gb * sn[e]);
-        dz[ae_second(e)] = fmaf(gb, c[e], -(ga * sn[e]));
-      }
+      for (int u = 0; u < AE_ROPE_U; ++u) {
+        const int h = base + u * AE_TEAMS + team;
+        u64 g2[8], dz[8], k2[8];
+        ae_unpack16<BF16>(gv[u][0], gv[u][1], g2);
+        ae_read8(f[1], t, k2);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) dz[k] = ae_mul2(ae_partner(g2, k), k2[k]);
+        ae_read8(f[0], t, k2);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) dz[k] = ae_fma22(g2[k], k2[k], dz[k]);
 #if AE_NORM
-      float f[16], sum = 0.f, dot = 0.f;  // of x^2, of x dz w
-      ae_unpack16<BF16>(v[u], f);
+        u64 z[8];
+        ae_unpack16<BF16>(v[u][0], v[u][1], z);
+        u64 sum = ae_mul2(z[0], z[0]);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) sum = fmaf(f[j], f[j], sum);
-      float r = rsqrtf(fmaf(ae_team_sum(sum), 1.f / AE_D, a.eps));
-      if (base + u * AE_TEAMS + team >= h1) r = 0.f;  // no head: with eps = 0 its zeros would make the sums NaN
+        for (int k = 1; k < 8; ++k) sum = ae_fma22(z[k], z[k], sum);
+        float r = rsqrtf(fmaf(ae_team_sum(ae_sum2(sum)), 1.f / AE_D, a.eps));
+        if (h >= h1) r = 0.f;  // no head: with eps = 0 its zeros would make the sums NaN
+        u64 dot = 0;  // of (dz r w) x: sum of dn n
+        ae_read8(sm.w[0], t, k2);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        f[j] *= r;  // n
-        dw[j] = fmaf(dz[j], f[j], dw[j]);
-        dz[j] *= w[j];
-        dot = fmaf(dz[j], f[j], dot);
-      }
-      const float mean = ae_team_sum(dot) * (1.f / AE_D);
+        for (int k = 0; k < 8; ++k) {
+          dz[k] = ae_mul2(dz[k], ae_pack2f(r, r));
+          dw2[k] = ae_fma22(dz[k], z[k], dw2[k]);
+          dz[k] = ae_mul2(dz[k], k2[k]);
+          dot = ae_fma22(dz[k], z[k], dot);
+        }
+        const float mean = -r * r * ae_team_sum(ae_sum2(dot)) * (1.f / AE_D);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) dz[j] = r * fmaf(-f[j], mean, dz[j]);
+        for (int k = 0; k < 8; ++k) dz[k] = ae_fma22(z[k], ae_pack2f(mean, mean), dz[k]);
 #endif
-      const int h = base + u * AE_TEAMS + team;
-      if (h < h1)
+        if (h < h1)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) *(uint4*)(y + h * AE_D + at[k]) = ae_pack8<BF16>(dz + 8 * k);
+          for (int c = 0; c < 2; ++c) __stcs((uint4*)(y + h * AE_D + at[c]), ae_pack8<BF16>(dz + 4 * c));
+      }
+      base += AE_ROPE_U * AE_TEAMS;
+      if (base >= h1) break;
+      load(base + team);
     }
-    base += AE_ROPE_U * AE_TEAMS;
-    if (base >= h1) break;
-    load(base);
-  }
-}
-
-template <int BF16>
-AE_DEVICE void ae_rope_bwd(const AeQkRopeArgs& a, AeRopeSmem& sm) {
-  const int kind = (int)blockIdx.x >= a.ctas[0], cta = (int)blockIdx.x - kind * a.ctas[0];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = lane % AE_TPR;
-  float w[16], dw[16];
-  ae_load_weights(a, kind, t, w);
-#pragma unroll
-  for (int j = 0; j < 16; ++j) dw[j] = 0.f;
-  const i64 items = (i64)a.T * a.slices[kind];
-  for (i64 item = (i64)cta * AE_ROPE_WARPS + warp; item < items; item += (i64)a.ctas[kind] * AE_ROPE_WARPS) {
-    const int token = (int)(item / a.slices[kind]), h0 = (int)(item - (i64)token * a.slices[kind]) * a.per;
-    ae_rope_bwd_heads<BF16>(a, sm, kind, w, dw, token, h0, min(h0 + a.per, a.H[kind]));
   }
 #if AE_NORM
   if (!a.dw_part) return;
+  float dw[16];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ae_unpack2f(dw2[j], dw[2 * j], dw[2 * j + 1]);
 #pragma unroll
   for (int j = 0; j < 16; ++j)
 #pragma unroll
@@ -334,8 +395,8 @@ AE_DEVICE void ae_rope_bwd(const AeQkRopeArgs& a, AeRopeSmem& sm) {
 }
 
 extern "C" __global__ void __launch_bounds__(AE_ROPE_THREADS, AE_ROPE_CTAS) ae_qk_rope_bwd(const __grid_constant__ AeQkRopeArgs a) {
-  __shared__ AeRopeSmem sm;
-  ae_load_turns(a, sm);
+  __shared__ __align__(16) AeRopeSmem sm;
+  for (int i = threadIdx.x; i < AE_PAIRS; i += AE_ROPE_THREADS) sm.turns[i] = a.turns[i];
   ae_grid_wait();
   ae_grid_trigger();
   if (a.bf16)
@@ -348,20 +409,20 @@ extern "C" __global__ void __launch_bounds__(AE_ROPE_THREADS, AE_ROPE_CTAS) ae_q
 
 // The weights' gradients: a CTA sums 32 dims of the CTAs' rows, for queries or keys.
 extern "C" __global__ void __launch_bounds__(AE_ROPE_THREADS) ae_qk_rope_dw(const __grid_constant__ AeQkRopeArgs a) {
-  __shared__ float sm[AE_ROPE_WARPS][32];
+  __shared__ float sm[AE_ROPE_THREADS / 32][32];
   ae_grid_wait();
   ae_grid_trigger();
   const int kind = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = blockIdx.x * 32 + lane;
   const float* const part = a.dw_part + (i64)(kind ? a.ctas[0] : 0) * AE_D + d;
   float sum = 0.f;
 #pragma unroll 8
-  for (int i = warp; i < a.ctas[kind]; i += AE_ROPE_WARPS) sum += part[(i64)i * AE_D];
+  for (int i = warp; i < a.ctas[kind]; i += AE_ROPE_THREADS / 32) sum += part[(i64)i * AE_D];
   sm[warp][lane] = sum;
   __syncthreads();
   if (warp == 0) {
     sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < AE_ROPE_WARPS; ++i) sum += sm[i][lane];
+    for (int i = 0; i < AE_ROPE_THREADS / 32; ++i) sum += sm[i][lane];
     if (a.w32)
       ((float*)a.dw[kind])[d] = sum;
     else

@@ -203,7 +203,7 @@ EXPORTS = ["ae_compile", "ae_module_from_cubin", "ae_module_cubin", "ae_query", 
            "ae_launch_linear_segments", "ae_launch_attn_packed", "ae_launch_plan_pages", "ae_launch_cache8_write",
            "ae_launch_cache8_decode", "ae_cache8_decode_workspace",
            "ae_cache8_decode_merges", "ae_launch_cache8_merge", "ae_launch_plan_forks", "ae_launch_plan_compaction", "ae_launch_copy_pages",
-           "ae_plan_lists_workspace", "ae_launch_qk_rope", "ae_qk_rope_workspace"]
+           "ae_plan_lists_workspace", "ae_plan_lists_phases", "ae_launch_qk_rope", "ae_qk_rope_workspace"]
 
 
 def lib() -> C.CDLL:
@@ -251,7 +251,8 @@ def lib() -> C.CDLL:
             L.ae_launch_plan_forks.argtypes = [C.c_void_p, C.POINTER(PlanForksParams), C.c_void_p]
             L.ae_launch_plan_compaction.argtypes = [C.c_void_p, C.POINTER(PlanCompactionParams), C.c_void_p]
             L.ae_launch_copy_pages.argtypes = [C.c_void_p, C.POINTER(CopyPagesParams), C.c_void_p]
-            L.ae_plan_lists_workspace.argtypes, L.ae_plan_lists_workspace.restype = [C.c_int32], C.c_int64
+            L.ae_plan_lists_workspace.argtypes, L.ae_plan_lists_workspace.restype = [C.c_int32] * 2, C.c_int64
+            L.ae_plan_lists_phases.argtypes = [C.c_int32] * 3
             L.ae_launch_qk_rope.argtypes = [C.c_void_p, C.POINTER(QkRopeParams), C.c_void_p]
             L.ae_qk_rope_workspace.argtypes, L.ae_qk_rope_workspace.restype = [C.c_void_p], C.c_int64
             L.ae_launch_probe.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,

@@ -239,7 +239,9 @@ int ae_launch_cache8_decode(void* module, const AeCache8DecodeParams* p, void* s
  * the order of the rows, and `copies` gets {page, new page, slots, 0} (unused entries at the end all 0).  Pages that no row holds any more go on
  * top of the free list, in ascending order.  Nothing that is read is changed.  *status receives 0 or bits: 1 the free pages ran out (such
  * a row ends with its whole pages), 2 a length beyond the table, 4 more pages came back than had been taken (the rest is left out), 8 a parent that is no row, a negative
- * length or more tokens kept than there are, 16 a page outside the pool. */
+ * length or more tokens kept than there are, 16 a page outside the pool.
+ * Where ae_plan_lists_phases(B, max_pages, num_pages) is 0, one launch with a module of all phases (config: reserved[1] = 0, shared memory for 1024 rows and 16384
+ * pages: 16 B + 12 words + 6 num_pages + 16 bytes, with a word for 32 pages in groups of four); else modules of the phases 1, 2, 3 (reserved[1]), one behind the other with the same parameters.  Here and below. */
 typedef struct AePlanForksParams {
   const int32_t* parents;     /* [B] */
   const int32_t* seq_lens;    /* [B] */
@@ -253,16 +255,17 @@ typedef struct AePlanForksParams {
   int32_t* head_out;          /* [1] */
   int32_t* copies;            /* [B][4], 16-byte aligned */
   uint32_t* status;           /* [1] */
-  void* workspace;            /* ae_plan_lists_workspace(num_pages) bytes with any contents, 16-byte aligned */
+  void* workspace;            /* ae_plan_lists_workspace(B, num_pages) bytes with any contents, 16-byte aligned */
   int64_t table_stride;
   int32_t B, max_pages, n_free, page_size, num_pages; /* B: at most 4096; page_size: a power of two; B * max_pages below 2^31 */
 } AePlanForksParams;
-int64_t ae_plan_lists_workspace(int32_t num_pages);
+int64_t ae_plan_lists_workspace(int32_t B, int32_t num_pages);
+int ae_plan_lists_phases(int32_t B, int32_t max_pages, int32_t num_pages);
 int ae_launch_plan_forks(void* module, const AePlanForksParams* p, void* stream);
 
 /* Moves the pages in use to the front of a pool: with U of them, those from U on go into the unused ones below U, both in ascending order.
  * table_out has the new numbers, copies {page, new page, slots in use, 0} for each move (n_copies >= num_pages / 2; unused entries all 0), free_out
- * all pages in order, and *head_out is U.  Status bits 2, 8, 16 as above. */
+ * all pages in order, and *head_out is U.  Status bits 2, 8, 16 as above; four phases. */
 typedef struct AePlanCompactionParams {
   const int32_t* seq_lens;    /* [B] */
   const int32_t* block_table; /* [B, max_pages] */
@@ -296,8 +299,8 @@ int ae_launch_copy_pages(void* module, const AeCopyPagesParams* p, void* stream)
 /* ---- norm and rotation of query and key heads ------------------------------------------------
  * The module's kernel name selects what is launched: "ae_qk_rope_fwd" writes y from x; "ae_qk_rope_bwd" the gradients of x from those of y
  * (g), and with `workspace` (ae_qk_rope_workspace(module) bytes) the sums that "ae_qk_rope_dw", launched behind it with the same
- * parameters, turns into the weights' gradients.  Config: head_dim, reserved[0] rotary dims, [1] heads of a thread team on their way, [2] CTAs of an SM
- * (backward).  Index 0: queries, 1: keys (H 0: none). */
+ * parameters, turns into the weights' gradients.  Config: head_dim, reserved[0] rotary dims, and of the forward or the
+ * backward (the sums: the backward) [1] warps of a CTA, [2] heads of a thread team on their way together, [3] CTAs of an SM.  Index 0: queries, 1: keys (H 0: none). */
 typedef struct AeQkRopeParams {
   const void* x[2];       /* [B, S, H, D] 16-bit, rows 16-byte aligned */
   const void* g[2];
