@@ -23,8 +23,8 @@ STATUS_TEXT = {1: "the free pages ran out", 2: "a length is beyond block_table's
                8: "a parent is no row, a length is negative, or more tokens are kept than there are", 16: "a page is outside the pool"}
 LIST_THREADS, LIST_BATCH = (1024, 512), 4  # threads of the kernel of all phases, and of those of one
 LIST_SMEM = 16 * 1024 + 12 * 512 + 6 * 16384 + 16  # 1024 rows, 16384 pages
-COPY_THREADS, COPY_PART, COPY_CTAS = 128, 32768, 16
-COPY_DEFINES = {"AE_COPY_THREADS": COPY_THREADS, "AE_COPY_PART": COPY_PART}
+COPY_THREADS, COPY_UNROLL, COPY_CTAS, COPY_PART = 64, 16, 32, 32768  # threads, reads of each on their way, CTAs of an SM, bytes of a part
+COPY_DEFINES = {"AE_COPY_THREADS": COPY_THREADS, "AE_COPY_UNROLL": COPY_UNROLL}
 
 
 def _check(what, status):
@@ -163,6 +163,9 @@ def _refuse_copies(pools, copies):
     _ints("copies", copies, 2, copies.device)
     if copies.shape[1] != 4 or (copies.shape[0] > 1 and copies.stride(0) != 4) or copies.data_ptr() % 16:
         raise ValueError("copies must be contiguous [n, 4] at a multiple of 16 bytes")
+    for p in pools:
+        if not isinstance(p, (PagedCache8, torch.Tensor)):
+            raise TypeError(f"a pool is a PagedCache8 or a tensor, got {type(p).__name__}")
     tensors = [t for p in pools for t in ((p.k, p.v) if isinstance(p, PagedCache8) else (p,))]
     for t in tensors:
         if not t.is_cuda:

@@ -28,7 +28,7 @@ def turns_of(frequency: float) -> int:
 
 
 # of each kernel: warps of a CTA, heads of a team on their way together (the forward takes four, two or one itself), CTAs of an SM
-SHAPES = ((4, 4, 4), (8, 1, 3), (8, 1, 1))
+SHAPES = ((4, 4, 4), (8, 1, 3), (32, 1, 1))
 
 
 def _defines(D: int, R: int, norm: bool, interleaved: bool, which: int) -> dict:
@@ -62,7 +62,7 @@ class QKNormRope:
     def __init__(self, head_dim: int, rotary_dim: int | None = None, base: float = 10000.0, inv_freq=None, interleaved: bool = False, norm: bool = True,
                  eps: float = 1e-6, rotary_scale: float = 1.0):
         rotary_dim = head_dim if rotary_dim is None else rotary_dim
-        if head_dim not in HEAD_DIMS:
+        if type(head_dim) is not int or head_dim not in HEAD_DIMS:
             raise NotImplementedError(f"head dim {head_dim}: one of {HEAD_DIMS}")
         if isinstance(rotary_dim, bool) or not isinstance(rotary_dim, int) or rotary_dim % 16 or not 16 <= rotary_dim <= head_dim:
             raise ValueError(f"rotary_dim {rotary_dim}: a multiple of 16 up to head_dim = {head_dim}")

@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime_api.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -578,6 +579,12 @@ bool good_table(const Tensor& table, const Tensor& like, int64_t B) {
   return good_ints(table, 2, like) && table.size(0) == B && table.size(1) >= 1 && B * table.size(1) <= 0x7fffffff;
 }
 
+// What passes between the launches; with one launch nothing does.
+Tensor list_workspace(int64_t B, int64_t max_pages, int64_t num_pages, const Tensor& like) {
+  const bool one = ae_plan_lists_phases((int)B, (int)max_pages, (int)num_pages) == 0;
+  return one ? Tensor() : at::empty({ae_plan_lists_workspace((int)B, (int)num_pages)}, like.options().dtype(at::kByte));
+}
+
 // One launch with the first kernel, or one for each of the others.
 template <class P, class F>
 void list_phases(const std::vector<uint64_t>& kernels, const P& p, F&& launch) {
@@ -600,7 +607,7 @@ py::object plan_forks(const std::vector<uint64_t>& kernels, const Tensor& parent
   Parts parts(4 * B + B * W + B + n_free + 2, lens.options());
   Tensor copies = parts.take({B, 4}), table_out = parts.take({B, W}), lens_out = parts.take({B}), free_out = parts.take({n_free}), head = parts.take({1}),
          status = parts.take({1});
-  const Tensor workspace = at::empty({ae_plan_lists_workspace((int)B, (int)num_pages)}, lens.options().dtype(at::kByte));
+  const Tensor workspace = list_workspace(B, table.size(1), num_pages, lens);
   AePlanForksParams p;
   memset(&p, 0, sizeof p);
   p.parents = (const int32_t*)parents.data_ptr(); p.seq_lens = (const int32_t*)lens.data_ptr();
@@ -608,7 +615,7 @@ py::object plan_forks(const std::vector<uint64_t>& kernels, const Tensor& parent
   p.block_table = (const int32_t*)table.data_ptr(); p.free_pages = (const int32_t*)free_pages.data_ptr();
   p.free_head = (const int32_t*)free_head.data_ptr();
   p.table_out = (int32_t*)table_out.data_ptr(); p.lens_out = (int32_t*)lens_out.data_ptr(); p.free_out = (int32_t*)free_out.data_ptr();
-  p.head_out = (int32_t*)head.data_ptr(); p.copies = (int32_t*)copies.data_ptr(); p.status = word(status); p.workspace = workspace.data_ptr();
+  p.head_out = (int32_t*)head.data_ptr(); p.copies = (int32_t*)copies.data_ptr(); p.status = word(status); p.workspace = workspace.defined() ? workspace.data_ptr() : nullptr;
   p.table_stride = table.stride(0);
   p.B = (int)B; p.max_pages = (int)W; p.n_free = (int)n_free; p.page_size = (int)page_size; p.num_pages = (int)num_pages;
   list_phases(kernels, p, [&](void* k) { check(ae_launch_plan_forks(k, &p, stream_of(lens)), "ae_launch_plan_forks"); });
@@ -627,12 +634,12 @@ py::object plan_compaction(const std::vector<uint64_t>& kernels, const Tensor& l
   const int64_t W = table.size(1), n = num_pages / 2;
   Parts parts(4 * n + B * W + num_pages + 2, lens.options());
   Tensor copies = parts.take({n, 4}), table_out = parts.take({B, W}), free_out = parts.take({num_pages}), head = parts.take({1}), status = parts.take({1});
-  const Tensor workspace = at::empty({ae_plan_lists_workspace((int)B, (int)num_pages)}, lens.options().dtype(at::kByte));
+  const Tensor workspace = list_workspace(B, table.size(1), num_pages, lens);
   AePlanCompactionParams p;
   memset(&p, 0, sizeof p);
   p.seq_lens = (const int32_t*)lens.data_ptr(); p.block_table = (const int32_t*)table.data_ptr();
   p.table_out = (int32_t*)table_out.data_ptr(); p.free_out = (int32_t*)free_out.data_ptr(); p.head_out = (int32_t*)head.data_ptr();
-  p.copies = (int32_t*)copies.data_ptr(); p.status = word(status); p.workspace = workspace.data_ptr();
+  p.copies = (int32_t*)copies.data_ptr(); p.status = word(status); p.workspace = workspace.defined() ? workspace.data_ptr() : nullptr;
   p.table_stride = table.stride(0);
   p.B = (int)B; p.max_pages = (int)W; p.page_size = (int)page_size; p.num_pages = (int)num_pages; p.n_copies = (int)n;
   list_phases(kernels, p, [&](void* k) { check(ae_launch_plan_compaction(k, &p, stream_of(lens)), "ae_launch_plan_compaction"); });
@@ -678,8 +685,10 @@ bool copy_pages(uint64_t kernel, const py::list& pools, const Tensor& copies) {
       const Cache8& c = *h.cast<std::shared_ptr<Cache8>>();
       all.emplace_back(c.k, c.ks);
       all.emplace_back(c.v, c.vs);
-    } else {
+    } else if (THPVariable_Check(h.ptr())) {
       all.emplace_back(h.cast<Tensor>(), Tensor());
+    } else {
+      return false;
     }
   }
   std::vector<AePagePool> d(all.size());

@@ -15,8 +15,8 @@
 // Bound by HBM for long calls: everything is read and written once.  What that takes is bytes on their way, and a warp has four chains of reads in a row
 // (position, two batches of queries, keys): the forward asks L2 for a token's heads before anything else.  In a graph, 40 heads of 128 dims, bf16: 16029 tokens (236 MB) 39.3 us,
 // 6.0 TB/s (42.9 without that request; 44 to 45 with the factors made by every team for itself; 79 with factors at 64-byte steps, four-fold bank conflicts;
-// 84 with whole CTAs a token, whose barriers leave nothing on its way); forward and backward of 16384 tokens (839 MB) 154 us.  64 tokens, one a request: 2.6.
-// The backward is joined work of 24 warps an SM with one head a team on its way (80 registers): 97 us, 5.2 TB/s; a ring of copies through shared memory, two heads on their
+// 84 with whole CTAs a token, whose barriers leave nothing on its way); forward and backward of 16384 tokens (839 MB) 147 us.  64 tokens, one a request: 2.6.
+// The backward is joined work of 24 warps an SM with one head a team on its way (80 registers): 90 us, 5.6 TB/s; a ring of copies through shared memory, two heads on their
 // way, or requests to L2 ahead took 1 to 30 % more.
 // Expects AE_D (32, 64, 128 or 256), AE_R (rotary dims, a multiple of 16), AE_NORM, AE_NEXT (pairs of neighbours), AE_ROPE_WARPS, AE_ROPE_U (backward: heads
 // of a team on their way together), AE_ROPE_CTAS (of an SM), AE_ROPE_KERNEL (0 forward, 1 backward, 2 the weights' sums).
@@ -149,12 +149,10 @@ AE_DEVICE void ae_read8(const float* f, int t, u64 (&x)[8]) {
 
 // n heads on their way into L2, by a warp: what registers have no room for yet.
 AE_DEVICE void ae_prefetch_heads(const u16* x, i64 st, int n) {
-  const int lane = threadIdx.x & 31;
-  if (st == AE_D) {
-    if (lane == 0 && n > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(x), "r"(n * AE_D * 2) : "memory");
-  } else {
-    for (int h = lane; h < n; h += 32) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(x + h * st), "r"(AE_D * 2) : "memory");
-  }
+  const bool run = st == AE_D;  // heads behind each other go in pieces of 8 KB
+  const int each = run ? 8192 / (2 * AE_D) : 1;
+  for (int h = (threadIdx.x & 31) * each; h < n; h += 32 * each)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(x + h * st), "r"(min(each, n - h) * AE_D * 2) : "memory");
 }
 
 // U heads of each team from h on: y = x f0 + partner(x) f1 times the norm's factor; f1 holds the partner's weight.
@@ -162,11 +160,10 @@ template <int BF16, int U>
 AE_DEVICE void ae_rope_batch(const AeQkRopeArgs& a, const u64 (&f)[2][8], const u16* x, u16* y, i64 st, const int (&at)[2], int h, int end) {
   uint4 v[U][2];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    v[u][0] = v[u][1] = make_uint4(0, 0, 0, 0);
-    if (h + u * AE_TEAMS < end)
+  for (int u = 0; u < U; ++u) {  // a team without a head reads the last one's values, which nothing takes
+    const i64 hh = min(h + u * AE_TEAMS, end - 1);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) v[u][c] = *(const uint4*)(x + (h + u * AE_TEAMS) * st + at[c]);
+    for (int c = 0; c < 2; ++c) v[u][c] = *(const uint4*)(x + hh * st + at[c]);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -300,16 +297,14 @@ AE_DEVICE void ae_rope_bwd(const AeQkRopeArgs& a, AeRopeSmem& sm) {
     const u16* const x = AE_NORM ? here.heads(a.x[kind], a.x_st[kind]) : g;
     u16* const y = (u16*)a.y[kind] + (i64)token * H * AE_D;
     uint4 v[AE_ROPE_U][2], gv[AE_ROPE_U][2];
-    auto load = [&](int h) {
+    auto load = [&](int h) {  // a team without a head reads the last one's values, which nothing takes
 #pragma unroll
       for (int u = 0; u < AE_ROPE_U; ++u) {
-        v[u][0] = v[u][1] = gv[u][0] = gv[u][1] = make_uint4(0, 0, 0, 0);
-        if (h + u * AE_TEAMS < h1) {
+        const int hh = min(h + u * AE_TEAMS, h1 - 1);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            gv[u][c] = *(const uint4*)(g + (h + u * AE_TEAMS) * g_st + at[c]);
-            if (AE_NORM) v[u][c] = *(const uint4*)(x + (h + u * AE_TEAMS) * x_st + at[c]);
-          }
+        for (int c = 0; c < 2; ++c) {
+          gv[u][c] = *(const uint4*)(g + hh * g_st + at[c]);
+          if (AE_NORM) v[u][c] = *(const uint4*)(x + hh * x_st + at[c]);
         }
       }
     };
@@ -348,14 +343,13 @@ AE_DEVICE void ae_rope_bwd(const AeQkRopeArgs& a, AeRopeSmem& sm) {
         u64 sum = ae_mul2(z[0], z[0]);
 #pragma unroll
         for (int k = 1; k < 8; ++k) sum = ae_fma22(z[k], z[k], sum);
-        float r = rsqrtf(fmaf(ae_team_sum(ae_sum2(sum)), 1.f / AE_D, a.eps));
-        if (h >= h1) r = 0.f;  // no head: with eps = 0 its zeros would make the sums NaN
+        const float r = rsqrtf(fmaf(ae_team_sum(ae_sum2(sum)), 1.f / AE_D, a.eps));
         u64 dot = 0;  // of (dz r w) x: sum of dn n
         ae_read8(sm.w[0], t, k2);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           dz[k] = ae_mul2(dz[k], ae_pack2f(r, r));
-          dw2[k] = ae_fma22(dz[k], z[k], dw2[k]);
+          if (h < h1) dw2[k] = ae_fma22(dz[k], z[k], dw2[k]);
           dz[k] = ae_mul2(dz[k], k2[k]);
           dot = ae_fma22(dz[k], z[k], dot);
         }

@@ -255,7 +255,7 @@ typedef struct AePlanForksParams {
   int32_t* head_out;          /* [1] */
   int32_t* copies;            /* [B][4], 16-byte aligned */
   uint32_t* status;           /* [1] */
-  void* workspace;            /* ae_plan_lists_workspace(B, num_pages) bytes with any contents, 16-byte aligned */
+  void* workspace;            /* of single phases: ae_plan_lists_workspace(B, num_pages) bytes with any contents, 16-byte aligned */
   int64_t table_stride;
   int32_t B, max_pages, n_free, page_size, num_pages; /* B: at most 4096; page_size: a power of two; B * max_pages below 2^31 */
 } AePlanForksParams;
