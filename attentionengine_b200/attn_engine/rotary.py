@@ -4,8 +4,8 @@
     q, k = rope(q, k, positions, q_weight, k_weight)             # [B, S, H, D] or [T, H, D], with gradients
     o = engine(q, k, v)
 
-In a serving step ``positions`` is ``plan_pages(...).positions``.  The reference's scripts take queries and keys as they come
-(attn_script/mha.py:86-104); models norm and rotate them first.
+In a serving step ``positions`` is ``plan_pages(...).positions``.  The reference's scripts take queries and keys as they come (attn_script/mha.py); models
+norm and rotate them first.
 """
 from __future__ import annotations
 
