@@ -235,6 +235,8 @@ class PagedLayers:
 
     def __init__(self, n_layers, Hq, Hkv, D, dtype, rows, num_pages, page_size, max_len, device="cuda", rope=None, weights=None):
         self.page_size, self.rows, self.num_pages = page_size, rows, num_pages
+        if weights is not None and (rope is None or len(weights) != n_layers):
+            raise ValueError(f"weights are (q_weight, k_weight) of each of the {n_layers} layers, for a rope")
         self.rope, self.weights = rope, weights if weights is not None else [(None, None)] * n_layers
         self.caches = [PagedCache8(num_pages, page_size, Hkv, D, device=device) for _ in range(n_layers)]
         self.prompt = softmax_engine("B", Hq, Hkv, "S", D, D, dtype, True, packed=True)

@@ -5,12 +5,14 @@ Bounds: keys and values are held in e4m3 (half a step: 2^-4 of the value; 2^-5 r
 the values' size beside the value's own rounding, and a score by 2^-5 of |q| |k| / sqrt(D).  The plain form takes the codes as the cache rounds them: with the same scales it
 is exact, without (a forked page keeps the coarser scale of the page it was copied from) codes differ by nothing but subnormals.  What is left are the 16-bit
 roundings of rotated heads, probabilities and outputs: four of 2^-9 (fp16: 2^-12) rms of the output's norm; 2^-7 (2^-10) holds them."""
+import random
+
 import pytest
 import torch
 
 import cache8_ref
 import rope_ref
-from attentionengine_b200 import QKNormRope, examples
+from attentionengine_b200 import QKNormRope, copy_pages, examples, plan_compaction, plan_forks
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +107,49 @@ def test_what_does_not_fit_is_reported():
     serve.fork(ints([0, 0, 7]))
     with pytest.raises(ValueError, match="plan_forks"):
         serve.check()
+
+
+def test_weights_of_other_layers_are_refused():
+    w = [(None, None)]
+    for kw in (dict(rope=QKNormRope(64), weights=w), dict(weights=w * 2)):
+        with pytest.raises(ValueError, match="weights"):
+            examples.PagedLayers(2, 2, 1, 64, torch.float16, 3, 4, 16, 64, **kw)
+
+
+@pytest.mark.parametrize("kind", ["grouped heads", "latent"])
+def test_16_bit_pools(kind):
+    """Forks, cuts, a compaction and their copies in the pools of the 16-bit decodes: each row's output is bit for bit that of its tokens in an untouched pool."""
+    rng = random.Random(4)
+    g = torch.Generator().manual_seed(3)
+    randn = lambda *s: torch.randn(*s, generator=g).half().cuda()  # noqa: E731
+    page, B, N = 128 if kind == "grouped heads" else 64, 5, 60
+    lens = [rng.randrange(1, 7 * page) for _ in range(B)]
+    ids, table, at = rng.sample(range(N), N), [], 0
+    for n in lens:
+        need = -(-n // page)
+        table.append(ids[at:at + need] + [0] * (8 - need))
+        at += need
+    if kind == "grouped heads":
+        eng = examples.decode_engine("B", 8, 2, 1, "S", 64, torch.float16)
+        pools, q = [randn(N, page, 2, 64), randn(N, page, 2, 64)], randn(1, 1, 8, 64).expand(B, -1, -1, -1).contiguous()
+
+        def decode(pools, table, lens):
+            return eng.decode_varlen(q, *pools, lens, block_table=table)
+    else:
+        eng = examples.mla_engine("B", 16, "S", torch.float16, 0.1)
+        pools, q = [randn(N, page, 1, 576)], randn(1, 1, 16, 576).expand(B, -1, -1, -1).contiguous()
+
+        def decode(pools, table, lens):
+            return torch.cat([t.float().flatten(1) for t in eng.decode_paged(q, *pools, table, lens, num_split=1)], 1)
+
+    parents, keep = [2, 2, 2, 0, 4], [lens[2], lens[2], lens[2] // 2 + 1, lens[0], lens[4] // 3 + 1]
+    want = decode([p.clone() for p in pools], ints([table[p] for p in parents]), ints(keep))
+    f = plan_forks(ints(parents), ints(lens), ints(table), ints(ids), ints([at]), page, N, keep_lens=ints(keep))
+    copy_pages(pools, f.copies)
+    f.check()
+    assert torch.equal(decode(pools, f.block_table, f.seq_lens), want)
+    c = plan_compaction(f.seq_lens, f.block_table, page, N)
+    copy_pages(pools, c.copies)
+    c.check()
+    held = c.free_head.item()
+    assert torch.equal(decode([p[:held].contiguous() for p in pools], c.block_table, f.seq_lens), want)
