@@ -107,6 +107,7 @@ def plan_forks(parents, seq_lens, block_table, free_pages, free_head, page_size:
     ``copies``.  Pages that no row holds any more go back to the free list, lowest on top.  So a sampled prompt is B rows with one parent, a beam
     search's step its parents, and a cut (speculation that failed) a row that keeps less of itself.
 
+    Rows are shortened through ``keep_lens`` alone: a length that a caller lowers by itself would let ``plan_pages`` put new tokens into a page that other rows hold.
     Pages that something beside the table's rows is to keep (a prefix for later requests) need a row of their own in it.  What does not fit is left
     out and reported in ``status``."""
     _sizes(page_size, num_pages)

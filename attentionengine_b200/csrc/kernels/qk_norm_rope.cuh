@@ -15,8 +15,8 @@
 // Bound by HBM for long calls: everything is read and written once.  What that takes is bytes on their way, and a warp has four chains of reads in a row
 // (position, two batches of queries, keys): the forward asks L2 for a token's heads before anything else.  In a graph, 40 heads of 128 dims, bf16: 16029 tokens (236 MB) 39.3 us,
 // 6.0 TB/s (42.9 without that request; 44 to 45 with the factors made by every team for itself; 79 with factors at 64-byte steps, four-fold bank conflicts;
-// 84 with whole CTAs a token, whose barriers leave nothing on its way); forward and backward of 16384 tokens (839 MB) 147 us.  64 tokens, one a request: 2.6.
-// The backward is joined work of 24 warps an SM with one head a team on its way (80 registers): 90 us, 5.6 TB/s; a ring of copies through shared memory, two heads on their
+// 84 with whole CTAs a token, whose barriers leave nothing on its way); forward and backward of 16384 tokens (839 MB) 145 us.  64 tokens, one a request: 2.6.
+// The backward is joined work of 24 warps an SM with one head a team on its way (80 registers): 88 us, 5.7 TB/s; a ring of copies through shared memory, two heads on their
 // way, or requests to L2 ahead took 1 to 30 % more.
 // Expects AE_D (32, 64, 128 or 256), AE_R (rotary dims, a multiple of 16), AE_NORM, AE_NEXT (pairs of neighbours), AE_ROPE_WARPS, AE_ROPE_U (backward: heads
 // of a team on their way together), AE_ROPE_CTAS (of an SM), AE_ROPE_KERNEL (0 forward, 1 backward, 2 the weights' sums).
@@ -86,6 +86,9 @@ AE_DEVICE u64 ae_partner(const u64 (&x)[8], int k) {
   return x[k ^ 4];
 #endif
 }
+// Whether thread t's values are rotated ones; the others must not meet their partners, not even times 0 (an infinity would make them NaN).
+AE_DEVICE bool ae_rotates(int t) { return AE_R == AE_D || t < AE_R / 16; }
+
 AE_DEVICE float ae_team_sum(float x) {
 #pragma unroll
   for (int o = 1; o < AE_TPR; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
@@ -97,7 +100,7 @@ AE_DEVICE float ae_team_sum(float x) {
 #define AE_KINDS (AE_ROPE_KERNEL == 0 ? 2 : 1)
 // Factors of each value and of its partner, as the threads read them (ae_place).
 struct AeRopeSmem {
-  float f[AE_ROPE_WARPS][AE_KINDS][2][AE_D];
+  float f[AE_ROPE_WARPS][AE_KINDS][2][AE_D];  // forward: with the weights; backward: cos and sin
   float w[AE_KINDS][AE_D];  // weights, in that order too
   u64 turns[AE_PAIRS];
 #if AE_ROPE_KERNEL == 1 && AE_NORM
@@ -136,11 +139,12 @@ struct AeRopeToken {
   AE_DEVICE const u16* heads(const void* x, const i64 (&st)[3]) const { return (const u16*)x + b * st[0] + s * st[1]; }
 };
 
-// Thread t's 16 values.
-AE_DEVICE void ae_read8(const float* f, int t, u64 (&x)[8]) {
+// Thread t's 16 values, or the first 8.
+template <int N>
+AE_DEVICE void ae_read(const float* f, int t, u64 (&x)[N]) {
   const u32 at = smem_u32(f) + 16 * t;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < N / 2; ++i)
     asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(x[2 * i]), "=l"(x[2 * i + 1]) : "r"(at + 16 * AE_TPR * i) : "memory");
 }
 
@@ -157,7 +161,7 @@ AE_DEVICE void ae_prefetch_heads(const u16* x, i64 st, int n) {
 
 // U heads of each team from h on: y = x f0 + partner(x) f1 times the norm's factor; f1 holds the partner's weight.
 template <int BF16, int U>
-AE_DEVICE void ae_rope_batch(const AeQkRopeArgs& a, const u64 (&f)[2][8], const u16* x, u16* y, i64 st, const int (&at)[2], int h, int end) {
+AE_DEVICE void ae_rope_batch(const AeQkRopeArgs& a, const u64 (&f)[2][8], bool rotates, const u16* x, u16* y, i64 st, const int (&at)[2], int h, int end) {
   uint4 v[U][2];
 #pragma unroll
   for (int u = 0; u < U; ++u) {  // a team without a head reads the last one's values, which nothing takes
@@ -170,7 +174,10 @@ AE_DEVICE void ae_rope_batch(const AeQkRopeArgs& a, const u64 (&f)[2][8], const 
     u64 z[8], o[8];
     ae_unpack16<BF16>(v[u][0], v[u][1], z);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) o[k] = ae_fma22(z[k], f[0][k], ae_mul2(ae_partner(z, k), f[1][k]));
+    for (int k = 0; k < 8; ++k) {
+      const u64 other = rotates ? ae_partner(z, k) : 0;
+      o[k] = ae_fma22(z[k], f[0][k], ae_mul2(other, f[1][k]));
+    }
 #if AE_NORM
     u64 sum = ae_mul2(z[0], z[0]);
 #pragma unroll
@@ -199,13 +206,13 @@ AE_DEVICE void ae_rope_heads(const AeQkRopeArgs& a, const AeRopeSmem& sm, bool n
   const int at[2] = {ae_chunk(t, 0), ae_chunk(t, 1)};
   u64 f[2][8];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) ae_read8(sm.f[threadIdx.x >> 5][kind][i], t, f[i]);
+  for (int i = 0; i < 2; ++i) ae_read(sm.f[threadIdx.x >> 5][kind][i], t, f[i]);
 #pragma unroll 1
-  for (; h0 + 2 * AE_TEAMS < h1; h0 += 4 * AE_TEAMS) ae_rope_batch<BF16, 4>(a, f, x, y, st, at, h0 + team, h1);
+  for (; h0 + 2 * AE_TEAMS < h1; h0 += 4 * AE_TEAMS) ae_rope_batch<BF16, 4>(a, f, ae_rotates(t), x, y, st, at, h0 + team, h1);
   if (h0 + AE_TEAMS < h1)
-    ae_rope_batch<BF16, 2>(a, f, x, y, st, at, h0 + team, h1);
+    ae_rope_batch<BF16, 2>(a, f, ae_rotates(t), x, y, st, at, h0 + team, h1);
   else if (h0 < h1)
-    ae_rope_batch<BF16, 1>(a, f, x, y, st, at, h0 + team, h1);
+    ae_rope_batch<BF16, 1>(a, f, ae_rotates(t), x, y, st, at, h0 + team, h1);
 }
 
 template <int BF16>
@@ -275,13 +282,7 @@ AE_DEVICE void ae_rope_bwd(const AeQkRopeArgs& a, AeRopeSmem& sm) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = lane % AE_TPR, team = lane / AE_TPR;
   const int at[2] = {ae_chunk(t, 0), ae_chunk(t, 1)};
   const i64 x_st = a.x_st[kind][2], g_st = a.g_st[kind][2];
-  for (int d = threadIdx.x; d < AE_D; d += AE_ROPE_THREADS) {
-    const int place = ae_place(d);
-    sm.w[0][place] = ae_weight(a, kind, d);
-    if (d >= AE_R)
-#pragma unroll
-      for (int k = 0; k < AE_ROPE_WARPS; ++k) sm.f[k][0][0][place] = 1.f, sm.f[k][0][1][place] = 0.f;
-  }
+  for (int d = threadIdx.x; d < AE_D; d += AE_ROPE_THREADS) sm.w[0][ae_place(d)] = ae_weight(a, kind, d);
   __syncthreads();
   u64 dw2[8];
 #pragma unroll
@@ -315,13 +316,17 @@ AE_DEVICE void ae_rope_bwd(const AeQkRopeArgs& a, AeRopeSmem& sm) {
     }
     __syncwarp();  // the factors of the token in front have been read
 #pragma unroll
-    for (int i = lane; i < AE_PAIRS; i += 32) {  // dz = g f0 + partner(g) f1
+    for (int i = lane; i < AE_PAIRS; i += 32) {  // dz_a = g_a c + g_b s, dz_b = g_b c - g_a s
       const float2 r = ae_turn(sm.turns[i], p);
       const float c = r.x * a.scale, s = r.y * a.scale;
-      const int pa = ae_place(AE_NEXT ? 2 * i : i), pb = ae_place(AE_NEXT ? 2 * i + 1 : i + AE_R / 2);
-      f[0][pa] = f[0][pb] = c;
-      f[1][pa] = s;
-      f[1][pb] = -s;
+#if AE_NEXT
+      f[0][ae_place(2 * i)] = f[0][ae_place(2 * i + 1)] = c;
+      f[1][ae_place(2 * i)] = s;
+      f[1][ae_place(2 * i + 1)] = -s;
+#else
+      f[0][ae_place(i)] = c;  // of both halves
+      f[1][ae_place(i)] = s;
+#endif
     }
     __syncwarp();
 #pragma unroll 1
@@ -331,12 +336,29 @@ AE_DEVICE void ae_rope_bwd(const AeQkRopeArgs& a, AeRopeSmem& sm) {
         const int h = base + u * AE_TEAMS + team;
         u64 g2[8], dz[8], k2[8];
         ae_unpack16<BF16>(gv[u][0], gv[u][1], g2);
-        ae_read8(f[1], t, k2);
+        if (ae_rotates(t)) {
+#if AE_NEXT
+          ae_read(f[1], t, k2);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) dz[k] = ae_mul2(ae_partner(g2, k), k2[k]);
-        ae_read8(f[0], t, k2);
+          for (int k = 0; k < 8; ++k) dz[k] = ae_mul2(ae_partner(g2, k), k2[k]);
+          ae_read(f[0], t, k2);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) dz[k] = ae_fma22(g2[k], k2[k], dz[k]);
+          for (int k = 0; k < 8; ++k) dz[k] = ae_fma22(g2[k], k2[k], dz[k]);
+#else
+          u64 c2[4], s2[4];
+          ae_read(f[0], t, c2);
+          ae_read(f[1], t, s2);
+          const u64 minus = ae_pack2f(-1.f, -1.f);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            dz[k] = ae_fma22(g2[k + 4], s2[k], ae_mul2(g2[k], c2[k]));
+            dz[k + 4] = ae_fma22(ae_mul2(g2[k], s2[k]), minus, ae_mul2(g2[k + 4], c2[k]));
+          }
+#endif
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) dz[k] = g2[k];
+        }
 #if AE_NORM
         u64 z[8];
         ae_unpack16<BF16>(v[u][0], v[u][1], z);
@@ -345,7 +367,7 @@ AE_DEVICE void ae_rope_bwd(const AeQkRopeArgs& a, AeRopeSmem& sm) {
         for (int k = 1; k < 8; ++k) sum = ae_fma22(z[k], z[k], sum);
         const float r = rsqrtf(fmaf(ae_team_sum(ae_sum2(sum)), 1.f / AE_D, a.eps));
         u64 dot = 0;  // of (dz r w) x: sum of dn n
-        ae_read8(sm.w[0], t, k2);
+        ae_read(sm.w[0], t, k2);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           dz[k] = ae_mul2(dz[k], ae_pack2f(r, r));

@@ -198,6 +198,33 @@ def test_rows_of_zeros_and_what_is_not_finite():
     assert (out == 1).all() and (dw == 15).all() and (dv == 0).all()
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("norm", [False, True])
+def test_dims_that_are_not_rotated_keep_to_themselves(interleaved, norm):
+    """An infinity or NaN in one of them reaches no other dim, forward or backward, but through the norm's factor (which it makes 0 or NaN)."""
+    g = gen(15)
+    rope = QKNormRope(128, rotary_dim=64, interleaved=interleaved, norm=norm)
+    pos = torch.arange(6, device="cuda")
+    for bad in (float("inf"), float("nan")):
+        x, grad = randn(g, 6, 3, 128, dtype=torch.float16), randn(g, 6, 3, 128, dtype=torch.float16)
+        clean = rope(x, None, pos)[0]
+        for d in (64, 71, 72, 80, 127):
+            y = x.clone()
+            y[2, 1, d] = bad
+            out = rope(y, None, pos)[0]
+            rest = torch.arange(128, device="cuda") != d
+            assert not out[2, 1, d].isfinite()
+            want = clean[2, 1] if not norm else torch.zeros_like(clean[2, 1]) if bad == float("inf") else torch.full_like(clean[2, 1], bad)
+            assert torch.equal(out[2, 1][rest].nan_to_num(7.0), want[rest].nan_to_num(7.0))
+            out[2, 1] = clean[2, 1]
+            assert torch.equal(out, clean)
+            if not norm:
+                leaf, gr = x.clone().requires_grad_(), grad.clone()
+                gr[2, 1, d] = bad
+                got, fine = (torch.autograd.grad(rope(leaf, None, pos)[0], leaf, t)[0] for t in (gr, grad))
+                assert not got[2, 1, d].isfinite() and torch.equal(got[2, 1][rest], fine[2, 1][rest])
+
+
 def test_nothing_to_do():
     rope = QKNormRope(64)
     w = torch.ones(64, device="cuda", requires_grad=True)
