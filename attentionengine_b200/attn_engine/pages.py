@@ -23,8 +23,7 @@ STATUS_TEXT = {1: "the free pages ran out", 2: "a length is beyond block_table's
                8: "a parent is no row, a length is negative, or more tokens are kept than there are", 16: "a page is outside the pool"}
 LIST_THREADS, LIST_BATCH = (1024, 512), 4  # threads of the kernel of all phases, and of those of one
 LIST_SMEM = 16 * 1024 + 12 * 512 + 6 * 16384 + 16  # 1024 rows, 16384 pages
-COPY_THREADS, COPY_UNROLL, COPY_CTAS, COPY_PART = 64, 16, 32, 32768  # threads, reads of each on their way, CTAs of an SM, bytes of a part
-COPY_DEFINES = {"AE_COPY_THREADS": COPY_THREADS, "AE_COPY_UNROLL": COPY_UNROLL}
+COPY_THREADS, COPY_UNROLL, COPY_CTAS, COPY_PART = 64, (8, 16), 32, 32768  # threads, reads of each on their way, CTAs of an SM, bytes of a part
 
 
 def _check(what, status):
@@ -84,11 +83,19 @@ def _compaction_kernels():
     return _list_kernels(rt.KIND_PLAN_COMPACTION, "plan_compaction.cuh", "ae_plan_compaction", 4)
 
 
+def _copy_source(runs: bool) -> str:
+    return rt.kernel_source("copy_pages.cuh", defines={"AE_COPY_THREADS": COPY_THREADS, "AE_COPY_UNROLL": COPY_UNROLL[runs], "AE_COPY_RUNS": int(runs)})
+
+
 @functools.lru_cache(maxsize=None)
-def _copy_kernel():
-    cfg = rt.KernelConfig(kind=rt.KIND_COPY_PAGES, threads=COPY_THREADS)
-    cfg.reserved[0], cfg.reserved[1] = COPY_PART, COPY_CTAS
-    return rt.compile_module(rt.kernel_source("copy_pages.cuh", defines=COPY_DEFINES), "ae_copy_pages", cfg)
+def _copy_kernels():
+    """For pools of any layout, and for those whose slots lie behind each other."""
+    out = []
+    for runs in (False, True):
+        cfg = rt.KernelConfig(kind=rt.KIND_COPY_PAGES, threads=COPY_THREADS)
+        cfg.reserved[0], cfg.reserved[1], cfg.reserved[2] = COPY_PART, COPY_CTAS, int(runs)
+        out.append(rt.compile_module(_copy_source(runs), "ae_copy_pages", cfg))
+    return tuple(out), [m.handle.value for m in out]
 
 
 def _sizes(page_size, num_pages):
@@ -154,9 +161,10 @@ def copy_pages(pools, copies) -> None:
     contiguous, all of one pool size and page size.
 
     ``copies`` of ``plan_forks`` and ``plan_compaction`` fit as they are.  It ends at its first entry without slots; entries with pages outside the pools or more
-    slots than a page has are passed over.  New pages are distinct, and none is another entry's source.  48 pools (24 caches) a launch."""
+    slots than a page has are passed over.  New pages are distinct, and none is another entry's source.  48 pools (24 caches) a launch, those whose slots
+    do not lie behind each other apart."""
     pools = list(pools) if isinstance(pools, (list, tuple)) else [pools]
-    if not rt.host().copy_pages(_copy_kernel().handle.value, [p._native if isinstance(p, PagedCache8) else p for p in pools], copies):
+    if not rt.host().copy_pages(*_copy_kernels()[1], [p._native if isinstance(p, PagedCache8) else p for p in pools], copies):
         _refuse_copies(pools, copies)
 
 

@@ -690,7 +690,7 @@ bool pool_of(const Tensor& t, AePagePool& d) {
 }
 
 // `pools`: caches (their native side) and tensors.  False when they or the list do not fit.
-bool copy_pages(uint64_t kernel, const py::list& pools, const Tensor& copies) {
+bool copy_pages(uint64_t any, uint64_t runs, const py::list& pools, const Tensor& copies) {
   if (!good_ints(copies, 2, copies) || copies.size(1) != 4 || (copies.size(0) > 1 && copies.stride(0) != 4) || copies.size(0) > 0x7fffffff ||
       reinterpret_cast<uintptr_t>(copies.data_ptr()) % 16)
     return false;
@@ -730,10 +730,12 @@ bool copy_pages(uint64_t kernel, const py::list& pools, const Tensor& copies) {
   p.copies = (const int32_t*)copies.data_ptr();
   p.n_copies = (int)copies.size(0);
   p.num_pages = (int)all[0].first.size(0); p.page_size = (int)all[0].first.size(1);
-  for (size_t i = 0; i < n; i += AE_MAX_COPY_POOLS) {
-    p.n_pools = (int)std::min<size_t>(n - i, AE_MAX_COPY_POOLS);
-    std::copy(d.begin() + i, d.begin() + i + p.n_pools, p.pools);
-    check(ae_launch_copy_pages(handle(kernel), &p, stream_of(copies)), "ae_launch_copy_pages");
+  d.resize(n);
+  const auto split = std::stable_partition(d.begin(), d.end(), [](const AePagePool& x) { return x.rows == 1 && x.slot_stride == x.run_bytes; });
+  for (auto at = d.begin(); at != d.end(); at += p.n_pools) {
+    p.n_pools = (int)std::min<size_t>((at < split ? split : d.end()) - at, AE_MAX_COPY_POOLS);
+    std::copy(at, at + p.n_pools, p.pools);
+    check(ae_launch_copy_pages(handle(at < split ? runs : any), &p, stream_of(copies)), "ae_launch_copy_pages");
   }
   for (auto& t : all)  // what autograd has saved of a pool has changed
     if (!t.first.is_inference()) t.first.unsafeGetTensorImpl()->bump_version();

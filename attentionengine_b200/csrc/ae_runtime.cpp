@@ -1393,12 +1393,16 @@ int ae_launch_copy_pages(void* module, const AeCopyPagesParams* p, void* stream)
       set_error("copy_pages: a pool with rows of at least a byte, pages below 2 GB, extra words of 4 bytes");
       return AE_ERR_INVALID;
     }
+    if (m->cfg.reserved[2] && !(s.rows == 1 && s.slot_stride == s.run_bytes)) {
+      set_error("copy_pages: this module is for pools whose slots lie behind each other");
+      return AE_ERR_INVALID;
+    }
     d.base = (u8*)s.base; d.extra = (u8*)s.extra;
     d.page_st = s.page_stride; d.slot_st = s.slot_stride; d.row_st = s.row_stride; d.extra_st = s.extra_stride;
     d.rows = s.rows; d.run = s.run_bytes; d.extra_bytes = s.extra_bytes;
     const uint64_t all = (uint64_t)(uintptr_t)s.base | (uint64_t)s.page_stride | (uint64_t)s.run_bytes | (p->page_size > 1 ? (uint64_t)s.slot_stride : 0) |
                          (s.rows > 1 ? (uint64_t)s.row_stride : 0);
-    d.vec = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
+    d.vec = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1;
     d.slots_part = (int)std::max<int64_t>(1, part_bytes / slot);
     d.first = a.parts;
     a.parts += (p->page_size + d.slots_part - 1) / d.slots_part;

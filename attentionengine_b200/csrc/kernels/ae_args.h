@@ -381,7 +381,7 @@ struct AeCopyPool {
   i64 page_st, slot_st, row_st, extra_st;  // bytes
   int rows, run;     // of a slot; run: contiguous bytes
   int extra_bytes;
-  int vec;           // bytes of an access: 16, 4 or 1
+  int vec;           // bytes of an access: 16, 4, 2 or 1
   int first;         // its first part of a copy's
   int slots_part;    // slots of a part
 };

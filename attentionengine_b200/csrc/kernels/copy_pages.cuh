@@ -2,35 +2,46 @@
 //
 // A copy's bytes are cut into parts, and a CTA takes parts in turn: one load of the list's entry, then sixteen loads a thread in front of their
 // stores.  HBM-bound once a few hundred parts are under way: 1500 pages of 64 tokens, 8 heads of 128 dims, in four layers (1.5 GB
-// in and out) 248 us, 6.1 TB/s; 96 begun ones in eight layers (96 MB) 18.6 us, 5.2 TB/s.  Eight reads a thread in 256 of them, 257 and 20.8; four, 283 and 25; parts of
+// in and out) 251 us, 6.1 TB/s; 96 begun ones in eight layers (96 MB) 18.4 us, 5.2 TB/s.  Eight reads a thread in 256 of them, 257 and 20.8; four, 283 and 25; parts of
 // 8 KB, 275 and 25.5, of 64 KB, 248 and 20.2.  Which page goes where and how many slots stands on the device; a list ends at
 // its first entry without slots, which every CTA looks for itself (its length is next to nothing beside the pages that it names).  Entries that name a
 // page outside the pool, or more slots than a page has, are passed over.
-// Expects AE_COPY_THREADS, AE_COPY_UNROLL (reads of a thread in front of its writes).
+// A build for pools whose slots lie behind each other (AE_COPY_RUNS), and one for others, whose places take registers of their own: 1200 pages whose 8 heads lie
+// one behind the other 27.5 us, 5.7 TB/s (37 with both in one build, 85 without reads in front of the writes).  Seven CTAs an SM at least: left to the compiler 173
+// registers, the begun pages 21.4 us.
+// Expects AE_COPY_THREADS, AE_COPY_UNROLL (reads of a thread in front of its writes), AE_COPY_RUNS.
 
 // n units of V, from the unit `from` on of a page's part.  A pool's slots are runs of `per` units, row_st bytes apart, `rows` of them in slot_st bytes.
 template <typename V>
 AE_DEVICE void ae_copy_part(const AeCopyPool& p, const u8* src, u8* dst, int from, int n) {
-  const int per = p.run / (int)sizeof(V);
-  if (p.rows == 1 && p.slot_st == p.run) {  // slots behind each other
-    src += (i64)from * sizeof(V);
-    dst += (i64)from * sizeof(V);
-    for (int i = threadIdx.x; i < n; i += AE_COPY_THREADS * AE_COPY_UNROLL) {
-      V v[AE_COPY_UNROLL];
+#if AE_COPY_RUNS
+  src += (i64)from * sizeof(V);
+  dst += (i64)from * sizeof(V);
+  for (int i = threadIdx.x; i < n; i += AE_COPY_THREADS * AE_COPY_UNROLL) {
+    V v[AE_COPY_UNROLL];
 #pragma unroll
-      for (int u = 0; u < AE_COPY_UNROLL; ++u)
-        if (i + u * AE_COPY_THREADS < n) v[u] = __ldcs((const V*)src + i + u * AE_COPY_THREADS);
+    for (int u = 0; u < AE_COPY_UNROLL; ++u)
+      if (i + u * AE_COPY_THREADS < n) v[u] = __ldcs((const V*)src + i + u * AE_COPY_THREADS);
 #pragma unroll
-      for (int u = 0; u < AE_COPY_UNROLL; ++u)
-        if (i + u * AE_COPY_THREADS < n) __stcs((V*)dst + i + u * AE_COPY_THREADS, v[u]);
-    }
-  } else {
-    for (int i = from + threadIdx.x; i < from + n; i += AE_COPY_THREADS) {
-      const int row = i / per, slot = row / p.rows;
-      const i64 at = slot * p.slot_st + (row - slot * p.rows) * p.row_st + (i64)(i - row * per) * sizeof(V);
-      *(V*)(dst + at) = *(const V*)(src + at);
-    }
+    for (int u = 0; u < AE_COPY_UNROLL; ++u)
+      if (i + u * AE_COPY_THREADS < n) __stcs((V*)dst + i + u * AE_COPY_THREADS, v[u]);
   }
+#else
+  const int per = p.run / (int)sizeof(V), end = from + n;
+  for (int i0 = from + threadIdx.x; i0 < end; i0 += AE_COPY_THREADS * AE_COPY_UNROLL) {
+    V v[AE_COPY_UNROLL];
+    i64 at[AE_COPY_UNROLL];
+#pragma unroll
+    for (int u = 0; u < AE_COPY_UNROLL; ++u) {
+      const int i = min(i0 + u * AE_COPY_THREADS, end - 1), row = i / per, slot = row / p.rows;
+      at[u] = slot * p.slot_st + (row - slot * p.rows) * p.row_st + (i64)(i - row * per) * sizeof(V);
+      v[u] = __ldcs((const V*)(src + at[u]));
+    }
+#pragma unroll
+    for (int u = 0; u < AE_COPY_UNROLL; ++u)
+      if (i0 + u * AE_COPY_THREADS < end) __stcs((V*)(dst + at[u]), v[u]);
+  }
+#endif
 }
 
 // Entries in front of the first without slots.
@@ -54,7 +65,7 @@ AE_DEVICE int ae_list_length(const AePageCopy* copies, int most) {
   return most;
 }
 
-extern "C" __global__ void __launch_bounds__(AE_COPY_THREADS) ae_copy_pages(const __grid_constant__ AeCopyPagesArgs a) {
+extern "C" __global__ void __launch_bounds__(AE_COPY_THREADS, 7) ae_copy_pages(const __grid_constant__ AeCopyPagesArgs a) {
   ae_grid_wait();
   ae_grid_trigger();
   const i64 items = (i64)ae_list_length(a.copies, a.n_copies) * a.parts;
@@ -77,6 +88,8 @@ extern "C" __global__ void __launch_bounds__(AE_COPY_THREADS) ae_copy_pages(cons
       ae_copy_part<uint4>(p, src, dst, s0 * slot, (s1 - s0) * slot);
     else if (p.vec == 4)
       ae_copy_part<u32>(p, src, dst, s0 * slot, (s1 - s0) * slot);
+    else if (p.vec == 2)
+      ae_copy_part<u16>(p, src, dst, s0 * slot, (s1 - s0) * slot);
     else
       ae_copy_part<u8>(p, src, dst, s0 * slot, (s1 - s0) * slot);
   }

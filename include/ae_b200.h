@@ -281,7 +281,8 @@ typedef struct AePlanCompactionParams {
 int ae_launch_plan_compaction(void* module, const AePlanCompactionParams* p, void* stream);
 
 /* The first slots of pages into other pages, in up to AE_MAX_COPY_POOLS pools.  `copies` ends at its first entry without slots; entries that name pages
- * outside the pools, or more slots than a page has, are passed over.  Destinations are distinct and no entry's source. */
+ * outside the pools, or more slots than a page has, are passed over.  Destinations are distinct and no entry's source.  Config: reserved[0] bytes of a part, [1] CTAs
+ * of an SM, [2] 1: for pools of one row a slot, slots behind each other, alone. */
 #define AE_MAX_COPY_POOLS 48
 typedef struct AePagePool {
   void* base;            /* [num_pages, page_size, rows, run_bytes], strides in bytes */

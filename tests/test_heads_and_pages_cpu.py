@@ -41,7 +41,7 @@ def test_entry_points_refuse_bad_arguments():
     L = rt.lib()
     for name in ("ae_launch_plan_forks", "ae_launch_plan_compaction", "ae_launch_copy_pages", "ae_launch_qk_rope"):
         assert getattr(L, name)(None, None, None) == 1
-    forks, pack, copy = pages._forks_kernels()[0][0], pages._compaction_kernels()[0][0], pages._copy_kernel()
+    forks, pack, copy = pages._forks_kernels()[0][0], pages._compaction_kernels()[0][0], pages._copy_kernels()[0][0]
     p = rt.PlanForksParams(*(64 * (i + 1) for i in range(13)))
     p.B, p.max_pages, p.n_free, p.page_size, p.num_pages = 2, 3, 4, 16, 5
     assert L.ae_launch_plan_forks(copy.handle, C.byref(p), None) == 6
@@ -65,6 +65,9 @@ def test_entry_points_refuse_bad_arguments():
         for k, v in pool.items():
             setattr(q.pools[0], k, v)
         assert L.ae_launch_copy_pages(copy.handle, C.byref(q), None) == 1, pool
+    rows = rt.CopyPagesParams.from_buffer_copy(bytes(m))
+    rows.pools[0].rows, rows.pools[0].run_bytes = 2, 32
+    assert L.ae_launch_copy_pages(pages._copy_kernels()[0][1].handle, C.byref(rows), None) == 1
     assert L.ae_plan_lists_workspace(3, 5) == 16 * 3 + 12 * 4 + 4 * 5
     assert L.ae_plan_lists_phases(1, 1, 1) == 0 and L.ae_plan_lists_phases(4096, 500, 100000) == 1
     fwd, bwd, dw = rotary._kernels(64, 64, True, False)
