@@ -83,15 +83,16 @@ AE_DEVICE int ae_pack_lists(const AePlanCompactionArgs& a, const AeListState& st
 AE_DEVICE void ae_pack_tables(const AePlanCompactionArgs& a, const AeListState& st, const AeListShare sh, int used) {
   for (AeEntries e(sh, a.B, a.max_pages); e.more();) {
     int page[AE_LIST_BATCH], place[AE_LIST_BATCH];
+    bool moves[AE_LIST_BATCH];  // only pages of a row have a place: with none in use, the 0 of an entry behind its row is not below `used` either
     const u32 i0 = e.i;
 #pragma unroll
     for (int j = 0; j < AE_LIST_BATCH; ++j) {
-      page[j] = 0;
-      if (e.more() && (i64)e.c << a.page_log2 < ae_len(a, e.r)) page[j] = a.table[(i64)e.r * a.table_stride + e.c];
+      moves[j] = e.more() && (i64)e.c << a.page_log2 < ae_len(a, e.r);
+      page[j] = moves[j] ? a.table[(i64)e.r * a.table_stride + e.c] : 0;
       e.next(sh.step());
     }
 #pragma unroll
-    for (int j = 0; j < AE_LIST_BATCH; ++j) place[j] = page[j] >= used && page[j] < a.num_pages ? (int)ae_word(st.owner + page[j]) : -1;
+    for (int j = 0; j < AE_LIST_BATCH; ++j) place[j] = moves[j] && page[j] >= used && page[j] < a.num_pages ? (int)ae_word(st.owner + page[j]) : -1;
 #pragma unroll
     for (int j = 0; j < AE_LIST_BATCH; ++j)
       if (place[j] >= 0) page[j] = st.holes ? st.holes[place[j]] : __ldcg(&a.copies[place[j]].dst);

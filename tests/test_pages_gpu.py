@@ -164,6 +164,16 @@ def test_compaction(B, P, longest, spare, groups, seed):
     assert t.tolist() == table and n.tolist() == lens
 
 
+@pytest.mark.parametrize("B,W,N", [(1, 8, 5001), (7, 13, 20), (40, 300, 9000), (3, 2, 20000), (2000, 3, 64)])
+def test_compaction_of_rows_without_tokens(B, W, N):
+    dirt = torch.full((1 << 18,), 0x7f7f7f7f, dtype=torch.int32, device="cuda")  # what a plan's memory may hold before it
+    del dirt
+    c = plan_compaction(ints([0] * B), torch.full((B, W), -9, dtype=torch.int32, device="cuda"), 16, N)
+    c.check()
+    for name, w in ref.compaction([0] * B, [[-9] * W] * B, 16, N).items():
+        assert getattr(c, name).tolist() == w, name
+
+
 def test_compaction_reports():
     for lens, table, code in (([-1, 3], [[0], [1]], 8), ([17, 3], [[0], [1]], 2), ([3, 3], [[9], [1]], 16), ([3, 3], [[-1], [1]], 16)):
         p = plan_compaction(ints(lens), ints(table), 16, 4)
