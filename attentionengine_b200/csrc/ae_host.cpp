@@ -682,7 +682,7 @@ bool pool_of(const Tensor& t, AePagePool& d) {
     d.row_stride = st(2, run);
     if (d.row_stride == run) run *= rows, rows = 1, d.row_stride = run;
   }
-  if (run > 0x7fffffff || rows > 0x7fffffff || run * rows * t.size(1) > 0x7fffffff) return false;
+  if (run > 0x7fffffff || rows > 0x7fffffff || run * rows * t.size(1) > AE_MAX_COPY_UNITS) return false;
   d.slot_stride = st(1, run * rows);
   d.page_stride = st(0, d.slot_stride * t.size(1));
   d.rows = (int)rows; d.run_bytes = (int)run;
@@ -691,7 +691,7 @@ bool pool_of(const Tensor& t, AePagePool& d) {
 
 // `pools`: caches (their native side) and tensors.  False when they or the list do not fit.
 bool copy_pages(uint64_t any, uint64_t runs, const py::list& pools, const Tensor& copies) {
-  if (!good_ints(copies, 2, copies) || copies.size(1) != 4 || (copies.size(0) > 1 && copies.stride(0) != 4) || copies.size(0) > 0x7fffffff ||
+  if (!good_ints(copies, 2, copies) || copies.size(1) != 4 || (copies.size(0) > 1 && copies.stride(0) != 4) || copies.size(0) > AE_MAX_COPY_UNITS ||
       reinterpret_cast<uintptr_t>(copies.data_ptr()) % 16)
     return false;
   std::vector<std::pair<Tensor, Tensor>> all;  // slots, and the scales of a page

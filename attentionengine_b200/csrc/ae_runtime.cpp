@@ -1377,7 +1377,7 @@ int ae_launch_copy_pages(void* module, const AeCopyPagesParams* p, void* stream)
     set_error("module kind does not match the entry point");
     return AE_ERR_UNSUPPORTED;
   }
-  if (p->n_copies < 0 || p->n_pools < 0 || p->n_pools > AE_MAX_COPY_POOLS || p->num_pages < 0 || p->page_size < 1) return AE_ERR_INVALID;
+  if (p->n_copies < 0 || p->n_copies > AE_MAX_COPY_UNITS || p->n_pools < 0 || p->n_pools > AE_MAX_COPY_POOLS || p->num_pages < 0 || p->page_size < 1) return AE_ERR_INVALID;
   if (p->n_copies == 0 || p->n_pools == 0) return AE_OK;
   if (!p->copies || (reinterpret_cast<uintptr_t>(p->copies) & 15)) return AE_ERR_INVALID;
   AeCopyPagesArgs a;
@@ -1388,7 +1388,7 @@ int ae_launch_copy_pages(void* module, const AeCopyPagesParams* p, void* stream)
     const AePagePool& s = p->pools[i];
     AeCopyPool& d = a.pools[i];
     const int64_t slot = (int64_t)s.rows * s.run_bytes;
-    if (!s.base || s.rows < 1 || s.run_bytes < 1 || slot * p->page_size > 0x7fffffff || (s.extra && (s.extra_bytes < 0 || s.extra_bytes % 4 || s.extra_stride % 4 ||
+    if (!s.base || s.rows < 1 || s.run_bytes < 1 || slot * p->page_size > AE_MAX_COPY_UNITS || (s.extra && (s.extra_bytes < 0 || s.extra_bytes % 4 || s.extra_stride % 4 ||
         (reinterpret_cast<uintptr_t>(s.extra) & 3)))) {
       set_error("copy_pages: a pool with rows of at least a byte, pages below 2 GB, extra words of 4 bytes");
       return AE_ERR_INVALID;

@@ -284,6 +284,7 @@ int ae_launch_plan_compaction(void* module, const AePlanCompactionParams* p, voi
  * outside the pools, or more slots than a page has, are passed over.  Destinations are distinct and no entry's source.  Config: reserved[0] bytes of a part, [1] CTAs
  * of an SM, [2] 1: for pools of one row a slot, slots behind each other, alone. */
 #define AE_MAX_COPY_POOLS 48
+#define AE_MAX_COPY_UNITS 0x7fff0000  /* bytes of a page, entries of a list: a loop's step behind the last stays below 2^31 */
 typedef struct AePagePool {
   void* base;            /* [num_pages, page_size, rows, run_bytes], strides in bytes */
   void* extra;           /* 4-byte words that a page has beside its slots, or null */

@@ -273,6 +273,24 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(t[8990], t[8999]) and (t[8500, :63] == 7).all() and (t[8500, 63] == 0).all() and (t[8501] == 0).all()
 
 
+def test_the_largest_pages():
+    """A byte short of the limit, and of bytes, so that a loop's last step comes as near to 2^31 as it can; one more is refused."""
+    t = torch.zeros(2, 0x7fff0001, dtype=torch.uint8, device="cuda")
+    with pytest.raises(ValueError, match="below 2 GB"):
+        copy_pages([t], ints([[0, 1, 1, 0]]))
+    for pool in (t[:, 1:], t[:, None, 1:]):
+        t.zero_()
+        pool[0, ..., -40000:] = 5
+        n = pool.shape[1]
+        copy_pages([pool], ints([[0, 1, n, 0]]))
+        assert torch.equal(pool[0], pool[1]) and t[1, 0] == 0
+    t.zero_()
+    wide = t.view(-1)[:2 * 0x7fff0000].view(2, 0x3fff8000, 2)[:, :, :1]  # bytes that do not lie behind each other
+    wide[0, -40000:] = 6
+    copy_pages([wide], ints([[0, 1, wide.shape[1], 0]]))
+    assert torch.equal(wide[0], wide[1]) and (t.view(-1)[:2 * 0x7fff0000].view(2, 0x3fff8000, 2)[:, :, 1] == 0).all()
+
+
 def test_plans_and_copies_in_a_graph():
     """Captured once, replayed on other lengths and parents; a call on another stream beside it."""
     rng, P, N, B = random.Random(8), 16, 120, 6

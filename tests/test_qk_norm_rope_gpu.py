@@ -359,3 +359,27 @@ def test_refusals():
     import torch.autograd.forward_ad as fwd
     with fwd.dual_level(), pytest.raises(NotImplementedError):
         rope(fwd.make_dual(q, q), k, pos)
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_offsets_beyond_32_bits(inter):
+    """The last of 4.6 GB of heads: as in a call of their own."""
+    rope = QKNormRope(256, interleaved=inter)
+    T, last = 70001, 37
+    q = torch.zeros(T, 128, 256, dtype=torch.bfloat16, device="cuda")
+    k = torch.zeros(T, 1, 256, dtype=torch.bfloat16, device="cuda")
+    gq, gk = torch.zeros_like(q), torch.zeros_like(k)
+    g = gen(31)
+    for t in (q, k, gq, gk):
+        t[-last:] = randn(g, last, *t.shape[1:], dtype=torch.bfloat16)
+    pos = torch.arange(T, device="cuda")
+    own = [t[-last:].clone().requires_grad_() for t in (q, k)]
+    want = rope(*own, pos[-last:])
+    dwant = torch.autograd.grad(want, own, [gq[-last:], gk[-last:]])
+    leaves = [t.requires_grad_() for t in (q, k)]
+    out = rope(*leaves, pos)
+    for a, b in zip(out, want):
+        assert torch.equal(a[-last:], b) and not a[:-last].any()
+    got = torch.autograd.grad(out, leaves, [gq, gk])
+    for a, b in zip(got, dwant):
+        assert torch.equal(a[-last:], b) and not a[:-last].any()
