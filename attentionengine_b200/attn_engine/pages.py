@@ -111,8 +111,9 @@ def plan_forks(parents, seq_lens, block_table, free_pages, free_head, page_size:
     All int32 tensors on one GPU: ``parents``, ``seq_lens``, ``keep_lens`` [B]; ``block_table`` [B, max_pages] of pages below ``num_pages``; ``free_pages`` [n]
     of which the first ``free_head[0]`` are taken.  Whole pages are shared between the rows that have them in common.  A begun page stays with
     one row, and only if none holds it whole; the others take a free page each, in the order of the rows, which ``copy_pages`` fills from
-    ``copies``.  Pages that no row holds any more go back to the free list, lowest on top.  So a sampled prompt is B rows with one parent, a beam
-    search's step its parents, and a cut (speculation that failed) a row that keeps less of itself.
+    ``copies``.  Pages that no row holds any more go back to the free list, lowest on top; where the list does not last, they serve the rows behind it,
+    lowest first.  So a sampled prompt is B rows with one parent, a beam search's step its parents, and a cut (speculation that failed) a row that keeps less
+    of itself.
 
     Rows are shortened through ``keep_lens`` alone: a length that a caller lowers by itself would let ``plan_pages`` put new tokens into a page that other rows hold.
     Pages that something beside the table's rows is to keep (a prefix for later requests) need a row of their own in it.  What does not fit is left

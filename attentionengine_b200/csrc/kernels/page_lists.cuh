@@ -18,6 +18,7 @@ struct AeListState {
   u32 *held, *whole, *begun;  // [words] each, behind each other
   u32* owner;                 // [num_pages] of begun pages: a key, or slots; of moving pages: their place in the list
   int* holes;                 // [num_pages / 2] pages that moving ones take, by place; null: the list's
+  u16* reusing;               // [B] of the forks, in shared memory: rows that copy into pages which the step gives back
 };
 AE_DEVICE u32 ae_word(const u32* p) {  // written by another phase
 #if AE_PHASE == 0

@@ -3,7 +3,8 @@
 // Row i takes over the first n_i = min(keep_i, len of its parent) tokens: n_i / P whole pages, which any number of rows may hold together since nothing
 // is written into a whole page any more, and a begun one of n_i % P tokens.  A begun page stays with one row: none where some row holds it
 // whole, else a row that goes on from itself, else the lowest.  The others take a new page each, in the order of the rows, and an entry {page, new
-// page, n_i % P} of the list of copies.  Pages that rows held before and none holds any more go back on top of the free list, in
+// page, n_i % P} of the list of copies.  New pages are the free list's; behind those, the ones that rows held before and none holds any more, in
+// ascending order (none of them is read by a copy, since a copy's page is one that some row has begun).  The rest of the latter goes back on top of the free list, in
 // ascending order: the taken ones stand in front of free_head, so there is room for them.
 //
 // No count of a page's holders is kept.  Phase 1 says what every row takes over and clears the bitmaps; phase 2 sets the pages' bits (held before, held
@@ -113,14 +114,30 @@ AE_DEVICE void ae_fork_lists(const AePlanForksArgs& a, const AeListState& st, co
   auto freed = [&](int w) { return ae_word(st.held + w) & ~(ae_word(st.whole + w) | ae_word(st.begun + w)); };
   const int share = (a.words + sh.ctas - 1) / sh.ctas, w0 = min(sh.cta * share, a.words), w1 = min(w0 + share, a.words);
   ae_count_bits(a.words, w0, freed, before, all_freed);
-  // page j of those freed stands at top + j, as far as there is room
-  const int got = min(taken, a.n_free - head), top = max(head + got - all_freed, 0), room = head + got - top;
+  // got: taken from the list; reused: of the freed ones, the first; page reused + j of those stands at top + j, as far as there is room
+  const int got = min(taken, a.n_free - head), reused = min(taken - got, all_freed), back = all_freed - reused;
+  const int top = max(head + got - back, 0), room = head + got - top;
+  if (reused > 0)  // the rows that copy into freed pages; read behind a barrier of ae_each_page
+    for (int r = r0, i = order - got; r < r1; ++r)
+      if (copy >> (r - r0) & 1) {
+        if (i >= 0 && i < reused) st.reusing[i] = (u16)r;
+        ++i;
+      }
   ae_each_page(w0, w1, before, freed, [&](int page, bool is, int j) {
-    if (is && j < room) a.free_out[top + j] = page;
+    if (!is) return;
+    if (j >= reused) {
+      if (j - reused < room) a.free_out[top + j - reused] = page;
+      return;
+    }
+    const int r = st.reusing[j];
+    const int4 row = st.rows[r];
+    const AePageCopy e = {row.z, page, row.y & (P - 1), 0};
+    a.copies[got + j] = e;
+    a.table_out[(i64)r * W + (row.y >> a.page_log2)] = page;
   });
   for (u32 i = sh.first(); i < (u32)a.n_free; i += sh.step())
     if ((int)i < top || (int)i >= top + room) a.free_out[i] = a.free_pages[i];
-  u32 bad = all_freed > room ? 4u : 0u;
+  u32 bad = back > room ? 4u : 0u;
   for (int r = r0; r < r1; ++r) {
     const bool copies = copy >> (r - r0) & 1;
     const int mine = order;
@@ -129,10 +146,10 @@ AE_DEVICE void ae_fork_lists(const AePlanForksArgs& a, const AeListState& st, co
     const int4 row = st.rows[r];
     int n = row.y;
     const int part = n & (P - 1);
-    if (row.z >= 0) {
+    if (row.z >= 0 && !(copies && mine >= got && mine < got + reused)) {
       int page = row.z;
       if (copies) {
-        const bool there = head + mine < a.n_free;
+        const bool there = mine < got;
         page = there ? a.free_pages[head + mine] : -1;
         AePageCopy e = {row.z, page, part, 0};
         if (!ae_in_pool(page, a.num_pages)) {  // no page: the row ends with its whole ones
@@ -160,6 +177,10 @@ AE_DEVICE void ae_fork_lists(const AePlanForksArgs& a, const AeListState& st, co
 extern "C" __global__ void __launch_bounds__(AE_LIST_THREADS) ae_plan_forks(const __grid_constant__ AePlanForksArgs a) {
   const AeListShare sh = {(int)blockIdx.x, (int)gridDim.x};
   AeListState st;
+#if AE_PHASE == 0 || AE_PHASE == 3
+  __shared__ u16 reusing[4096];
+  st.reusing = reusing;
+#endif
 #if AE_PHASE == 0
   extern __shared__ uint4 smem_raw[];
   st.rows = (int4*)smem_raw;

@@ -236,9 +236,9 @@ int ae_launch_cache8_decode(void* module, const AeCache8DecodeParams* p, void* s
 
 /* Pages of a step in which row i of B goes on from the first keep_lens[i] tokens of row parents[i] (all of them without keep_lens; -1: the row
  * ends).  Whole pages are shared; a begun page that another row holds too is copied: the row takes the next of free_pages behind *free_head, in
- * the order of the rows, and `copies` gets {page, new page, slots, 0} (unused entries at the end all 0).  Pages that no row holds any more go on
- * top of the free list, in ascending order.  Nothing that is read is changed.  *status receives 0 or bits: 1 the free pages ran out (such
- * a row ends with its whole pages), 2 a length beyond the table, 4 more pages came back than had been taken (the rest is left out), 8 a parent that is no row, a negative
+ * the order of the rows (behind the last of them, the lowest page that no row holds any more), and `copies` gets {page, new page, slots, 0} (unused entries at
+ * the end all 0).  Pages that no row holds any more go on top of the free list, in ascending order.  Nothing that is read is changed.  *status receives 0 or bits:
+ * 1 the free pages and those that came back ran out (such a row ends with its whole pages), 2 a length beyond the table, 4 more pages came back than had been taken (the rest is left out), 8 a parent that is no row, a negative
  * length or more tokens kept than there are, 16 a page outside the pool.
  * Where ae_plan_lists_phases(B, max_pages, num_pages) is 0, one launch with a module of all phases (config: reserved[1] = 0, shared memory for 1024 rows and 16384
  * pages: 16 B + 12 words + 6 num_pages + 16 bytes, with a word for 32 pages in groups of four); else modules of the phases 1, 2, 3 (reserved[1]), one behind the other with the same parameters.  Here and below. */
