@@ -5,8 +5,9 @@
 // for the pairs (a, b) = (i, i + R / 2), or (2i, 2i + 1); the D - R values behind are z.  Backward, from the gradient g of y:
 //   dz_a = m (g_a cos + g_b sin),  dz_b = m (g_b cos - g_a sin),  dw = sum over tokens and heads of dz n,
 //   dx = (mean(x^2) + eps)^-1/2 (dz w - n mean(dz w n)).
-// Angles: p f / 2 pi is wanted modulo 1, so a frequency is held as its 64-bit fraction of a turn and the product wraps around by itself: exact for any
-// position, where an fp32 angle is off by 0.03 at position 500000.
+// Angles: p f / 2 pi is wanted modulo 1, so a frequency is held as its 64-bit fraction of a turn and the product wraps around by itself.  That is off by
+// p 2^-65 of a turn (the frequency's rounding), and by 2^-26 of one for the angle's fp32, which is the larger part up to p = 2^39; beyond, 64-bit positions lose
+// their angle bit by bit (an eighth of a turn at 2^62).  An fp32 product is off by 0.03 radians at position 500000.
 //
 // A team of D / 16 threads has a head, each thread 16 values that hold both halves of its 8 pairs, so that the rotation needs no exchange and the norm
 // log2(D / 16) shuffles.  A warp has a token, or where tokens are few a share of its heads: its lanes make the token's cosines and sines once and fold
