@@ -27,14 +27,14 @@ def turns_of(frequency: float) -> int:
     return round((t - math.floor(t)) * 2 ** 64) % 2 ** 64
 
 
-# of each kernel: warps of a CTA, heads of a team on their way together (the forward takes four, two or one itself), CTAs of an SM
-SHAPES = ((4, 4, 4), (8, 1, 3), (32, 1, 1))
+SHAPES = ((4, 4), (8, 3), (32, 1))  # of each kernel: warps of a CTA, CTAs of an SM
+BWD_HEADS = 1  # of a team on their way together in the backward (the forward takes four, two or one)
 
 
 def _defines(D: int, R: int, norm: bool, interleaved: bool, which: int) -> dict:
-    warps, u, ctas = SHAPES[which]
-    return {"AE_D": D, "AE_R": R, "AE_NORM": int(norm), "AE_NEXT": int(interleaved), "AE_ROPE_KERNEL": which, "AE_ROPE_WARPS": warps, "AE_ROPE_U": u,
-            "AE_ROPE_CTAS": ctas}
+    warps, ctas = SHAPES[which]
+    return {"AE_D": D, "AE_R": R, "AE_NORM": int(norm), "AE_NEXT": int(interleaved), "AE_ROPE_KERNEL": which, "AE_ROPE_WARPS": warps,
+            "AE_ROPE_CTAS": ctas, **({"AE_ROPE_U": BWD_HEADS} if which == 1 else {})}
 
 
 @functools.lru_cache(maxsize=None)
@@ -42,9 +42,7 @@ def _kernels(D: int, R: int, norm: bool, interleaved: bool):
     out = []
     for i, name in enumerate(("ae_qk_rope_fwd", "ae_qk_rope_bwd", "ae_qk_rope_dw")):
         cfg = rt.KernelConfig(kind=rt.KIND_QK_ROPE, head_dim=D, threads=32 * SHAPES[i][0])
-        cfg.reserved[0] = R
-        for j in range(3):
-            cfg.reserved[1 + j] = SHAPES[min(i, 1)][j]  # the sums: the backward's
+        cfg.reserved[1], cfg.reserved[3] = SHAPES[min(i, 1)]  # the sums: the backward's
         out.append(rt.compile_module(rt.kernel_source("qk_norm_rope.cuh", defines=_defines(D, R, norm, interleaved, i)), name, cfg))
     return tuple(out)
 

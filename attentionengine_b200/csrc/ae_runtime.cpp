@@ -1473,7 +1473,7 @@ int ae_launch_qk_rope(void* module, const AeQkRopeParams* p, void* stream) {
     set_error("norm and rotation: too many heads for one launch");
     return AE_ERR_INVALID;
   }
-  // Inputs that L2 does not hold are asked for early: 16029 tokens of 40 heads of 128 dims (118 MB) 42.9 -> 39.3 us; 3333 of 32 heads of 64 dims, 14 MB
+  // Inputs that L2 does not hold are asked for early: 11542 tokens of 40 heads of 128 dims (118 MB) 42.9 -> 39.3 us; 3333 of 32 heads of 64 dims, 14 MB
   // in L2 from the call before, 7.0 -> 7.4.
   a.prefetch = both && a.slices[0] == 1 && T * (a.H[0] + a.H[1]) * D * 2 > (48 << 20);
   // Queries' and keys' CTAs in proportion to their work: a token costs as much as two heads beside its own.  16384 tokens of 32 and 8 heads, forward and backward:

@@ -4,10 +4,13 @@
 // stores.  HBM-bound once a few hundred parts are under way: 1500 pages of 64 tokens, 8 heads of 128 dims, in four layers (1.5 GB
 // in and out) 251 us, 6.1 TB/s; 96 begun ones in eight layers (96 MB) 18.4 us, 5.2 TB/s.  Eight reads a thread in 256 of them, 257 and 20.8; four, 283 and 25; parts of
 // 8 KB, 275 and 25.5, of 64 KB, 248 and 20.2.  Which page goes where and how many slots stands on the device; a list ends at
-// its first entry without slots, which every CTA looks for itself (its length is next to nothing beside the pages that it names).  Entries that name a
-// page outside the pool, or more slots than a page has, are passed over.
+// its first entry without slots, which every CTA looks for itself, 256 entries a step, before it copies anything: 2 to 5 ns an entry.  That is next to nothing for a
+// list of 1500 pages of 64 KB, and the larger part for long lists of small pages: in a graph, 1500 entries of 1 KB 5.9 us, 16300 of them 86 us, 16300 of 16 KB (534 MB) 162 us, in
+// eight pools (4.3 GB) 757 us, 5.6 TB/s.  Entries that name a page outside the pool, or more slots than a page has, are passed over.
+// An access is as wide as a slot's bytes and place allow (16, 4, 2 or 1), in slots that lie behind each other too, so odd slots take up to 16 times the
+// instructions.
 // A build for pools whose slots lie behind each other (AE_COPY_RUNS), and one for others, whose places take registers of their own: 1200 pages whose 8 heads lie
-// one behind the other 27.5 us, 5.7 TB/s (37 with both in one build, 85 without reads in front of the writes).  Seven CTAs an SM at least: left to the compiler 173
+// one behind the other 27.5 to 28.5 us, 5.5 TB/s (37 with both in one build, 85 without reads in front of the writes).  Seven CTAs an SM at least: left to the compiler 173
 // registers, the begun pages 21.4 us.
 // Expects AE_COPY_THREADS, AE_COPY_UNROLL (reads of a thread in front of its writes), AE_COPY_RUNS.
 

@@ -3,7 +3,7 @@
 //
 // Phase 1 clears the bitmaps and the slots of begun pages; phase 2 sets the pages' bits (held whole, begun) and takes the maximum of a begun page's slots; in
 // phase 3 one running sum over the pages serves both sides: page x is hole number x - (in use below x), or mover number (in use below x) - (in use below
-// U), and holes write the list's second number, moving pages the others; phase 4 writes the tables.
+// U), and holes write the list's second number, moving pages the others; phase 4 writes the tables, from the places that phase 3 wrote.
 
 AE_DEVICE int ae_len(const AePlanCompactionArgs& a, int r) {  // in the table
   return (int)min((i64)max(a.lens[r], 0), (i64)a.max_pages << a.page_log2);

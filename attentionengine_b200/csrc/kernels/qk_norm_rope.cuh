@@ -14,7 +14,7 @@
 // them (forward: with the weights) into two factors a value, which pass through shared memory.  Arithmetic on two fp32 values an instruction.
 //
 // Bound by HBM for long calls: everything is read and written once.  What that takes is bytes on their way, and a warp has four chains of reads in a row
-// (position, two batches of queries, keys): the forward asks L2 for a token's heads before anything else.  In a graph, 40 heads of 128 dims, bf16: 16029 tokens (236 MB) 39.3 us,
+// (position, two batches of queries, keys): the forward asks L2 for a token's heads before anything else.  In a graph, 40 heads of 128 dims, bf16: 11542 tokens (236 MB) 39.3 us,
 // 6.0 TB/s (42.9 without that request; 44 to 45 with the factors made by every team for itself; 79 with factors at 64-byte steps, four-fold bank conflicts;
 // 84 with whole CTAs a token, whose barriers leave nothing on its way); forward and backward of 16384 tokens (839 MB) 145 us.  64 tokens, one a request: 2.6.
 // The backward is joined work of 24 warps an SM with one head a team on its way (80 registers): 88 us, 5.7 TB/s; a ring of copies through shared memory, two heads on their

@@ -301,8 +301,8 @@ int ae_launch_copy_pages(void* module, const AeCopyPagesParams* p, void* stream)
 /* ---- norm and rotation of query and key heads ------------------------------------------------
  * The module's kernel name selects what is launched: "ae_qk_rope_fwd" writes y from x; "ae_qk_rope_bwd" the gradients of x from those of y
  * (g), and with `workspace` (ae_qk_rope_workspace(module) bytes) the sums that "ae_qk_rope_dw", launched behind it with the same
- * parameters, turns into the weights' gradients.  Config: head_dim, reserved[0] rotary dims, and of the forward or the
- * backward (the sums: the backward) [1] warps of a CTA, [2] heads of a thread team on their way together, [3] CTAs of an SM.  Index 0: queries, 1: keys (H 0: none). */
+ * parameters, turns into the weights' gradients.  Config: head_dim, and of the forward or the backward (the sums: the backward) reserved[1] warps of a CTA, [3] CTAs
+ * of an SM.  Index 0: queries, 1: keys (H 0: none). */
 typedef struct AeQkRopeParams {
   const void* x[2];       /* [B, S, H, D] 16-bit, rows 16-byte aligned */
   const void* g[2];
