@@ -56,7 +56,7 @@ class QKNormRope:
 
     Everything is computed in fp32 and rounded once, angles in 64-bit fixed point.  With the frequencies as 64-bit floats, an angle is off by 2^-26 of a turn, as any in fp32, and
     by 2^-65 of one for each position: nothing beside the former up to position 2^39 (so for every int32), an eighth of a turn at 2^62.  A row's squares are summed
-    in fp32, so values beyond 1e18 make it overflow as they do in any fp32 norm."""
+    in fp32, so values beyond 1e18 make it overflow as they do in any fp32 norm: finite ones become 0."""
 
     def __init__(self, head_dim: int, rotary_dim: int | None = None, base: float = 10000.0, inv_freq=None, interleaved: bool = False, norm: bool = True,
                  eps: float = 1e-6, rotary_scale: float = 1.0):

@@ -25,6 +25,9 @@
 #define AE_TPR (AE_D / 16)      // threads of a team
 #define AE_TEAMS (32 / AE_TPR)  // teams of a warp
 #define AE_PAIRS (AE_R / 2)
+// The forward's products come before the norm's factor.  That is 0 for values whose squares' sum is infinite, and must find them finite: so a power of two
+// goes from the factors of the values to the norm's, room for weights times rotary_scale up to 180.
+#define AE_ROOM (AE_NORM ? 256.f : 1.f)
 
 // cos and sin of the turns that position p makes.
 AE_DEVICE float2 ae_turn(u64 per_position, i64 p) {
@@ -183,7 +186,7 @@ AE_DEVICE void ae_rope_batch(const AeQkRopeArgs& a, const u64 (&f)[2][8], bool r
     u64 sum = ae_mul2(z[0], z[0]);
 #pragma unroll
     for (int k = 1; k < 8; ++k) sum = ae_fma22(z[k], z[k], sum);
-    const float r = rsqrtf(fmaf(ae_team_sum(ae_sum2(sum)), 1.f / AE_D, a.eps));
+    const float r = rsqrtf(fmaf(ae_team_sum(ae_sum2(sum)), 1.f / AE_D, a.eps)) * AE_ROOM;
 #pragma unroll
     for (int k = 0; k < 8; ++k) o[k] = ae_mul2(o[k], ae_pack2f(r, r));
 #endif
@@ -234,7 +237,7 @@ AE_DEVICE void ae_rope_fwd(const AeQkRopeArgs& a, AeRopeSmem& sm) {
   }
   for (int i = threadIdx.x; i < 2 * AE_D; i += AE_ROPE_THREADS) {
     const int kind = i / AE_D, d = i % AE_D, place = ae_place(d);
-    const float w = ae_weight(a, kind, d);
+    const float w = ae_weight(a, kind, d) * (1.f / AE_ROOM);
     sm.w[kind][place] = w;
     if (d >= AE_R)
 #pragma unroll
